@@ -79,6 +79,21 @@ class RangeDecoderState(C.Structure):
     _fields_ = [("low", C.c_uint64), ("range", C.c_uint64), ("code", C.c_uint64), ("pos", C.c_uint64)]
 
 
+DTL_F32, DTL_BF16, DTL_F16 = 0, 1, 2
+
+
+class Logits(C.Structure):
+    """dtl_logits: rows of logits in device memory, `stride` elements apart."""
+
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int), ("rows", sz), ("vocab", sz), ("stride", sz)]
+
+
+class Teacher(C.Structure):
+    """dtl_teacher: k ids and log probabilities per row in device memory."""
+
+    _fields_ = [("ids", C.c_void_p), ("id_bytes", C.c_int), ("log_probs", f32p), ("k", sz), ("rest", C.c_int)]
+
+
 class KernelStat(C.Structure):
     _fields_ = [
         ("name", C.c_char * 32),
@@ -121,6 +136,20 @@ _SIGS = {
     "dtl_symbol_ranges_static": (C.c_int, [C.c_void_p, sz, sz, C.c_void_p, sz, C.c_void_p, C.c_void_p,
                                            C.c_void_p, C.c_void_p, C.c_void_p]),
     "dtl_status_from_bits": (C.c_int, [C.c_int]),
+    "dtl_token_scores_scratch": (sz, [sz, sz, sz]),
+    "dtl_token_scores": (C.c_int, [C.POINTER(Logits), C.c_void_p, C.c_int, C.c_float, sz, C.c_void_p, C.c_void_p,
+                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, sz, C.c_void_p]),
+    "dtl_token_scores_backward": (C.c_int, [C.POINTER(Logits), C.c_void_p, C.c_int, C.c_float, C.c_void_p, C.c_void_p,
+                                            C.c_void_p, C.c_void_p, C.c_void_p, sz, C.c_void_p]),
+    "dtl_distill_scratch": (sz, [sz, sz]),
+    "dtl_distill": (C.c_int, [C.POINTER(Logits), C.POINTER(Teacher), C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, sz,
+                              C.c_void_p]),
+    "dtl_distill_backward": (C.c_int, [C.POINTER(Logits), C.POINTER(Teacher), C.c_float, C.c_void_p, C.c_void_p,
+                                       C.c_void_p, sz, C.c_void_p]),
+    "dtl_distill_step": (C.c_int, [C.POINTER(Logits), C.POINTER(Teacher), C.c_float, C.c_void_p, C.c_void_p, C.c_void_p,
+                                   sz, C.c_void_p, sz, C.c_void_p]),
+    "dtl_session_token_scores": (C.c_int, [C.c_void_p, sz, sz, u32p, C.c_float, sz, f32p, f32p, C.POINTER(C.c_int32),
+                                           f32p]),
     "dtl_range_encoder_new": (C.c_int, [vpp]),
     "dtl_range_encode": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64]),
     "dtl_range_encoder_finish": (C.c_int, [C.c_void_p, u8p, sz, C.POINTER(sz)]),

@@ -36,6 +36,11 @@ SOURCES = [
     "dtl_codec.cpp",
 ]
 
+# Operators with arithmetic of their own, outside the reference's contract
+# that csrc is held to: hardware 2^x and fused multiply-adds.
+SCORES_SRC = PKG / "csrc_scores"
+SCORES_SOURCES = ["dtl_scores.hip"]
+
 NUMERIC_FLAGS = [
     "-ffp-contract=off",
     "-fno-fast-math",
@@ -82,9 +87,9 @@ def build_library(verbose: bool = False, jobs: int = 0) -> Path:
     tmp = OUT_DIR / (LIB_NAME + ".tmp")
     common = [hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", *NUMERIC_FLAGS,
               "-Wno-unused-result"]
-    objs = [OUT_DIR / (Path(s).stem + ".o") for s in SOURCES]
-    cmds = [common + EXTRA_FLAGS.get(s, []) + ["-c", str(CSRC / s), "-o", str(o)]
-            for s, o in zip(SOURCES, objs)]
+    paths = [CSRC / s for s in SOURCES] + [SCORES_SRC / s for s in SCORES_SOURCES]
+    objs = [OUT_DIR / (p.stem + ".o") for p in paths]
+    cmds = [common + EXTRA_FLAGS.get(p.name, []) + ["-c", str(p), "-o", str(o)] for p, o in zip(paths, objs)]
     jobs = jobs or min(len(cmds), os.cpu_count() or 1, 16)
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         for f in [ex.submit(_run, c, verbose) for c in cmds]:

@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "../../include/detllm.h"
+#include "../csrc_scores/dtl_scores.h"
 #include "dtl_device.h"
 #include "dtl_gguf.h"
 #include "dtl_sha256.h"
@@ -775,6 +776,10 @@ struct dtl_session {
   size_t wide_rows = 0;  // 0: none (DETLLM_NO_WIDE_LANES)
   // Device bytes that lanes past the first may still take (DETLLM_LANE_MEMORY).
   size_t lane_budget = SIZE_MAX;
+  // dtl_session_token_scores: device memory for its tokens, scratch and results,
+  // grown by the calls that need more.
+  Arena score_arena;
+  uint8_t* score_mem = nullptr;
   // Pinned slices and their events for large results (copy_out), set up by
   // the first such copy.
   uint8_t* out_pin = nullptr;
@@ -1969,6 +1974,58 @@ int dtl_forward_ranges(dtl_session* s, const uint32_t* tokens, size_t n, size_t 
   // the chunks still in flight, oldest first
   for (size_t c = nchunks > (size_t)nl ? nchunks - nl : 0; c < nchunks; c++)
     if (int st = collect((int)(c % nl))) return st;
+  s->prof.collect();
+  return DTL_OK;
+}
+
+int dtl_session_token_scores(dtl_session* s, size_t first, size_t n, const uint32_t* tokens, float temperature,
+                             size_t top, float* log_probs, float* entropy, int32_t* top_ids, float* top_log_probs) {
+  if (!s || (log_probs && !tokens) || (top && (!top_ids || !top_log_probs))) return DTL_ERR_INVALID_ARGUMENT;
+  if (!(temperature >= kScoreMinTemperature && temperature <= kScoreMaxTemperature)) return DTL_ERR_INVALID_ARGUMENT;
+  const size_t V = s->m->vocab;
+  Lane& L = *s->ln;
+  if (n == 0 || n > L.rows_valid || first > L.rows_valid - n) return DTL_ERR_SHAPE;
+  if (V > (size_t)kScoreMaxVocab) return DTL_ERR_CDF_TOO_MANY_SYMBOLS;
+  if (top > (size_t)kScoreMaxTop || top > V) return DTL_ERR_SHAPE;
+  if (log_probs)
+    for (size_t i = 0; i < n; i++)
+      if (tokens[i] >= V) return DTL_ERR_CDF_SYMBOL_OUT_OF_RANGE;
+  HIP_TRY(hipSetDevice(s->m->device));
+  // tokens, log probabilities, entropy, alternatives' ids and log
+  // probabilities, then the scratch
+  const size_t scratch = score_scratch_bytes(n, V, top);
+  const size_t o_ids = 12 * n, o_lps = o_ids + 4 * n * top, o_scratch = (o_lps + 4 * n * top + 255) & ~(size_t)255;
+  if (s->score_arena.bytes() < o_scratch + scratch) {
+    s->score_mem = nullptr;
+    s->score_arena.release();
+    const int st = s->score_arena.alloc(&s->score_mem, o_scratch + scratch);
+    if (st) return st;
+  }
+  uint8_t* mem = s->score_mem;
+  if (log_probs) HIP_TRY(hipMemcpyAsync(mem, tokens, 4 * n, hipMemcpyHostToDevice, L.stream));
+  ScoreArgs a{};
+  a.z = L.logits + first * V;
+  a.stride = V;
+  a.rows = n;
+  a.dtype = DTL_F32;
+  a.vocab = (int)V;
+  a.tokens = log_probs ? mem : nullptr;
+  a.temperature = temperature;
+  a.top = (int)top;
+  a.log_probs = log_probs ? (float*)(mem + 4 * n) : nullptr;
+  a.entropy = (float*)(mem + 8 * n);
+  a.top_ids = (int32_t*)(mem + o_ids);
+  a.top_log_probs = (float*)(mem + o_lps);
+  a.scratch = mem + o_scratch;
+  s->prof.timed(L.stream, "token_scores", (double)n * V * 4.0, 0.0, [&] { launch_token_scores(a, L.stream); });
+  HIP_TRY(hipGetLastError());
+  if (log_probs) HIP_TRY(hipMemcpyAsync(log_probs, a.log_probs, 4 * n, hipMemcpyDeviceToHost, L.stream));
+  if (entropy) HIP_TRY(hipMemcpyAsync(entropy, a.entropy, 4 * n, hipMemcpyDeviceToHost, L.stream));
+  if (top) {
+    HIP_TRY(hipMemcpyAsync(top_ids, a.top_ids, 4 * n * top, hipMemcpyDeviceToHost, L.stream));
+    HIP_TRY(hipMemcpyAsync(top_log_probs, a.top_log_probs, 4 * n * top, hipMemcpyDeviceToHost, L.stream));
+  }
+  HIP_TRY(hipStreamSynchronize(L.stream));
   s->prof.collect();
   return DTL_OK;
 }

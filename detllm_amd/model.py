@@ -13,7 +13,7 @@ from __future__ import annotations
 import ctypes as C
 import enum
 from dataclasses import dataclass
-from typing import Callable, Iterable, Optional, Sequence
+from typing import Callable, Iterable, NamedTuple, Optional, Sequence
 
 import numpy as np
 
@@ -157,6 +157,36 @@ class F32Llama:
         return b"".join(parts)
 
 
+    def scores_for_tokens_chunked(self, tokens: Sequence[int], chunk_size: int, top: int = 0,
+                                  temperature: float = 1.0) -> "TokenScores":
+        """What the model says of a text: at each position the log probability of
+        the token that follows (0 behind the last), the entropy, and the `top`
+        alternatives (a teacher's targets).  No counterpart in the reference."""
+        toks = _tokens(tokens)
+        if toks.size == 0 or chunk_size <= 0 or toks.size > self.config.context_length:
+            raise DetllmError(int(ModelError.Shape), "scores_for_tokens_chunked")
+        chunk = min(int(chunk_size), toks.size)
+        follow = np.append(toks[1:], np.uint32(0))
+        with Session(self, toks.size, chunk) as s:
+            parts = []
+            for p in range(0, toks.size, chunk):
+                s.forward_chunk(toks[p : p + chunk], p)
+                parts.append(s.token_scores(follow[p : p + chunk], top=top, temperature=temperature))
+        got = TokenScores(*(np.concatenate(a) for a in zip(*parts)))
+        got.log_probs[-1] = 0.0
+        return got
+
+
+class TokenScores(NamedTuple):
+    """dtl_session_token_scores: per row the log probability of its token, the
+    entropy, and the ids and log probabilities of the largest logits."""
+
+    log_probs: np.ndarray
+    entropy: np.ndarray
+    top_ids: np.ndarray
+    top_log_probs: np.ndarray
+
+
 class Session:
     """KvCache + ForwardWorkspace + RopeTables of one decode stream (device)."""
 
@@ -289,6 +319,24 @@ class Session:
             "dtl_forward_ranges",
         )
         return cum[:n], freq[:n], total[:n]
+
+    def token_scores(self, tokens: Sequence[int], first: int = 0, top: int = 0,
+                     temperature: float = 1.0) -> TokenScores:
+        """Log probability of tokens[i] under row first + i of the last forward,
+        the row's entropy and its `top` alternatives, p = softmax(logits / temperature)."""
+        toks = _tokens(tokens)
+        n = toks.size
+        lp = np.empty(n, np.float32)
+        entropy = np.empty(n, np.float32)
+        ids = np.empty((n, top), np.int32)
+        lps = np.empty((n, top), np.float32)
+        check(
+            lib.dtl_session_token_scores(self._h, first, n, ptr(toks, C.c_uint32), temperature, top,
+                                         ptr(lp, C.c_float), ptr(entropy, C.c_float), ptr(ids, C.c_int32),
+                                         ptr(lps, C.c_float)),
+            "dtl_session_token_scores",
+        )
+        return TokenScores(lp, entropy, ids, lps)
 
     def cdf(self, row: int = 0, tail_symbols: int = 0):
         """logits_to_cdf_* of one row: (freq[u32], cum[u64], total)."""

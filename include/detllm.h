@@ -229,6 +229,15 @@ int dtl_forward_ranges(dtl_session *session, const uint32_t *tokens, size_t n, s
                        size_t n_sym, const uint32_t *rows, const uint32_t *symbols,
                        size_t tail_symbols, uint64_t *cum, uint32_t *freq, uint64_t *total);
 
+/* dtl_token_scores (below) of rows [first, first+n) of the session's last
+ * logits: log_probs[i] of tokens[i] (< vocab), entropy[i], and the `top`
+ * alternatives of each row into top_ids / top_log_probs[n][top].  Results on
+ * the host; log_probs (then tokens), entropy and, with top 0, the alternatives
+ * may be NULL. */
+int dtl_session_token_scores(dtl_session *session, size_t first, size_t n, const uint32_t *tokens,
+                             float temperature, size_t top, float *log_probs, float *entropy,
+                             int32_t *top_ids, float *top_log_probs);
+
 /* logits_to_cdf_with_scratch / _with_byte_escapes (cdf.rs:52-106): the
  * full table for one row; freq and cum hold vocab + tail_symbols entries. */
 int dtl_cdf(dtl_session *session, size_t row, size_t tail_symbols, uint32_t *freq, uint64_t *cum,
@@ -261,6 +270,94 @@ int dtl_symbol_ranges_static(const float *logits, size_t rows, size_t vocab, con
                              int *status_bits, void *stream);
 /* The dtl_status a device status word of dtl_symbol_ranges_static reports. */
 int dtl_status_from_bits(int bits);
+
+/* ---- scores of logits rows, and distillation ------------------------------
+ * No counterpart in the reference.  What rows of logits say of given tokens
+ * (log probability: -log2 of it is the ideal code length; entropy; the most
+ * likely alternatives), and the loss that moves a smaller model towards such
+ * alternatives, with gradients.  Their arithmetic is their own (32-bit sums in
+ * a fixed order, hardware 2^x); no payload depends on them.  A row's results
+ * are the same bits whatever the other rows and however many there are.
+ *
+ * Pointers are device memory of the current device, the work is enqueued on
+ * `stream` (a hipStream_t; NULL is the default stream) without waiting for it,
+ * and nothing is allocated, so the calls can be captured into a graph.
+ * `scratch` (16-byte aligned) belongs to one call at a time: calls, or captured
+ * graphs, that may overlap need one each.  Errors are found on the host before
+ * anything is enqueued; 0 rows are no error and enqueue nothing. */
+typedef enum { DTL_F32 = 0, DTL_BF16 = 1, DTL_F16 = 2 } dtl_dtype;
+
+/* logits[rows][vocab], row i at data + i * stride elements; vocab <= 2^18,
+ * rows <= 2^24, any stride >= vocab, data aligned to an element. */
+typedef struct dtl_logits {
+    const void *data;
+    int dtype;
+    size_t rows, vocab, stride;
+} dtl_logits;
+
+/* Scratch bytes of dtl_token_scores (0 for many rows). */
+size_t dtl_token_scores_scratch(size_t rows, size_t vocab, size_t top);
+/* With p = softmax(z / temperature) of a row: log p of tokens[row] (token_bytes
+ * 4 or 8: int32 or int64), the entropy -sum p log p, and the `top` (<= 128,
+ * <= vocab) largest logits, descending, ties to the lower index, with their
+ * log p in top_ids / top_log_probs[rows][top].  log_probs, entropy and stats may
+ * be NULL; tokens may be NULL if log_probs is.  temperature is in [1e-4, 1e4].
+ *   token < 0: padding, log_prob 0.  token >= vocab: NaN.
+ *   A logit of -inf is masked: log p -inf, and no alternative; where fewer than
+ *   `top` remain the ids behind them are -1 with log p -inf.
+ *   Every logit masked: log_prob -inf, entropy 0, no alternatives.
+ *   A NaN or +inf among the logits: NaN for the row (padding's 0 stays), ids -1.
+ * stats ([rows][2] floats) is what dtl_token_scores_backward needs. */
+int dtl_token_scores(const dtl_logits *logits, const void *tokens, int token_bytes, float temperature,
+                     size_t top, float *log_probs, float *entropy, float *stats, int32_t *top_ids,
+                     float *top_log_probs, void *scratch, size_t scratch_bytes, void *stream);
+/* The gradient of the logits (their type, row i at grad + i * grad_stride
+ * elements; may be the logits themselves at the same stride) for the gradients
+ * of log_probs and of entropy, either of which may be NULL.  stats and entropy
+ * are the forward's.  Zero in rows whose gradients are zero (padding's is) or
+ * whose logits are all masked, whatever else they hold; NaN in rows that gave
+ * NaN. */
+int dtl_token_scores_backward(const dtl_logits *logits, const void *tokens, int token_bytes,
+                              float temperature, const float *stats, const float *entropy,
+                              const float *grad_log_probs, const float *grad_entropy, void *grad,
+                              size_t grad_stride, void *stream);
+
+/* A teacher's alternatives: per row k (1 to 256) ids (id_bytes 4 or 8) and
+ * their log probabilities v at the loss's temperature, as dtl_token_scores
+ * gives them.  A slot with an id below 0 or a v of -inf is empty; ids that
+ * occur twice count twice.  rest 0: p = softmax(v) over the row's slots.  rest 1:
+ * p = e^v, and what they leave of 1 is the teacher's mass outside the list. */
+typedef struct dtl_teacher {
+    const void *ids;
+    int id_bytes;
+    const float *log_probs;
+    size_t k;
+    int rest;
+} dtl_teacher;
+
+/* Scratch bytes of dtl_distill and dtl_distill_step. */
+size_t dtl_distill_scratch(size_t rows, size_t vocab);
+/* loss[row] = T^2 (sum_k p_k (log p_k - log q[id_k]) + rest (log rest - log
+ * q_rest)), q = softmax(logits / T) and q_rest = 1 - q over the listed ids; the
+ * last term only with teacher->rest and where a logit outside the list is not
+ * masked.  A row without slots in use: 0, and its logits are not read.  A
+ * masked logit that the teacher gives mass to: +inf.  An id >= vocab, a v that
+ * is NaN or +inf, a logit that is NaN or +inf: NaN.  stats ([rows][5] floats,
+ * may be NULL) is what dtl_distill_backward needs. */
+int dtl_distill(const dtl_logits *logits, const dtl_teacher *teacher, float temperature, float *loss,
+                float *stats, void *scratch, size_t scratch_bytes, void *stream);
+/* The gradient of the logits (as in dtl_token_scores_backward) for the gradient
+ * of each row's loss.  Zero in rows whose gradient is zero, that have no slot in
+ * use or whose logits are all masked. */
+int dtl_distill_backward(const dtl_logits *logits, const dtl_teacher *teacher, float temperature,
+                         const float *stats, const float *grad_loss, void *grad, size_t grad_stride,
+                         void *stream);
+/* Both in one call for row weights known beforehand (NULL: ones): loss[row] is
+ * weights[row] times dtl_distill's, grad the gradient of their sum.  Reads the
+ * logits from memory once.  A row of weight 0 is not read: loss 0, gradient 0. */
+int dtl_distill_step(const dtl_logits *logits, const dtl_teacher *teacher, float temperature,
+                     const float *weights, float *loss, void *grad, size_t grad_stride, void *scratch,
+                     size_t scratch_bytes, void *stream);
 
 /* logits_to_cdf / logits_to_symbol_range on caller logits (host memory):
  * uploads them and runs the same device kernels (cdf.rs:47-199). */
