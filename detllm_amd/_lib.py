@@ -91,7 +91,7 @@ class Logits(C.Structure):
 class Teacher(C.Structure):
     """dtl_teacher: k ids and log probabilities per row in device memory."""
 
-    _fields_ = [("ids", C.c_void_p), ("id_bytes", C.c_int), ("log_probs", f32p), ("k", sz), ("rest", C.c_int)]
+    _fields_ = [("ids", C.c_void_p), ("id_bytes", C.c_int), ("log_probs", C.c_void_p), ("k", sz), ("rest", C.c_int)]
 
 
 class KernelStat(C.Structure):

@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kRowThreads = 512;
 constexpr int kRowWaves = kRowThreads / 64;
+constexpr int kPartThreads = 256;
 constexpr int kPer = kScoreSeg / 64;  // logits a lane holds of a segment
 constexpr int kKeysPerThread = kScoreMaxSegs / kRowWaves;
 constexpr double kLog2E = 1.4426950408889634074;
@@ -111,14 +112,18 @@ __device__ __forceinline__ packet load_packet(const char* row, int j, int V) {
   return p;
 }
 
-template <int DT>
+// ONCE: past the caches' usual policy, for logits that do not fit the 256 MB
+// memory-side cache anyway (see read_once).
+template <int DT, bool ONCE>
 __device__ __forceinline__ void load_seg(Seg<DT>& s, const char* row, int seg, int lane, int V) {
   constexpr int n = Type<DT>::kInPacket;
   const int at = seg * kScoreSeg + lane * n;
   if (seg * kScoreSeg + kScoreSeg <= V) {
 #pragma unroll
-    for (int q = 0; q < Type<DT>::kPackets; q++)
-      s.w[q] = *reinterpret_cast<const typename Type<DT>::mem*>(row + (size_t)(at + q * 64 * n) * Type<DT>::kBytes);
+    for (int q = 0; q < Type<DT>::kPackets; q++) {
+      const auto* p = reinterpret_cast<const typename Type<DT>::mem*>(row + (size_t)(at + q * 64 * n) * Type<DT>::kBytes);
+      s.w[q] = ONCE ? __builtin_nontemporal_load(p) : *p;
+    }
   } else {
 #pragma unroll
     for (int q = 0; q < Type<DT>::kPackets; q++) s.w[q] = load_packet<DT>(row, at + q * 64 * n, V);
@@ -172,10 +177,45 @@ __device__ __forceinline__ float wave_max(float x) {
   x = fmaxf(x, dpp<0x143, 0xc>(x, no));
   return last_lane(x);
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp(uint32_t x, uint32_t idle) {
+  return __builtin_amdgcn_update_dpp((int)idle, (int)x, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = dpp<CTRL, ROWS>((uint32_t)b, 0u), hi = dpp<CTRL, ROWS>((uint32_t)(b >> 32), 0u);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+  x += dpp<0x111, 0xf>(x);
+  x += dpp<0x112, 0xf>(x);
+  x += dpp<0x114, 0xf>(x);
+  x += dpp<0x118, 0xf>(x);
+  x += dpp<0x142, 0xa>(x);
+  x += dpp<0x143, 0xc>(x);
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, 63), hi = __builtin_amdgcn_readlane((int)(b >> 32), 63);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Inclusive sums over the lanes up to each.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += dpp<0x111, 0xf>(x, 0u);
+  x += dpp<0x112, 0xf>(x, 0u);
+  x += dpp<0x114, 0xf>(x, 0u);
+  x += dpp<0x118, 0xf>(x, 0u);
+  x += dpp<0x142, 0xa>(x, 0u);
+  x += dpp<0x143, 0xc>(x, 0u);
   return x;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  x = max(x, dpp<0x111, 0xf>(x, 0u));
+  x = max(x, dpp<0x112, 0xf>(x, 0u));
+  x = max(x, dpp<0x114, 0xf>(x, 0u));
+  x = max(x, dpp<0x118, 0xf>(x, 0u));
+  x = max(x, dpp<0x142, 0xa>(x, 0u));
+  x = max(x, dpp<0x143, 0xc>(x, 0u));
+  return __builtin_amdgcn_readlane((int)x, 63);
 }
 
 // ---- a segment -----------------------------------------------------------------
@@ -196,20 +236,37 @@ __device__ __forceinline__ float lane_max(const Seg<DT>& z) {
   return m;
 }
 
-template <int DT, bool ENT>
-__device__ __forceinline__ Part seg_part(const Seg<DT>& z, float most, float c) {
-  Part p{wave_max(most), 0.0f, 0.0f};
+// The sums of a segment.  NEAR: t from one fused z c - mc, mc the rounded m c
+// (the sums are then relative to mc and are brought back to m c at the end);
+// otherwise from z - m, where z c or m c could overflow.
+template <int DT, bool ENT, bool NEAR>
+__device__ __forceinline__ void seg_sums(const Seg<DT>& z, float m, float c, float& sum, float& weighted) {
   float s[4] = {}, u[4] = {};
-  const float m = p.m == -__builtin_inff() ? 0.0f : p.m;
+  const float mc = m * c;
 #pragma unroll
   for (int i = 0; i < kPer; i++) {
-    const float t = (value<DT>(z, i) - m) * c;
+    const float v = value<DT>(z, i), t = NEAR ? __builtin_fmaf(v, c, -mc) : (v - m) * c;
     const float e = __builtin_amdgcn_exp2f(t);
     s[i & 3] += e;
     if (ENT) u[i & 3] = __builtin_fmaf(e, fmaxf(t, kLowest), u[i & 3]);
   }
-  p.s = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
-  if (ENT) p.u = wave_sum((u[0] + u[1]) + (u[2] + u[3]));
+  sum = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
+  weighted = ENT ? wave_sum((u[0] + u[1]) + (u[2] + u[3])) : 0.0f;
+  if (NEAR) {
+    const float d = __builtin_fmaf(m, c, -mc), f = __builtin_amdgcn_exp2f(-d);
+    weighted = (weighted - d * sum) * f;
+    sum *= f;
+  }
+}
+
+template <int DT, bool ENT>
+__device__ __forceinline__ Part seg_part(const Seg<DT>& z, float most, float c) {
+  Part p{wave_max(most), 0.0f, 0.0f};
+  const float m = p.m == -__builtin_inff() ? 0.0f : p.m;
+  if (__builtin_fabsf(m) < 0x1p60f)  // m c < 2^75
+    seg_sums<DT, ENT, true>(z, m, c, p.s, p.u);
+  else
+    seg_sums<DT, ENT, false>(z, m, c, p.s, p.u);
   return p;
 }
 
@@ -221,52 +278,79 @@ struct RowStats {
   bool bad;     // a logit is NaN or +inf
 };
 
-// One wave joins the parts of a row.  The first segment that holds the maximum
-// is read again for its sum without it.  `mask` (may be null): per segment and
-// lane the logits that the parts left out.
-template <int DT>
-__device__ RowStats join_parts(const char* row, int V, int nseg, const Part* parts, const uint32_t* mask, float c,
-                               int lane) {
+// A row's maximum and the first segment that holds it, by a whole wave.
+struct RowMax {
+  float m;
+  int first;
+  bool none;  // nothing to sum: a NaN or +inf (bad), or every logit masked
+  bool bad;
+};
+__device__ __forceinline__ RowMax find_max(const Part* parts, int nseg, int lane) {
   const float no = -__builtin_inff();
   const Part a = lane < nseg ? parts[lane] : Part{no, 0.0f, 0.0f};
   const Part b = lane + 64 < nseg ? parts[lane + 64] : Part{no, 0.0f, 0.0f};
-  RowStats st;
-  st.m = wave_max(fmaxf(a.m, b.m));
-  const bool nan = !(a.s == a.s) || !(b.s == b.s);
-  st.bad = __ballot(nan) != 0 || st.m == __builtin_inff();
-  st.r = st.u = 0.0;
-  if (st.bad || st.m == no) return st;
-  const uint64_t in_a = __ballot(a.m == st.m), in_b = __ballot(b.m == st.m);
-  const int first = in_a ? __builtin_ctzll(in_a) : 64 + __builtin_ctzll(in_b);
+  RowMax x;
+  x.m = wave_max(fmaxf(a.m, b.m));
+  x.bad = __ballot(!(a.s == a.s) || !(b.s == b.s)) != 0 || x.m == __builtin_inff();
+  x.none = x.bad || x.m == no;
+  const uint64_t in_a = __ballot(a.m == x.m), in_b = __ballot(b.m == x.m);
+  x.first = x.none ? 0 : in_a ? __builtin_ctzll(in_a) : 64 + __builtin_ctzll(in_b);
+  return x;
+}
 
-  Seg<DT> z;
-  load_seg<DT>(z, row, first, lane, V);
-  if (mask) mask_seg<DT>(z, mask[first * 64 + lane]);
-  const float most = lane_max<DT>(z);
-  const uint64_t have = __ballot(most == st.m);
+// A lane's sums of e and of e t over the segment that holds the maximum m, one
+// such logit left out.
+template <int DT, bool ENT>
+__device__ __forceinline__ void sums_without_max(const Seg<DT>& z, float m, float c, int lane, float& s, float& w) {
+  const uint64_t have = __ballot(lane_max<DT>(z) == m);
   bool out = lane == __builtin_ctzll(have);  // this lane's first maximum stays out
-  float s = 0.0f;
+  s = w = 0.0f;
 #pragma unroll
   for (int i = 0; i < kPer; i++) {
-    const float v = value<DT>(z, i), e = __builtin_amdgcn_exp2f((v - st.m) * c);
-    const bool skip = out && v == st.m;
+    const float v = value<DT>(z, i), t = (v - m) * c;
+    const bool skip = out && v == m;
     out = out && !skip;
-    s += skip ? 0.0f : e;
+    const float e = skip ? 0.0f : __builtin_amdgcn_exp2f(t);
+    s += e;
+    if (ENT) w = __builtin_fmaf(e, fmaxf(t, kLowest), w);
   }
-  double r = s, u = 0.0;
-  const Part* two[2] = {&a, &b};
+}
+
+// The row's sums from its parts, with those of the maximum's segment as above.
+template <bool ENT>
+__device__ __forceinline__ RowStats join_parts(const RowMax& x, const Part* parts, int nseg, float s, float w, float c,
+                                               int lane) {
+  RowStats st{x.m, 0.0, 0.0, x.bad};
+  if (x.none) return st;
+  double r = s, u = w;
 #pragma unroll
   for (int i = 0; i < 2; i++) {
-    const Part& p = *two[i];
-    if (p.m == no) continue;
-    const float d = fmaxf((p.m - st.m) * c, -1000.0f);
+    const int seg = lane + 64 * i;
+    if (seg >= nseg || seg == x.first || parts[seg].m == -__builtin_inff()) continue;
+    const Part p = parts[seg];
+    const float d = fmaxf((p.m - x.m) * c, -1000.0f);
     const double f = __builtin_amdgcn_exp2f(d);
-    if (lane + 64 * i != first) r += f * p.s;
-    u += f * ((double)p.u + (double)d * p.s);
+    r += f * p.s;
+    if (ENT) u += f * ((double)p.u + (double)d * p.s);
   }
   st.r = wave_sum(r);
-  st.u = wave_sum(u);
+  if (ENT) st.u = wave_sum(u);
   return st;
+}
+
+// Both by one wave, the maximum's segment read again.  `mask` (may be null): per
+// segment and lane the logits that the parts left out.
+template <int DT, bool ENT>
+__device__ __forceinline__ RowStats join_row(const char* row, int V, int nseg, const Part* parts, const uint32_t* mask, float c, int lane) {
+  const RowMax x = find_max(parts, nseg, lane);
+  float s = 0.0f, w = 0.0f;
+  if (!x.none) {
+    Seg<DT> z;
+    load_seg<DT, false>(z, row, x.first, lane, V);
+    if (mask) mask_seg<DT>(z, mask[x.first * 64 + lane]);
+    sums_without_max<DT, ENT>(z, x.m, c, lane, s, w);
+  }
+  return join_parts<ENT>(x, parts, nseg, s, w, c, lane);
 }
 
 // ---- the largest logits of a row ---------------------------------------------------
@@ -281,7 +365,9 @@ __device__ __forceinline__ float of_order(uint32_t k) {
   return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-struct TopLds {
+struct alignas(16) TopLds {
+  uint32_t bins[4][256];
+  uint32_t low[kRowWaves], high[kRowWaves];
   uint32_t counts[2][kRowWaves];
   uint32_t buckets, candidates, chosen;
   uint16_t ties[kScoreMaxSegs];
@@ -290,6 +376,17 @@ struct TopLds {
 };
 // Candidates: every logit of K + 64 buckets at most.
 constexpr size_t candidate_bytes(size_t top) { return (top + 64) * kPer * sizeof(uint64_t); }
+
+// Places for each lane's n entries at the end of a list, by a whole wave.
+__device__ __forceinline__ uint32_t append(uint32_t* length, uint32_t n, int lane) {
+  const uint32_t sum = wave_scan(n), all = __builtin_amdgcn_readlane((int)sum, 63);
+  uint32_t base = 0;
+  if (all != 0) {
+    if (lane == 0) base = atomicAdd(length, all);
+    base = __builtin_amdgcn_readfirstlane((int)base);
+  }
+  return base + sum - n;
+}
 
 // How many of the workgroup's flags are set, for step `step` of a loop: the two
 // sets of counts let one barrier a step do.
@@ -307,73 +404,130 @@ __device__ __forceinline__ int group_count(TopLds& t, int step, int in_wave, int
 // each bucket, a lane's share of a segment.  Put the buckets in the order of
 // their largest logits: the row's `top` largest lie in the first `top` buckets,
 // since each of those holds one that is as large.  So:
-//   1. tau, the value of bucket number `top` (bit by bit; 16 keys a thread);
-//   2. the buckets above tau, and those equal to it up to the segment where
-//      there are enough: the lowest indices among equals lie no further;
+//   1. tau, such that at least `top` buckets reach it and few more, by counting
+//      keys in 256 equal steps of an interval, then of the step that holds key
+//      `top`, four times at most, mostly once.  It starts at a key that a whole
+//      wave's threads reach (each by the largest of its keys): 64 keys are no less;
+//   2. the buckets from tau on.  If many equal tau, those only up to the segment
+//      where there are enough: the lowest indices among equals lie no further;
 //   3. their logits from tau on, read again (32 a bucket);
 //   4. these ranked by counting, each against each.
 // All but 3 is in LDS and registers, whatever the logits hold: rows of equal
 // logits take the same steps.  keys' memory is used again for the candidates.
-template <int DT, typename Emit>
-__device__ void select_top(const char* row, int V, int nseg, int top, uint64_t* memory, TopLds& t, Emit&& emit) {
+// `aside` is called once between 2 and 3 and may keep one wave busy; its results
+// are there when `emit` is called.
+template <int DT, typename Aside, typename Emit>
+__device__ __forceinline__ void select_top(const char* row, int V, int nseg, int top, uint64_t* memory, TopLds& t, Aside&& aside,
+                           Emit&& emit) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t* keys = reinterpret_cast<const uint32_t*>(memory);
-  uint32_t key[kKeysPerThread];
-#pragma unroll
-  for (int i = 0; i < kKeysPerThread; i++) key[i] = i * kRowWaves + wave < nseg ? keys[i * kRowThreads + tid] : 0;
-
-  uint32_t tau = 0;
-  for (int bit = 31; bit >= 0; bit--) {
-    const uint32_t trial = tau | 1u << bit;
-    int in_wave = 0;
-#pragma unroll
-    for (int i = 0; i < kKeysPerThread; i++)
-      if (i * kRowWaves < nseg) in_wave += __popcll(__ballot(key[i] >= trial));
-    const int n = group_count(t, bit, in_wave, wave, lane);
-    if (n >= top) tau = trial;
-    if (n == top) break;
-  }
-  if (tau == 0) tau = 1;  // fewer buckets than `top` hold anything unmasked
-
-  int above = 0;
-#pragma unroll
-  for (int i = 0; i < kKeysPerThread; i++)
-    if (i * kRowWaves + wave < nseg) {
-      above += __popcll(__ballot(key[i] > tau));
-      const int same = __popcll(__ballot(key[i] == tau));
-      if (lane == 0) t.ties[i * kRowWaves + wave] = same;
-    }
-  __syncthreads();  // the counts of the last step have been read
-  if (lane == 0) t.counts[0][wave] = above;
-  if (tid == 0) t.buckets = t.candidates = t.chosen = 0;
-  __syncthreads();
-  above = 0;
-#pragma unroll
-  for (int w = 0; w < kRowWaves; w++) above += t.counts[0][w];
-  int last = 0;
-  for (int have = above; last < nseg; last++) {
-    have += t.ties[last];
-    if (have >= top) break;
-  }
+  uint32_t key[kKeysPerThread], most = 0;
 #pragma unroll
   for (int i = 0; i < kKeysPerThread; i++) {
-    const int seg = i * kRowWaves + wave;
-    if (seg < nseg && (key[i] > tau || (key[i] == tau && seg <= last)))
-      t.bucket[atomicAdd(&t.buckets, 1u)] = (uint16_t)(seg * 64 + lane);
+    key[i] = i * kRowWaves + wave < nseg ? keys[i * kRowThreads + tid] : 0;
+    most = max(most, key[i]);
   }
+  const uint32_t low = ~wave_max(~most), high = wave_max(most);
+  if (lane == 0) {
+    t.low[wave] = low;
+    t.high[wave] = high;
+  }
+  for (int i = tid; i < 4 * 256; i += kRowThreads) (&t.bins[0][0])[i] = 0;
+  if (tid == 0) t.buckets = t.candidates = t.chosen = 0;
   __syncthreads();
+
+  uint32_t lo = 0, second = 0, hi = 0;
+#pragma unroll
+  for (int w = 0; w < kRowWaves; w++) {
+    const uint32_t x = t.low[w];
+    second = max(second, min(lo, x));
+    lo = max(lo, x);
+    hi = max(hi, t.high[w]);
+  }
+  lo = top == 1 ? hi : top > 64 ? second : lo;
+  lo = max(lo, 1u);  // 0 is masked
+  static_assert(kScoreMaxTop <= 128, "two waves' keys");
+  int above = 0, equal = 0;  // keys past the interval, and in the last one
+  uint32_t tau = lo;
+  for (int step = 0; step < 4 && lo <= hi; step++) {
+    const int bits = 32 - __builtin_clz((hi - lo) | 1u), shift = bits > 8 ? bits - 8 : 0;
+#pragma unroll
+    for (int i = 0; i < kKeysPerThread; i++)
+      if (key[i] >= lo && key[i] <= hi) atomicAdd(&t.bins[step][(key[i] - lo) >> shift], 1u);
+    __syncthreads();
+    // lane 0 has the four highest bins
+    const uint4 b = *reinterpret_cast<const uint4*>(&t.bins[step][252 - 4 * lane]);
+    const uint32_t sum = wave_scan(b.x + b.y + b.z + b.w);
+    const uint64_t reach = __ballot((int)sum >= top - above);
+    if (reach == 0) {  // fewer than `top` buckets hold anything unmasked
+      equal = __builtin_amdgcn_readlane((int)sum, 63);
+      tau = lo;
+      break;
+    }
+    uint32_t over = sum - (b.x + b.y + b.z + b.w), bin = 252 - 4 * lane + 3, in = b.w;
+    const uint32_t c[3] = {b.z, b.y, b.x};
+#pragma unroll
+    for (int i = 0; i < 3; i++)
+      if ((int)(over + in) < top - above) {
+        over += in;
+        in = c[i];
+        bin--;
+      }
+    const int at = __builtin_ctzll(reach);
+    above += __builtin_amdgcn_readlane((int)over, at);
+    equal = __builtin_amdgcn_readlane((int)in, at);
+    lo += (uint32_t)__builtin_amdgcn_readlane((int)bin, at) << shift;
+    hi = lo + min(hi - lo, (1u << shift) - 1u);
+    tau = lo;
+    if (shift == 0 || above + equal <= top + top / 4 + 8) break;
+  }
+
+  int last = nseg;  // the segment up to which keys equal to tau count
+  if (above + equal > top + 64) {  // then the interval is one key wide
+#pragma unroll
+    for (int i = 0; i < kKeysPerThread; i++)
+      if (i * kRowWaves + wave < nseg) {
+        const int same = __popcll(__ballot(key[i] == tau));
+        if (lane == 0) t.ties[i * kRowWaves + wave] = same;
+      }
+    __syncthreads();
+    last = 0;
+    for (int have = above; last < nseg; last++) {
+      have += t.ties[last];
+      if (have >= top) break;
+    }
+  }
+  uint32_t mine = 0;
+#pragma unroll
+  for (int i = 0; i < kKeysPerThread; i++)
+    if (key[i] > tau || (key[i] == tau && i * kRowWaves + wave <= last)) mine |= 1u << i;
+  uint32_t at = append(&t.buckets, __popc(mine), lane);
+  for (uint32_t m = mine; m; m &= m - 1)
+    t.bucket[at++] = (uint16_t)((__builtin_ctz(m) * kRowWaves + wave) * 64 + lane);
+  __syncthreads();
+  aside();
 
   constexpr int np = Type<DT>::kPackets, in = Type<DT>::kInPacket;
   const int work = (int)t.buckets * np;
-  for (int w = tid; w < work; w += kRowThreads) {
-    const int b = t.bucket[w / np];
-    const int j = (b >> 6) * kScoreSeg + (w % np) * (64 * in) + (b & 63) * in;
-    const packet p = load_packet<DT>(row, j, V);
+  for (int first = 0; first < work; first += kRowThreads) {
+    const int w = first + tid;
+    int j = 0;
+    uint32_t k[in], have = 0;
+    if (w < work) {
+      const int b = t.bucket[w / np];
+      j = (b >> 6) * kScoreSeg + (w % np) * (64 * in) + (b & 63) * in;
+      const packet p = load_packet<DT>(row, j, V);
 #pragma unroll
-    for (int i = 0; i < in; i++) {
-      const uint32_t k = order_of(value<DT>(p, i));
-      if (k >= tau) memory[atomicAdd(&t.candidates, 1u)] = (uint64_t)k << 18 | (uint32_t)(kScoreMaxVocab - 1 - (j + i));
+      for (int i = 0; i < in; i++) {
+        k[i] = order_of(value<DT>(p, i));
+        have += k[i] >= tau;
+      }
     }
+    uint32_t to = append(&t.candidates, have, lane);
+    if (have)
+#pragma unroll
+      for (int i = 0; i < in; i++)
+        if (k[i] >= tau) memory[to++] = (uint64_t)k[i] << 18 | (uint32_t)(kScoreMaxVocab - 1 - (j + i));
   }
   __syncthreads();
 
@@ -395,11 +549,17 @@ __device__ void select_top(const char* row, int V, int nseg, int top, uint64_t* 
     list = t.best;
     n = top;
   }
-  if (tid < n) {
-    const uint64_t mine = list[tid];
+  // eight threads count for one candidate
+  for (int first = 0; first < n; first += kRowThreads / 8) {
+    const int i = first + tid / 8;
+    const uint64_t one = list[min(i, n - 1)];
     int rank = 0;
-    for (int i = 0; i < n; i++) rank += list[i] > mine;
-    if (rank < top) emit(rank, kScoreMaxVocab - 1 - (int)(mine & (kScoreMaxVocab - 1)), of_order((uint32_t)(mine >> 18)));
+    for (int j = tid & 7; j < n; j += 8) rank += list[j] > one;
+    rank += __shfl_xor(rank, 1);
+    rank += __shfl_xor(rank, 2);
+    rank += __shfl_xor(rank, 4);
+    if (i < n && rank < top && (tid & 7) == 0)
+      emit(rank, kScoreMaxVocab - 1 - (int)(one & (kScoreMaxVocab - 1)), of_order((uint32_t)(one >> 18)));
   }
   if (tid < top && tid >= n) emit(tid, -1, -__builtin_inff());
 }
@@ -409,15 +569,15 @@ __device__ void select_top(const char* row, int V, int nseg, int top, uint64_t* 
 // Segments seg0 + wave, seg0 + wave + waves, ... below seg1: their parts, and
 // with KEYS their buckets' largest logits.  The next segment's loads are in
 // flight while one is reduced.
-template <int DT, bool ENT, bool KEYS>
+template <int DT, bool ENT, bool KEYS, bool ONCE>
 __device__ __forceinline__ void read_segs(const char* row, int V, int seg0, int seg1, int wave, int waves, int lane,
                                           float c, Part* parts, uint32_t* keys, const uint32_t* mask) {
   int seg = seg0 + wave;
   if (seg >= seg1) return;
   Seg<DT> z, next;
-  load_seg<DT>(z, row, seg, lane, V);
+  load_seg<DT, ONCE>(z, row, seg, lane, V);
   for (; seg < seg1; seg += waves) {
-    if (seg + waves < seg1) load_seg<DT>(next, row, seg + waves, lane, V);
+    if (seg + waves < seg1) load_seg<DT, ONCE>(next, row, seg + waves, lane, V);
     if (mask) {
       const uint32_t bits = mask[seg * 64 + lane];
       if (__ballot(bits != 0)) mask_seg<DT>(z, bits);
@@ -442,7 +602,7 @@ __device__ __forceinline__ long load_index(const void* p, int wide, size_t i) {
 
 struct ScoreK {
   const char* z;
-  size_t row_bytes, rows;
+  size_t row_bytes, row0;  // the launch's first row
   int V, nseg, groups;
   const void* tokens;
   int wide, top;
@@ -455,7 +615,7 @@ struct ScoreK {
   uint32_t* keys;  // [rows][nseg * 64]
 };
 
-template <int DT, bool TOP, int PHASE>
+template <int DT, bool TOP, int PHASE, bool ONCE>
 __global__ __launch_bounds__(kRowThreads) void k_scores(ScoreK a) {
   extern __shared__ uint64_t memory[];
   __shared__ Part lds_parts[PHASE == PARTS ? 1 : kScoreMaxSegs];
@@ -467,66 +627,63 @@ __global__ __launch_bounds__(kRowThreads) void k_scores(ScoreK a) {
   const float no = -__builtin_inff();
 
   if constexpr (PHASE == PARTS) {
-    for (size_t w = blockIdx.x; w < a.rows * a.groups; w += gridDim.x) {
-      const size_t row = w / a.groups;
-      const int g = (int)(w % a.groups), per = (a.nseg + a.groups - 1) / a.groups;
-      const int seg1 = min(a.nseg, (g + 1) * per);
-      read_segs<DT, true, TOP>(a.z + row * a.row_bytes, a.V, g * per, seg1, wave, waves, lane, a.c,
-                               a.parts + row * a.nseg, TOP ? a.keys + row * a.nseg * 64 : nullptr, nullptr);
-    }
+    const size_t row = blockIdx.x / a.groups;
+    const int g = (int)(blockIdx.x % a.groups), per = (a.nseg + a.groups - 1) / a.groups;
+    read_segs<DT, true, TOP, ONCE>(a.z + row * a.row_bytes, a.V, g * per, min(a.nseg, (g + 1) * per), wave, waves, lane, a.c,
+                             a.parts + row * a.nseg, TOP ? a.keys + row * a.nseg * 64 : nullptr, nullptr);
     return;
   }
 
   uint32_t* keys = reinterpret_cast<uint32_t*>(memory);
-  for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const char* z = a.z + row * a.row_bytes;
-    long y = -1;
-    float zy = 0.0f;
-    if (wave == 0 && a.tokens) {
-      y = load_index(a.tokens, a.wide, row);
-      if (y >= 0 && y < a.V) zy = load_one<DT>(z, (int)y);
+  const size_t row = a.row0 + blockIdx.x;
+  const char* z = a.z + row * a.row_bytes;
+  long y = -1;
+  float zy = 0.0f;
+  if (wave == 0 && a.tokens) {
+    y = load_index(a.tokens, a.wide, row);
+    if (y >= 0 && y < a.V) zy = load_one<DT>(z, (int)y);
+  }
+  if constexpr (PHASE == WHOLE) {
+    read_segs<DT, true, TOP, ONCE>(z, a.V, 0, a.nseg, wave, waves, lane, a.c, lds_parts, keys, nullptr);
+  } else {
+    for (int i = threadIdx.x; i < a.nseg; i += kRowThreads) lds_parts[i] = a.parts[row * a.nseg + i];
+    if (TOP)
+      for (int i = threadIdx.x; i < a.nseg * 64; i += kRowThreads) keys[i] = a.keys[row * a.nseg * 64 + i];
+  }
+  __syncthreads();
+  auto join = [&]() __attribute__((always_inline)) {
+    if (wave != 0) return;
+    const RowStats st = join_row<DT, true>(z, a.V, a.nseg, lds_parts, nullptr, a.c, lane);
+    const double l = st.bad ? (double)__builtin_nanf("") : log1p(st.r);
+    const float m = st.bad ? __builtin_nanf("") : st.m;
+    if (lane != 0) return;
+    row_m = m;
+    row_log = l;
+    if (a.stats) {
+      a.stats[2 * row] = m;
+      a.stats[2 * row + 1] = st.bad ? m : (float)st.r;
     }
-    if constexpr (PHASE == WHOLE) {
-      read_segs<DT, true, TOP>(z, a.V, 0, a.nseg, wave, waves, lane, a.c, lds_parts, keys, nullptr);
-    } else {
-      for (int i = threadIdx.x; i < a.nseg; i += kRowThreads) lds_parts[i] = a.parts[row * a.nseg + i];
-      if (TOP)
-        for (int i = threadIdx.x; i < a.nseg * 64; i += kRowThreads) keys[i] = a.keys[row * a.nseg * 64 + i];
+    if (a.entropy) a.entropy[row] = st.m == no && !st.bad ? 0.0f : (float)(l - kLn2 * st.u / (1.0 + st.r));
+    if (a.log_probs) {
+      float lp = 0.0f;
+      if (y >= a.V)
+        lp = __builtin_nanf("");
+      else if (y >= 0)
+        lp = m == no ? no : (float)(((double)zy - m) * a.inv_t - l);
+      a.log_probs[row] = lp;
     }
-    __syncthreads();
-    if (wave == 0) {
-      const RowStats st = join_parts<DT>(z, a.V, a.nseg, lds_parts, nullptr, a.c, lane);
-      const double l = st.bad ? (double)__builtin_nanf("") : log1p(st.r);
-      const float m = st.bad ? __builtin_nanf("") : st.m;
-      if (lane == 0) {
-        row_m = m;
-        row_log = l;
-        if (a.stats) {
-          a.stats[2 * row] = m;
-          a.stats[2 * row + 1] = st.bad ? m : (float)st.r;
-        }
-        if (a.entropy) a.entropy[row] = st.m == no && !st.bad ? 0.0f : (float)(l - kLn2 * st.u / (1.0 + st.r));
-        if (a.log_probs) {
-          float lp = 0.0f;
-          if (y >= a.V)
-            lp = __builtin_nanf("");
-          else if (y >= 0)
-            lp = m == no ? no : (float)(((double)zy - m) * a.inv_t - l);
-          a.log_probs[row] = lp;
-        }
-      }
-    }
-    if constexpr (TOP) {
-      int32_t* ids = a.top_ids + row * a.top;
-      float* lps = a.top_log_probs + row * a.top;
-      select_top<DT>(z, a.V, a.nseg, a.top, memory, tl, [&](int at, int id, float v) {
-        const float m = row_m;
-        const bool bad = !(m == m);
-        ids[at] = bad ? -1 : id;
-        lps[at] = bad ? m : id < 0 ? no : (float)(((double)v - m) * a.inv_t - row_log);
-      });
-    }
-    __syncthreads();
+  };
+  if constexpr (!TOP) {
+    join();
+  } else {
+    int32_t* ids = a.top_ids + row * a.top;
+    float* lps = a.top_log_probs + row * a.top;
+    select_top<DT>(z, a.V, a.nseg, a.top, memory, tl, join, [&](int at, int id, float v) __attribute__((always_inline)) {
+      const float m = row_m;
+      const bool bad = !(m == m);
+      ids[at] = bad ? -1 : id;
+      lps[at] = bad ? m : id < 0 ? no : (float)(((double)v - m) * a.inv_t - row_log);
+    });
   }
 }
 
@@ -536,7 +693,7 @@ __global__ __launch_bounds__(kRowThreads) void k_scores(ScoreK a) {
 struct ScoreGradK {
   const char* z;
   char* grad;
-  size_t row_bytes, grad_bytes, rows;
+  size_t row_bytes, grad_bytes, row0;
   int V, nseg, chunks;
   const void* tokens;
   int wide;
@@ -548,7 +705,7 @@ struct ScoreGradK {
 // Segments a wave takes one after another; a workgroup has kGradWaves waves.
 constexpr int kGradWaves = 4, kGradSegs = 2;
 
-template <int DT, typename F>
+template <int DT, bool ONCE, typename F>
 __device__ __forceinline__ void write_seg(const Seg<DT>& z, char* out, int seg, int lane, int V, F&& f) {
   constexpr int in = Type<DT>::kInPacket;
   const bool whole = seg * kScoreSeg + kScoreSeg <= V;
@@ -563,7 +720,11 @@ __device__ __forceinline__ void write_seg(const Seg<DT>& z, char* out, int seg, 
     for (int d = 0; d < 4; d++)
       p[d] = DT == DTL_F32 ? bits_of<DT>(v[d]) : bits_of<DT>(v[2 * d % in]) | bits_of<DT>(v[(2 * d + 1) % in]) << 16;
     if (whole || j + in <= V) {
-      *reinterpret_cast<typename Type<DT>::mem*>(out + (size_t)j * Type<DT>::kBytes) = p;
+      auto* to = reinterpret_cast<typename Type<DT>::mem*>(out + (size_t)j * Type<DT>::kBytes);
+      if (ONCE)
+        __builtin_nontemporal_store(p, to);
+      else
+        *to = p;
     } else {
 #pragma unroll
       for (int i = 0; i < in; i++)
@@ -576,49 +737,47 @@ template <int DT, bool ENT>
 __global__ __launch_bounds__(kGradWaves * 64) void k_scores_grad(ScoreGradK a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const float no = -__builtin_inff();
-  for (size_t w = blockIdx.x; w < a.rows * a.chunks; w += gridDim.x) {
-    const size_t row = w / a.chunks;
-    const int seg0 = (int)(w % a.chunks) * (kGradWaves * kGradSegs) + wave;
-    const char* z = a.z + row * a.row_bytes;
-    char* out = a.grad + row * a.grad_bytes;
-    const long y = a.tokens ? load_index(a.tokens, a.wide, row) : -1;
-    const double g = a.g && y >= 0 ? a.g[row] : 0.0f, h = ENT && a.h ? a.h[row] : 0.0f;
-    const float m = a.stats[2 * row];
-    const double r = a.stats[2 * row + 1], p0 = 1.0 / (1.0 + r);
-    // padding, and rows whose mask leaves nothing: zeros, whatever they hold
-    const bool zero = (g == 0.0 && h == 0.0) || m == no;
-    const bool bad = y >= a.V, here = y >= 0 && !bad && !zero && ((int)(y >> 11) - seg0) % kGradWaves == 0;
-    double l = 0.0, hh = 0.0;
-    if (ENT || here) {
-      l = log1p(r);
-      hh = ENT ? (double)a.entropy[row] - l : 0.0;
-    }
-    const float A = bad ? __builtin_nanf("") : (float)(-a.inv_t * p0 * (g + h * hh)), B = (float)(-a.inv_t * p0 * h * kLn2);
-    float at_y = 0.0f;
-    if (here) {
-      const double t = ((double)load_one<DT>(z, (int)y) - m) * a.inv_t, lp = t - l;
-      // log p of a masked token is -inf and its p log p is 0
-      at_y = (float)(a.inv_t * (-g * expm1(lp) - (ENT && h != 0.0 && lp > -1e30 ? h * exp(lp) * (t + hh) : 0.0)));
-    }
+  const size_t row = a.row0 + blockIdx.x / a.chunks;
+  const int seg0 = (int)(blockIdx.x % a.chunks) * (kGradWaves * kGradSegs) + wave;
+  const char* z = a.z + row * a.row_bytes;
+  char* out = a.grad + row * a.grad_bytes;
+  const long y = a.tokens ? load_index(a.tokens, a.wide, row) : -1;
+  const double g = a.g && y >= 0 ? a.g[row] : 0.0f, h = ENT && a.h ? a.h[row] : 0.0f;
+  const float m = a.stats[2 * row];
+  const double r = a.stats[2 * row + 1], p0 = 1.0 / (1.0 + r);
+  // padding, and rows whose mask leaves nothing: zeros, whatever they hold
+  const bool zero = (g == 0.0 && h == 0.0) || m == no;
+  const bool bad = y >= a.V, here = y >= 0 && !bad && !zero && ((int)(y >> 11) - seg0) % kGradWaves == 0;
+  double l = 0.0, hh = 0.0;
+  if (ENT || here) {
+    l = log1p(r);
+    hh = ENT ? (double)a.entropy[row] - l : 0.0;
+  }
+  const float A = bad ? __builtin_nanf("") : (float)(-a.inv_t * p0 * (g + h * hh)), B = (float)(-a.inv_t * p0 * h * kLn2);
+  float at_y = 0.0f;
+  if (here) {
+    const double t = ((double)load_one<DT>(z, (int)y) - m) * a.inv_t, lp = t - l;
+    // log p of a masked token is -inf and its p log p is 0
+    at_y = (float)(a.inv_t * (-g * expm1(lp) - (ENT && h != 0.0 && lp > -1e30 ? h * exp(lp) * (t + hh) : 0.0)));
+  }
 #pragma unroll
-    for (int i = 0; i < kGradSegs; i++) {
-      const int seg = seg0 + i * kGradWaves;
-      if (seg >= a.nseg) break;
-      Seg<DT> s;
-      if (zero) {
-        write_seg<DT>(s, out, seg, lane, a.V, [](float, int) { return 0.0f; });
-        continue;
-      }
-      load_seg<DT>(s, z, seg, lane, a.V);
-      auto value_of = [&](float v) {
-        const float t = (v - m) * a.c, e = __builtin_amdgcn_exp2f(t);
-        return e * (ENT ? __builtin_fmaf(B, fmaxf(t, kLowest), A) : A);
-      };
-      if (y >> 11 == seg)
-        write_seg<DT>(s, out, seg, lane, a.V, [&](float v, int j) { return j == (int)y ? at_y : value_of(v); });
-      else
-        write_seg<DT>(s, out, seg, lane, a.V, [&](float v, int) { return value_of(v); });
+  for (int i = 0; i < kGradSegs; i++) {
+    const int seg = seg0 + i * kGradWaves;
+    if (seg >= a.nseg) break;
+    Seg<DT> s;
+    if (zero) {
+      write_seg<DT, false>(s, out, seg, lane, a.V, [](float, int) { return 0.0f; });
+      continue;
     }
+    load_seg<DT, false>(s, z, seg, lane, a.V);
+    auto value_of = [&](float v) {
+      const float t = (v - m) * a.c, e = __builtin_amdgcn_exp2f(t);
+      return e * (ENT ? __builtin_fmaf(B, fmaxf(t, kLowest), A) : A);
+    };
+    if (y >> 11 == seg)
+      write_seg<DT, false>(s, out, seg, lane, a.V, [&](float v, int j) { return j == (int)y ? at_y : value_of(v); });
+    else
+      write_seg<DT, false>(s, out, seg, lane, a.V, [&](float v, int) { return value_of(v); });
   }
 }
 static_assert(kScoreSeg == 1 << 11, "the token's segment");
@@ -637,7 +796,7 @@ static_assert(kScoreSeg == 1 << 11, "the token's segment");
 struct DistillK {
   const char* z;
   char* grad;
-  size_t row_bytes, grad_bytes, rows;
+  size_t row_bytes, grad_bytes, row0;
   int V, nseg, groups;
   const void* ids;
   int wide, k;
@@ -650,58 +809,97 @@ struct DistillK {
   Part* parts;
 };
 
+// The row's slots and their logits.
 struct Slots {
   int32_t id[kDistillMaxK];  // -1: empty
   float v[kDistillMaxK];
+  float z[kDistillMaxK];
+  int bits[kDistillMaxK / 64];
 };
+enum { USED = 1, BROKEN = 2 };
 
-// Loads the slots; the result is, for every thread, whether the row has a slot
-// in use (1) and whether one is broken (2): an id past the vocabulary, a log
-// probability that is NaN or +inf.
-__device__ __forceinline__ int load_slots(Slots& s, const DistillK& a, size_t row) {
-  int bits = 0;
-  for (int i = threadIdx.x; i < kDistillMaxK; i += blockDim.x) {
-    int id = -1;
-    float v = -__builtin_inff();
-    if (i < a.k) {
-      const long j = load_index(a.ids, a.wide, row * a.k + i);
-      v = a.teacher[row * a.k + i];
-      if (j >= 0 && v != -__builtin_inff()) {
-        bits |= 1;
-        if (j >= a.V || !(v < __builtin_inff()))
-          bits |= 2;
-        else
-          id = (int)j;
+// Loads the slots: one for each of 256 threads.  After the barrier that follows,
+// slots_state tells whether the row has a slot in use and whether one is broken:
+// an id past the vocabulary, a log probability that is NaN or +inf (or with
+// rest such a logit, which the pass over the row leaves out).
+template <int DT, bool REST>
+__device__ __forceinline__ void load_slots(Slots& s, const DistillK& a, size_t row, const char* z) {
+  const int k = threadIdx.x;
+  if (k >= kDistillMaxK) return;
+  int id = -1, bits = 0;
+  float v = -__builtin_inff(), zk = v;
+  if (k < a.k) {
+    const long j = load_index(a.ids, a.wide, row * a.k + k);
+    v = a.teacher[row * a.k + k];
+    if (j >= 0 && v != -__builtin_inff()) {
+      bits = USED;
+      if (j >= a.V || !(v < __builtin_inff())) {
+        bits |= BROKEN;
+      } else {
+        id = (int)j;
+        zk = load_one<DT>(z, id);
+        if (REST && !(zk < __builtin_inff())) bits |= BROKEN;
       }
     }
-    s.id[i] = id;
-    s.v[i] = v;
   }
-  const int used = __syncthreads_or(bits & 1), broken = __syncthreads_or(bits & 2);
-  return (used ? 1 : 0) | (broken ? 2 : 0);
+  s.id[k] = id;
+  s.v[k] = v;
+  s.z[k] = zk;
+  const int any = (__ballot(bits & USED) ? USED : 0) | (__ballot(bits & BROKEN) ? BROKEN : 0);
+  if ((k & 63) == 0) s.bits[k >> 6] = any;
+}
+__device__ __forceinline__ int slots_state(const Slots& s) {
+  int bits = 0;
+#pragma unroll
+  for (int i = 0; i < kDistillMaxK / 64; i++) bits |= s.bits[i];
+  return __builtin_amdgcn_readfirstlane(bits);
 }
 
-// Which lane's which logit of a segment an id is: the bit of read_segs' mask.
+// Which lane's which logit of a segment an id is: the bit of the segments' mask.
 template <int DT>
-__device__ __forceinline__ void mask_bit(int id, int& word, uint32_t& bit) {
+__device__ __forceinline__ void mask_bit(uint32_t* mask, int id) {
   constexpr int in = Type<DT>::kInPacket;
   const int seg = id / kScoreSeg, at = id % kScoreSeg;
   const int q = at / (64 * in), lane = at / in % 64;
-  word = seg * 64 + lane;
-  bit = 1u << (q * in + at % in);
+  atomicOr(&mask[seg * 64 + lane], 1u << (q * in + at % in));
 }
-template <int DT>
-__device__ __forceinline__ void build_mask(uint32_t* mask, const Slots& s, int nseg) {
-  for (int i = threadIdx.x; i < nseg * 64; i += blockDim.x) mask[i] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < kDistillMaxK; i += blockDim.x)
-    if (s.id[i] >= 0) {
-      int word;
-      uint32_t bit;
-      mask_bit<DT>(s.id[i], word, bit);
-      atomicOr(&mask[word], bit);
+
+// What the slots alone give, a wave's share: with p proportional to e^(v - v0),
+// v0 the share's largest v (0 with rest, where p = e^v), z0 its largest logit.
+struct SlotSums {
+  double v0, sum, sum_v, sum_z;  // of e^(v - v0), and of it times v and times z - z0
+  double z0, in;                 // rest: sum of e^((z - z0) / T) over distinct ids
+};
+
+template <bool REST>
+__device__ __forceinline__ void sum_slots(const Slots& s, SlotSums* sums, int waves, double inv_t) {
+  const float no = -__builtin_inff();
+  for (int w = threadIdx.x >> 6; w < kDistillMaxK / 64; w += waves) {
+    const int lane = threadIdx.x & 63, k = w * 64 + lane, id = s.id[k];
+    const float v = s.v[k], z = s.z[k];
+    SlotSums t{};
+    if (!REST) {
+      const float most = wave_max(id >= 0 ? v : no);
+      t.v0 = most == no ? 0.0 : most;
     }
-  __syncthreads();
+    const double e = id >= 0 ? exp((double)v - t.v0) : 0.0;
+    t.sum = wave_sum(e);
+    t.sum_v = wave_sum(e > 0.0 ? e * v : 0.0);
+    const float z0 = wave_max(id >= 0 ? z : no);
+    t.z0 = z0;
+    t.sum_z = wave_sum(!(e > 0.0) ? 0.0 : z == no ? (double)no : e * ((double)z - z0));
+    if (REST) {
+      bool first = id >= 0;
+      const int4* ids = reinterpret_cast<const int4*>(s.id);
+      for (int j = 0; j < w * 16; j++) {
+        const int4 x = ids[j];
+        first = first && x.x != id && x.y != id && x.z != id && x.w != id;
+      }
+      for (int j = 0; j < 64; j++) first = first && (j >= lane || __builtin_amdgcn_readlane(id, j) != id);
+      t.in = wave_sum(first && z != no ? exp(((double)z - z0) * inv_t) : 0.0);
+    }
+    if (lane == 0) sums[w] = t;
+  }
 }
 
 // What a row's gradient needs besides its logits: m, share, rest / sum outside,
@@ -711,82 +909,66 @@ struct RowGrad {
 };
 static_assert(sizeof(RowGrad) == kDistillStats * sizeof(float), "stats");
 
-// One wave: the row's loss (times T^2) and what its gradient needs, from the
-// parts and the slots.
-template <int DT, bool REST>
-__device__ RowGrad join_distill(const DistillK& a, const char* z, const Part* parts, const uint32_t* mask,
-                                const Slots& s, int state, int lane, float* loss) {
+// The row's loss (times T^2) and what its gradient needs, from the row's stats
+// (with rest those outside the list) and the slots' sums.
+template <bool REST>
+__device__ __forceinline__ RowGrad join_distill(const DistillK& a, const RowStats& st, const SlotSums* sums, int state, float* loss) {
   const float no = -__builtin_inff(), nan = __builtin_nanf("");
-  constexpr int n = kDistillMaxK / 64;
-  RowGrad g{};
-  *loss = 0.0f;
-  if (state == 0) return g;
-  RowStats st = join_parts<DT>(z, a.V, a.nseg, parts, REST ? mask : nullptr, a.c, lane);
-  float zk[n];
-  bool first[n];
-  float most = no, most_v = no;
-#pragma unroll
-  for (int i = 0; i < n; i++) {
-    const int k = lane + 64 * i, id = s.id[k];
-    zk[i] = id >= 0 ? load_one<DT>(z, id) : no;
-    if (id >= 0) most_v = fmaxf(most_v, s.v[k]);
-    if (id >= 0) most = fmaxf(most, zk[i]);
-    first[i] = id >= 0;
-    if (REST && id >= 0)
-      for (int j = 0; j < k; j++) first[i] = first[i] && s.id[j] != id;
-    if (REST && id >= 0 && (!(zk[i] == zk[i]) || zk[i] == __builtin_inff())) st.bad = true;
+  if (!(state & USED)) {
+    *loss = 0.0f;
+    return RowGrad{};
   }
-  st.bad = __ballot(st.bad) != 0;
-  if (st.bad || (state & 2)) {
+  if (st.bad || (state & BROKEN)) {
     *loss = nan;
     return RowGrad{nan, nan, nan, nan, nan};
   }
-  // total of e relative to m, the row's largest logit; outside: without the list
-  double total, left = 0.0;
-  float m = st.m;
-  if (REST) {
-    most = wave_max(most);
-    m = fmaxf(st.m, most);
-    if (st.m != no) left = exp(((double)st.m - m) * a.inv_t) * (1.0 + st.r);
-    double in = 0.0;
+  constexpr int n = kDistillMaxK / 64;
+  double v0 = no, z0 = no;
 #pragma unroll
-    for (int i = 0; i < n; i++)
-      if (first[i] && zk[i] != no) in += exp(((double)zk[i] - m) * a.inv_t);
-    total = left + wave_sum(in);
-  } else {
-    total = 1.0 + st.r;
+  for (int i = 0; i < n; i++) {
+    if (sums[i].sum > 0.0) v0 = fmax(v0, sums[i].v0);
+    z0 = fmax(z0, sums[i].z0);
+  }
+  // total of e relative to m, the row's largest logit; left: without the list
+  double total = 1.0 + st.r, left = 0.0, m = st.m;
+  if (REST) {
+    m = fmax(m, z0);
+    if (st.m != no) left = exp((st.m - m) * a.inv_t) * (1.0 + st.r);
+    total = left;
   }
   if (m == no) {  // every logit masked: no q to compare with, nothing to move
     *loss = __builtin_inff();
     return RowGrad{no, 0.0f, 0.0f, 0.0f, 0.0f};
   }
-  most_v = wave_max(most_v);
-  double log_sum = 0.0;
-  if (!REST) {
-    double sum = 0.0;
+  double mass = 0.0, own = 0.0, cross = 0.0;  // sum of p, p v and p (z - m)
 #pragma unroll
-    for (int i = 0; i < n; i++)
-      if (s.id[lane + 64 * i] >= 0) sum += exp((double)s.v[lane + 64 * i] - most_v);
-    log_sum = most_v + log(wave_sum(sum));
+  for (int i = 0; i < n; i++) {
+    const SlotSums& x = sums[i];
+    if (REST && x.z0 > no) total += x.in * exp((x.z0 - m) * a.inv_t);
+    const double f = x.sum > 0.0 ? exp(x.v0 - v0) : 0.0;
+    if (f > 0.0) {
+      mass += f * x.sum;
+      own += f * x.sum_v;
+      cross += f * (x.sum_z + x.sum * (x.z0 - m));
+    }
   }
   const double log_total = REST ? log(total) : log1p(st.r);
-  double mass = 0.0, term = 0.0;
-#pragma unroll
-  for (int i = 0; i < n; i++)
-    if (s.id[lane + 64 * i] >= 0) {
-      const double lp = s.v[lane + 64 * i] - log_sum, p = exp(lp);
-      mass += p;
-      if (p > 0.0) term += p * (lp - (((double)zk[i] - m) * a.inv_t - log_total));
-    }
-  mass = wave_sum(mass);
-  term = wave_sum(term);
+  double log_sum = 0.0;
+  if (!REST) {
+    log_sum = v0 + log(mass);
+    cross /= mass;
+    own = own / mass - log_sum;
+    mass = 1.0;
+  }
+  double term = own - cross * a.inv_t + mass * log_total;
   double rest = 0.0;
   if (REST && left > 0.0) {
     rest = fmax(0.0, 1.0 - mass);
     if (rest > 0.0) term += rest * (log(rest) - (log(left) - log_total));
   }
   *loss = (float)((double)a.T * a.T * term);
-  g.m = m;
+  RowGrad g;
+  g.m = (float)m;
   g.share = (float)((mass + rest) / total);
   g.outside = rest > 0.0 ? (float)(rest / left) : 0.0f;
   g.log_hi = (float)log_sum;
@@ -794,30 +976,28 @@ __device__ RowGrad join_distill(const DistillK& a, const char* z, const Part* pa
   return g;
 }
 
-// Gradient of segments seg0 + wave, seg0 + wave + waves, ... below seg1, for
-// every j as if outside the list.
-template <int DT>
-__device__ __forceinline__ void grad_segs(const DistillK& a, const char* z, char* out, const RowGrad& g, float scale,
-                                          int seg0, int seg1, int wave, int waves, int lane) {
-  const bool zero = scale == 0.0f || g.m == -__builtin_inff();
+// Gradient of a segment for every j as if outside the list.
+template <int DT, bool ONCE>
+__device__ __forceinline__ void grad_seg(const DistillK& a, const Seg<DT>& s, char* out, const RowGrad& g, float scale,
+                                         int seg, int lane) {
   const float A = scale * (g.share - g.outside);
-  for (int seg = seg0 + wave; seg < seg1; seg += waves) {
-    Seg<DT> s;
-    if (zero) {
-      write_seg<DT>(s, out, seg, lane, a.V, [](float, int) { return 0.0f; });
-      continue;
-    }
-    load_seg<DT>(s, z, seg, lane, a.V);
-    write_seg<DT>(s, out, seg, lane, a.V,
-                  [&](float v, int) { return __builtin_amdgcn_exp2f((v - g.m) * a.c) * A; });
-  }
+  write_seg<DT, ONCE>(s, out, seg, lane, a.V,
+                      [&](float v, int) { return __builtin_amdgcn_exp2f((v - g.m) * a.c) * A; });
+}
+template <int DT>
+__device__ __forceinline__ void zero_seg(char* out, int seg, int lane, int V) {
+  Seg<DT> s;
+  write_seg<DT, false>(s, out, seg, lane, V, [](float, int) { return 0.0f; });
+}
+__device__ __forceinline__ bool grad_is_zero(const RowGrad& g, float scale) {
+  return scale == 0.0f || g.m == -__builtin_inff();
 }
 
-// The gradient at the list's ids from lo to hi, by one thread for each distinct
-// id: `zk` is its logit, read before the gradient was written (grad may be z).
+// The gradient at slot k's id, by the first slot of each distinct id.  Its
+// logit is the slots': the gradient may lie over the logits.
 template <int DT>
 __device__ __forceinline__ void grad_slot(const DistillK& a, char* out, const Slots& s, const RowGrad& g, float scale,
-                                          int k, float zk) {
+                                          int k) {
   const int id = s.id[k];
   double p = 0.0;
   for (int j = 0; j < a.k; j++)
@@ -825,71 +1005,167 @@ __device__ __forceinline__ void grad_slot(const DistillK& a, char* out, const Sl
       if (j < k) return;  // an earlier slot of the same id writes it
       p += exp(((double)s.v[j] - g.log_hi) - g.log_lo);
     }
-  const float e = __builtin_amdgcn_exp2f((zk - g.m) * a.c);
+  const float e = __builtin_amdgcn_exp2f((s.z[k] - g.m) * a.c);
   store_one<DT>(out, id, (float)((double)scale * ((double)e * g.share - p)));
 }
 
-template <int DT, bool REST, int PHASE, bool STEP>
+// Losses, by whole rows or from parts.
+template <int DT, bool REST, int PHASE, bool ONCE>
 __global__ __launch_bounds__(kRowThreads) void k_distill(DistillK a) {
-  extern __shared__ uint64_t memory[];
-  uint32_t* mask = reinterpret_cast<uint32_t*>(memory);  // REST, WHOLE and PARTS: [nseg * 64]
+  extern __shared__ uint32_t mask[];  // REST: [nseg * 64]
   __shared__ Part lds_parts[PHASE == PARTS ? 1 : kScoreMaxSegs];
   __shared__ Slots s;
-  __shared__ RowGrad row_grad;
+  __shared__ SlotSums sums[kDistillMaxK / 64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int waves = blockDim.x >> 6;
+  const size_t row = PHASE == PARTS ? blockIdx.x / a.groups : a.row0 + blockIdx.x;
+  const char* z = a.z + row * a.row_bytes;
+  const float w = a.weights ? a.weights[row] : 1.0f;
 
-  if constexpr (PHASE == PARTS) {
-    for (size_t w = blockIdx.x; w < a.rows * a.groups; w += gridDim.x) {
-      const size_t row = w / a.groups;
-      const int g = (int)(w % a.groups), per = (a.nseg + a.groups - 1) / a.groups;
-      if (load_slots(s, a, row) == 0) continue;
-      if (REST) build_mask<DT>(mask, s, a.nseg);
-      read_segs<DT, false, false>(a.z + row * a.row_bytes, a.V, g * per, min(a.nseg, (g + 1) * per), wave, waves, lane,
-                                  a.c, a.parts + row * a.nseg, nullptr, REST ? mask : nullptr);
+  if (REST)
+    for (int i = threadIdx.x; i < a.nseg * 64; i += blockDim.x) mask[i] = 0;
+  load_slots<DT, REST>(s, a, row, z);
+  __syncthreads();
+  // a row that does not count, or has no slots in use, is not read
+  const int state = w == 0.0f ? 0 : slots_state(s);
+  if (state) {
+    if (REST) {
+      if (threadIdx.x < kDistillMaxK && s.id[threadIdx.x] >= 0) mask_bit<DT>(mask, s.id[threadIdx.x]);
       __syncthreads();
     }
+    if constexpr (PHASE == PARTS) {
+      const int g = (int)(blockIdx.x % a.groups), per = (a.nseg + a.groups - 1) / a.groups;
+      read_segs<DT, false, false, ONCE>(z, a.V, g * per, min(a.nseg, (g + 1) * per), wave, waves, lane, a.c,
+                                        a.parts + row * a.nseg, nullptr, REST ? mask : nullptr);
+      return;
+    }
+    sum_slots<REST>(s, sums, waves, a.inv_t);
+    if constexpr (PHASE == WHOLE) {
+      read_segs<DT, false, false, ONCE>(z, a.V, 0, a.nseg, wave, waves, lane, a.c, lds_parts, nullptr,
+                                        REST ? mask : nullptr);
+    } else {
+      for (int i = threadIdx.x; i < a.nseg; i += kRowThreads) lds_parts[i] = a.parts[row * a.nseg + i];
+    }
+  }
+  if constexpr (PHASE == PARTS) return;
+  __syncthreads();
+  if (wave != 0) return;
+  RowStats st{};
+  if (state) st = join_row<DT, false>(z, a.V, a.nseg, lds_parts, REST ? mask : nullptr, a.c, lane);
+  float loss;
+  const RowGrad g = join_distill<REST>(a, st, sums, state, &loss);
+  if (lane == 0) {
+    a.loss[row] = state ? w * loss : 0.0f;
+    if (a.stats) reinterpret_cast<RowGrad*>(a.stats)[row] = g;
+  }
+}
+
+// A loss and its gradient.  Between the two a wave keeps its first NS segments of
+// the row in registers, so that they are read once; of longer rows (LONGER) the
+// rest is read again.
+template <int DT, bool REST, int NS, bool LONGER, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_distill_step(DistillK a) {
+  extern __shared__ uint32_t mask[];  // REST: [nseg * 64]
+  constexpr int waves = THREADS / 64;
+  __shared__ Part lds_parts[kScoreMaxSegs];
+  __shared__ Slots s;
+  __shared__ SlotSums sums[kDistillMaxK / 64];
+  __shared__ RowGrad row_grad;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const size_t row = a.row0 + blockIdx.x;
+  const char* z = a.z + row * a.row_bytes;
+  char* out = a.grad + row * a.grad_bytes;
+  const float w = a.weights ? a.weights[row] : 1.0f;
+  if (w == 0.0f) {  // a row that does not count is not read
+    for (int seg = wave; seg < a.nseg; seg += waves) zero_seg<DT>(out, seg, lane, a.V);
+    if (threadIdx.x == 0) a.loss[row] = 0.0f;
     return;
   }
+  Seg<DT> held[NS];
+#pragma unroll
+  for (int i = 0; i < NS; i++)
+    if (i * waves + wave < a.nseg) load_seg<DT, false>(held[i], z, i * waves + wave, lane, a.V);
+  if (REST)
+    for (int i = threadIdx.x; i < a.nseg * 64; i += THREADS) mask[i] = 0;
+  load_slots<DT, REST>(s, a, row, z);
+  __syncthreads();
+  const int state = slots_state(s);
+  if (REST) {
+    if (threadIdx.x < kDistillMaxK && s.id[threadIdx.x] >= 0) mask_bit<DT>(mask, s.id[threadIdx.x]);
+    __syncthreads();
+  }
+  sum_slots<REST>(s, sums, waves, a.inv_t);
+  auto reduce = [&](Seg<DT>& x, int seg) {
+    if (REST) {  // the listed logits' gradients are written by their slots
+      const uint32_t bits = mask[seg * 64 + lane];
+      if (__ballot(bits != 0)) mask_seg<DT>(x, bits);
+    }
+    const Part p = seg_part<DT, false>(x, lane_max<DT>(x), a.c);
+    if (lane == 0) lds_parts[seg] = p;
+    __builtin_amdgcn_sched_barrier(0);  // one segment's temporaries at a time
+  };
+#pragma unroll
+  for (int i = 0; i < NS; i++)
+    if (i * waves + wave < a.nseg) reduce(held[i], i * waves + wave);
+  if (LONGER)
+    for (int seg = NS * waves + wave; seg < a.nseg; seg += waves) {
+      Seg<DT> x;
+      load_seg<DT, false>(x, z, seg, lane, a.V);
+      reduce(x, seg);
+    }
+  __syncthreads();
 
-  for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const char* z = a.z + row * a.row_bytes;
-    const float w = a.weights ? a.weights[row] : 1.0f;
-    int state = load_slots(s, a, row);
-    if (w == 0.0f) state = 0;  // a row that does not count is not read
-    if (state) {
-      if (REST) build_mask<DT>(mask, s, a.nseg);
-      if constexpr (PHASE == WHOLE) {
-        read_segs<DT, false, false>(z, a.V, 0, a.nseg, wave, waves, lane, a.c, lds_parts, nullptr, REST ? mask : nullptr);
-      } else {
-        for (int i = threadIdx.x; i < a.nseg; i += kRowThreads) lds_parts[i] = a.parts[row * a.nseg + i];
+  // the wave that has the maximum's segment joins the row
+  const RowMax top = find_max(lds_parts, a.nseg, lane);
+  if (wave == top.first % waves) {
+    float rs = 0.0f, rw = 0.0f;
+    if (!top.none) {
+#pragma unroll
+      for (int i = 0; i < NS; i++)
+        if (top.first == i * waves + wave) sums_without_max<DT, false>(held[i], top.m, a.c, lane, rs, rw);
+      if (LONGER && top.first >= NS * waves) {
+        Seg<DT> y;
+        load_seg<DT, false>(y, z, top.first, lane, a.V);
+        if (REST) mask_seg<DT>(y, mask[top.first * 64 + lane]);
+        sums_without_max<DT, false>(y, top.m, a.c, lane, rs, rw);
       }
     }
-    __syncthreads();
-    if (wave == 0) {
-      float loss;
-      const RowGrad g = join_distill<DT, REST>(a, z, lds_parts, mask, s, state, lane, &loss);
-      if (lane == 0) {
-        row_grad = g;
-        if (a.loss) a.loss[row] = state ? w * loss : 0.0f;
-        if (a.stats) reinterpret_cast<RowGrad*>(a.stats)[row] = g;
-      }
-    }
-    __syncthreads();
-    if constexpr (STEP) {
-      const RowGrad g = row_grad;
-      const float scale = state ? w * a.T : 0.0f;
-      char* out = a.grad + row * a.grad_bytes;
-      const int k = threadIdx.x;
-      const bool patch = k < a.k && s.id[k] >= 0 && scale != 0.0f && g.m != -__builtin_inff();
-      const float zk = patch ? load_one<DT>(z, s.id[k]) : 0.0f;
-      __syncthreads();
-      grad_segs<DT>(a, z, out, g, scale, 0, a.nseg, wave, waves, lane);
-      __syncthreads();
-      if (patch) grad_slot<DT>(a, out, s, g, scale, k, zk);
-      __syncthreads();
+    float loss;
+    const RowGrad g =
+        join_distill<REST>(a, join_parts<false>(top, lds_parts, a.nseg, rs, rw, a.c, lane), sums, state, &loss);
+    if (lane == 0) {
+      row_grad = g;
+      a.loss[row] = state ? w * loss : 0.0f;
     }
   }
+  __syncthreads();
+  const RowGrad g = row_grad;
+  const float scale = state ? w * a.T : 0.0f;
+  const bool zero = grad_is_zero(g, scale);
+#pragma unroll
+  for (int i = 0; i < NS; i++) {
+    const int seg = i * waves + wave;
+    if (seg < a.nseg) {
+      if (zero)
+        zero_seg<DT>(out, seg, lane, a.V);
+      else
+        grad_seg<DT, true>(a, held[i], out, g, scale, seg, lane);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if (LONGER)
+    for (int seg = NS * waves + wave; seg < a.nseg; seg += waves) {
+      if (zero) {
+        zero_seg<DT>(out, seg, lane, a.V);
+      } else {
+        Seg<DT> x;
+        load_seg<DT, false>(x, z, seg, lane, a.V);
+        grad_seg<DT, true>(a, x, out, g, scale, seg, lane);
+      }
+    }
+  __syncthreads();
+  const int k = threadIdx.x;
+  if (!zero && k < a.k && s.id[k] >= 0) grad_slot<DT>(a, out, s, g, scale, k);
 }
 
 // The gradient alone, from the stats of the forward: workgroups of one chunk of
@@ -900,33 +1176,41 @@ template <int DT>
 __global__ __launch_bounds__(kGradWaves * 64) void k_distill_grad(DistillK a) {
   __shared__ Slots s;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  for (size_t w = blockIdx.x; w < a.rows * a.groups; w += gridDim.x) {
-    const size_t row = w / a.groups;
-    const int seg0 = (int)(w % a.groups) * kDistillChunk, seg1 = min(a.nseg, seg0 + kDistillChunk);
-    const char* z = a.z + row * a.row_bytes;
-    char* out = a.grad + row * a.grad_bytes;
-    const float weight = a.weights ? a.weights[row] : 1.0f;
-    const int state = load_slots(s, a, row);
-    const RowGrad g = reinterpret_cast<const RowGrad*>(a.stats)[row];
-    const float scale = state ? weight * a.T : 0.0f;
-    const int k = threadIdx.x, id = k < a.k ? s.id[k] : -1;
-    const bool patch = id >= seg0 * kScoreSeg && id < seg1 * kScoreSeg && scale != 0.0f && g.m != -__builtin_inff();
-    const float zk = patch ? load_one<DT>(z, id) : 0.0f;
-    __syncthreads();
-    grad_segs<DT>(a, z, out, g, scale, seg0, seg1, wave, kGradWaves, lane);
-    __syncthreads();
-    if (patch) grad_slot<DT>(a, out, s, g, scale, k, zk);
-    __syncthreads();
+  const size_t row = a.row0 + blockIdx.x / a.groups;
+  const int seg0 = (int)(blockIdx.x % a.groups) * kDistillChunk, seg1 = min(a.nseg, seg0 + kDistillChunk);
+  const char* z = a.z + row * a.row_bytes;
+  char* out = a.grad + row * a.grad_bytes;
+  const float weight = a.weights ? a.weights[row] : 1.0f;
+  const RowGrad g = reinterpret_cast<const RowGrad*>(a.stats)[row];
+  load_slots<DT, false>(s, a, row, z);
+  __syncthreads();
+  const float scale = slots_state(s) ? weight * a.T : 0.0f;
+  const bool zero = grad_is_zero(g, scale);
+  for (int seg = seg0 + wave; seg < seg1; seg += kGradWaves) {
+    if (zero) {
+      zero_seg<DT>(out, seg, lane, a.V);
+    } else {
+      Seg<DT> x;
+      load_seg<DT, false>(x, z, seg, lane, a.V);
+      grad_seg<DT, false>(a, x, out, g, scale, seg, lane);
+    }
   }
+  __syncthreads();
+  const int k = threadIdx.x, id = s.id[k];
+  if (!zero && id >= seg0 * kScoreSeg && id < seg1 * kScoreSeg) grad_slot<DT>(a, out, s, g, scale, k);
 }
-static_assert(kGradWaves * 64 >= kDistillMaxK && kRowThreads >= kDistillMaxK, "a thread a slot");
+static_assert(kGradWaves * 64 == kDistillMaxK && kRowThreads >= kDistillMaxK && kPartThreads >= kDistillMaxK,
+              "a thread a slot");
 
 // ---- launches ---------------------------------------------------------------------------
 
-// Rows from which on a row is one workgroup's: fewer would leave compute units
-// idle, and go to several workgroups each with a second launch to join them.
-constexpr size_t kWholeRows = 256;
-constexpr int kPartThreads = 256;
+// Whether a row is one workgroup's.  Few long rows would leave compute units idle
+// and go to several workgroups each, with a second launch to join them.  us by
+// whole rows / in parts, scores of bf16: 1 row of 32000 6.2 / 6.6, of 151936 15.1 /
+// 7.0; 64 rows 15.8 / 10.2, 128 rows 18.0 / 15.8, 255 rows 20.0 / 23.2; of 262144
+// 128 rows 27.0 / 20.5, 255 rows 28.7 / 32.3; a step of 64 rows of 151936 29.7 /
+// 25.8, 128 rows 32.1 / 34.1.
+bool whole_rows(size_t rows, int nseg) { return nseg <= 24 || rows >= 160; }
 
 int segments(size_t vocab) { return (int)((vocab + kScoreSeg - 1) / kScoreSeg); }
 
@@ -938,10 +1222,31 @@ int part_groups(size_t rows, int nseg) {
   return (int)(most < enough ? most : enough);
 }
 
-unsigned grid_of(size_t n) { return (unsigned)(n < (1u << 20) ? n : (1u << 20)); }
+// A launch of `per_row` workgroups a row; of many rows several, of as many as
+// keep the launch's threads below 2^32 (a row has 16 workgroups of 256 at most).
+constexpr size_t kRowsPerLaunch = 1u << 18;
+template <typename K>
+void launch_rows(void (*kernel)(K), size_t rows, int per_row, int threads, size_t lds, hipStream_t s, K k) {
+  for (k.row0 = 0; k.row0 < rows; k.row0 += kRowsPerLaunch) {
+    const size_t n = rows - k.row0 < kRowsPerLaunch ? rows - k.row0 : kRowsPerLaunch;
+    launch_kernel(kernel, dim3((unsigned)(n * per_row)), dim3(threads), lds, s, k);
+  }
+}
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// Reads that bypass the caches reach 7.0 TB/s instead of 6.2 on 1.24 GB of
+// logits, but leave nothing behind: a backward pass over 32 MB of them takes 18.6
+// us instead of 15.0.  So only where the logits are larger than the cache.
+bool read_once(size_t rows, size_t row_bytes) { return rows * row_bytes > (size_t)256 << 20; }
+
+template <typename F>
+void by_bool(bool b, F&& f) {
+  if (b)
+    f(std::true_type());
+  else
+    f(std::false_type());
+}
 template <typename F>
 void by_type(int dtype, F&& f) {
   if (dtype == DTL_F32)
@@ -956,8 +1261,8 @@ size_t type_bytes(int dtype) { return dtype == DTL_F32 ? 4 : 2; }
 }  // namespace
 
 size_t score_scratch_bytes(size_t rows, size_t vocab, size_t top) {
-  if (rows >= kWholeRows) return 0;
   const size_t nseg = segments(vocab);
+  if (whole_rows(rows, (int)nseg)) return 0;
   return round256(rows * nseg * sizeof(Part)) + (top ? rows * nseg * 64 * 4 : 0);
 }
 
@@ -966,7 +1271,6 @@ void launch_token_scores(const ScoreArgs& a, hipStream_t s) {
   ScoreK k{};
   k.z = static_cast<const char*>(a.z);
   k.row_bytes = a.stride * type_bytes(a.dtype);
-  k.rows = a.rows;
   k.V = a.vocab;
   k.nseg = segments(a.vocab);
   k.tokens = a.tokens;
@@ -985,19 +1289,20 @@ void launch_token_scores(const ScoreArgs& a, hipStream_t s) {
     if (lds < (size_t)k.nseg * 256) lds = (size_t)k.nseg * 256;
   }
   by_type(a.dtype, [&](auto dt) {
-    constexpr int DT = decltype(dt)::value;
-    if (a.rows >= kWholeRows) {
-      launch_kernel(a.top ? k_scores<DT, true, WHOLE> : k_scores<DT, false, WHOLE>, dim3(grid_of(a.rows)),
-                    dim3(kRowThreads), lds, s, k);
-      return;
-    }
-    k.groups = part_groups(a.rows, k.nseg);
-    k.parts = static_cast<Part*>(a.scratch);
-    k.keys = reinterpret_cast<uint32_t*>(static_cast<char*>(a.scratch) + round256(a.rows * k.nseg * sizeof(Part)));
-    launch_kernel(a.top ? k_scores<DT, true, PARTS> : k_scores<DT, false, PARTS>, dim3(grid_of(a.rows * k.groups)),
-                  dim3(kPartThreads), 0, s, k);
-    launch_kernel(a.top ? k_scores<DT, true, JOIN> : k_scores<DT, false, JOIN>, dim3(grid_of(a.rows)),
-                  dim3(kRowThreads), lds, s, k);
+    by_bool(a.top != 0, [&](auto with_top) {
+      constexpr int DT = decltype(dt)::value;
+      constexpr bool TOP = decltype(with_top)::value;
+      if (whole_rows(a.rows, k.nseg)) {
+        launch_rows(read_once(a.rows, k.row_bytes) ? k_scores<DT, TOP, WHOLE, true> : k_scores<DT, TOP, WHOLE, false>,
+                    a.rows, 1, kRowThreads, lds, s, k);
+        return;
+      }
+      k.groups = part_groups(a.rows, k.nseg);
+      k.parts = static_cast<Part*>(a.scratch);
+      k.keys = reinterpret_cast<uint32_t*>(static_cast<char*>(a.scratch) + round256(a.rows * k.nseg * sizeof(Part)));
+      launch_rows(k_scores<DT, TOP, PARTS, false>, a.rows, k.groups, kPartThreads, 0, s, k);
+      launch_rows(k_scores<DT, TOP, JOIN, false>, a.rows, 1, kRowThreads, lds, s, k);
+    });
   });
 }
 
@@ -1008,7 +1313,6 @@ void launch_token_scores_grad(const ScoreGradArgs& a, hipStream_t s) {
   k.grad = static_cast<char*>(a.grad);
   k.row_bytes = a.stride * type_bytes(a.dtype);
   k.grad_bytes = a.grad_stride * type_bytes(a.dtype);
-  k.rows = a.rows;
   k.V = a.vocab;
   k.nseg = segments(a.vocab);
   k.chunks = (k.nseg + kGradWaves * kGradSegs - 1) / (kGradWaves * kGradSegs);
@@ -1022,8 +1326,8 @@ void launch_token_scores_grad(const ScoreGradArgs& a, hipStream_t s) {
   k.h = a.g_entropy;
   by_type(a.dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    launch_kernel(a.g_entropy ? k_scores_grad<DT, true> : k_scores_grad<DT, false>,
-                  dim3(grid_of(a.rows * k.chunks)), dim3(kGradWaves * 64), 0, s, k);
+    launch_rows(a.g_entropy ? k_scores_grad<DT, true> : k_scores_grad<DT, false>, a.rows, k.chunks, kGradWaves * 64, 0,
+                s, k);
   });
 }
 
@@ -1034,7 +1338,6 @@ DistillK distill_kernel_args(const DistillArgs& a) {
   k.grad = static_cast<char*>(a.grad);
   k.row_bytes = a.stride * type_bytes(a.dtype);
   k.grad_bytes = a.grad_stride * type_bytes(a.dtype);
-  k.rows = a.rows;
   k.V = a.vocab;
   k.nseg = segments(a.vocab);
   k.ids = a.ids;
@@ -1053,7 +1356,7 @@ DistillK distill_kernel_args(const DistillArgs& a) {
 
 // Parts, and for a step of few rows the stats between its launches.
 size_t distill_scratch_bytes(size_t rows, size_t vocab, bool step) {
-  if (rows >= kWholeRows) return 0;
+  if (whole_rows(rows, segments(vocab))) return 0;
   return round256(rows * segments(vocab) * sizeof(Part)) + (step ? rows * sizeof(RowGrad) : 0);
 }
 
@@ -1062,35 +1365,56 @@ void launch_distill_grad(const DistillArgs& a, hipStream_t s) {
   DistillK k = distill_kernel_args(a);
   k.groups = (k.nseg + kDistillChunk - 1) / kDistillChunk;
   by_type(a.dtype, [&](auto dt) {
-    launch_kernel(k_distill_grad<decltype(dt)::value>, dim3(grid_of(a.rows * k.groups)), dim3(kGradWaves * 64), 0, s, k);
+    launch_rows(k_distill_grad<decltype(dt)::value>, a.rows, k.groups, kGradWaves * 64, 0, s, k);
   });
 }
+
+namespace {
+template <int DT, bool REST, int NS, bool LONGER, int THREADS>
+void launch_step_as(const DistillK& k, size_t rows, hipStream_t s) {
+  launch_rows(k_distill_step<DT, REST, NS, LONGER, THREADS>, rows, 1, THREADS, REST ? (size_t)k.nseg * 256 : 0, s, k);
+}
+// A step of whole rows.  Eight waves and two segments a wave in registers leave
+// room for two or three workgroups a compute unit, one reading while another
+// writes; us of 4096 rows with sixteen waves and every segment held / eight and
+// two / eight and three: vocabularies of 32000 bf16 189 / 135 / -, 49152 bf16 233
+// / 174 / 200, 151936 bf16 773 / 538 / 515, 32000 f32 286 / 202 / -, 49152 f32 337
+// / 314 / 329; 2048 rows of 151936 f32 - / 556 / -.
+template <int DT, bool REST>
+void launch_step(const DistillK& k, size_t rows, hipStream_t s) {
+  if (k.nseg <= 4) return launch_step_as<DT, REST, 1, false, 256>(k, rows, s);
+  if (k.nseg <= 8) return launch_step_as<DT, REST, 1, false, 512>(k, rows, s);
+  if (k.nseg <= 16) return launch_step_as<DT, REST, 2, false, 512>(k, rows, s);
+  if (DT == DTL_F32 || k.nseg <= 32) return launch_step_as<DT, REST, 2, true, 512>(k, rows, s);
+  if constexpr (DT != DTL_F32) launch_step_as<DT, REST, 3, true, 512>(k, rows, s);
+}
+}  // namespace
 
 void launch_distill(const DistillArgs& a, hipStream_t s) {
   if (a.rows == 0) return;
   DistillK k = distill_kernel_args(a);
   const size_t lds = a.rest ? (size_t)k.nseg * 256 : 0;
   by_type(a.dtype, [&](auto dt) {
-    constexpr int DT = decltype(dt)::value;
-    if (a.rows >= kWholeRows) {
+    by_bool(a.rest, [&](auto with_rest) {
+      constexpr int DT = decltype(dt)::value;
+      constexpr bool REST = decltype(with_rest)::value;
+      if (whole_rows(a.rows, k.nseg)) {
+        if (a.grad)
+          launch_step<DT, REST>(k, a.rows, s);
+        else
+          launch_rows(read_once(a.rows, k.row_bytes) ? k_distill<DT, REST, WHOLE, true> : k_distill<DT, REST, WHOLE, false>,
+                      a.rows, 1, kRowThreads, lds, s, k);
+        return;
+      }
+      k.groups = part_groups(a.rows, k.nseg);
+      k.parts = static_cast<Part*>(a.scratch);
       if (a.grad)
-        launch_kernel(a.rest ? k_distill<DT, true, WHOLE, true> : k_distill<DT, false, WHOLE, true>,
-                      dim3(grid_of(a.rows)), dim3(kRowThreads), lds, s, k);
-      else
-        launch_kernel(a.rest ? k_distill<DT, true, WHOLE, false> : k_distill<DT, false, WHOLE, false>,
-                      dim3(grid_of(a.rows)), dim3(kRowThreads), lds, s, k);
-      return;
-    }
-    k.groups = part_groups(a.rows, k.nseg);
-    k.parts = static_cast<Part*>(a.scratch);
-    if (a.grad)
-      k.stats = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + round256(a.rows * k.nseg * sizeof(Part)));
-    launch_kernel(a.rest ? k_distill<DT, true, PARTS, false> : k_distill<DT, false, PARTS, false>,
-                  dim3(grid_of(a.rows * k.groups)), dim3(kPartThreads), lds, s, k);
-    launch_kernel(a.rest ? k_distill<DT, true, JOIN, false> : k_distill<DT, false, JOIN, false>, dim3(grid_of(a.rows)),
-                  dim3(kRowThreads), lds, s, k);
+        k.stats = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + round256(a.rows * k.nseg * sizeof(Part)));
+      launch_rows(k_distill<DT, REST, PARTS, false>, a.rows, k.groups, kPartThreads, lds, s, k);
+      launch_rows(k_distill<DT, REST, JOIN, false>, a.rows, 1, kRowThreads, lds, s, k);
+    });
   });
-  if (a.grad && a.rows < kWholeRows) {
+  if (a.grad && !whole_rows(a.rows, k.nseg)) {
     DistillArgs b = a;
     b.stats = k.stats;
     launch_distill_grad(b, s);

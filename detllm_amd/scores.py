@@ -18,6 +18,7 @@ the same for this library's own sessions, without torch.
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -101,14 +102,30 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+# Without their wrappers: a call on a few rows is as short as its host side.
+_device_now = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(device: torch.device, entry, *args) -> None:
     """The entry point on the current stream of `device`."""
-    if device.index == torch.cuda.current_device():
-        status = entry(*args, torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    if index == _device_now():
+        status = entry(*args, _stream_of(index))
     else:
-        with torch.cuda.device(device):
-            status = entry(*args, torch.cuda.current_stream().cuda_stream)
-    check(status, entry.__name__)
+        with torch.cuda.device(index):
+            status = entry(*args, _stream_of(index))
+    if status:
+        check(status, entry.__name__)
+
+
+_scores_scratch = lru_cache(maxsize=256)(lib.dtl_token_scores_scratch)
+_distill_scratch = lru_cache(maxsize=256)(lib.dtl_distill_scratch)
+
+
+def _scratch(n: int, device: torch.device) -> Optional[torch.Tensor]:
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 # ---- scores ------------------------------------------------------------------
@@ -117,14 +134,16 @@ def _call(device: torch.device, entry, *args) -> None:
 def _scores(logits, tokens, top, temperature, stats):
     z = _logits_view(logits)
     lead, dev = logits.shape[:-1], logits.device
-    out = {"dtype": torch.float32, "device": dev}
-    log_probs = torch.empty(lead, **out) if tokens is not None else None
-    entropy = torch.empty(lead, **out)
-    ids = torch.empty(*lead, top, dtype=torch.int32, device=dev) if top else None
-    lps = torch.empty(*lead, top, **out) if top else None
-    st = torch.empty(z.rows, 2, **out) if stats else None
-    n = lib.dtl_token_scores_scratch(z.rows, z.vocab, top)
-    scratch = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    log_probs = torch.empty(lead, dtype=torch.float32, device=dev) if tokens is not None else None
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+    ids = lps = st = None
+    if top:
+        ids = torch.empty((*lead, top), dtype=torch.int32, device=dev)
+        lps = torch.empty((*lead, top), dtype=torch.float32, device=dev)
+    if stats:
+        st = torch.empty((z.rows, 2), dtype=torch.float32, device=dev)
+    n = _scores_scratch(z.rows, z.vocab, top)
+    scratch = _scratch(n, dev)
     _call(dev, lib.dtl_token_scores, C.byref(z), _ptr(tokens), 0 if tokens is None else tokens.element_size(),
           temperature, top, _ptr(log_probs), _ptr(entropy), _ptr(st), _ptr(ids), _ptr(lps), _ptr(scratch), n)
     return log_probs, entropy, ids, lps, st
@@ -177,8 +196,11 @@ def _teacher(logits, ids, log_probs, rest):
     shape = (*logits.shape[:-1], k)
     ids = _beside(ids, logits, shape, _INDEX, "teacher_ids")
     log_probs = _beside(log_probs, logits, shape, _FLOAT, "teacher_log_probs")
-    t = _lib.Teacher(ids.data_ptr(), ids.element_size(), C.cast(log_probs.data_ptr(), _lib.f32p), k, int(bool(rest)))
-    return t, ids, log_probs
+    return _teacher_view(ids, log_probs, rest), ids, log_probs
+
+
+def _teacher_view(ids, log_probs, rest) -> _lib.Teacher:
+    return _lib.Teacher(ids.data_ptr(), ids.element_size(), log_probs.data_ptr(), ids.shape[-1], int(bool(rest)))
 
 
 def _distill(logits, ids, log_probs, temperature, rest, stats):
@@ -187,8 +209,8 @@ def _distill(logits, ids, log_probs, temperature, rest, stats):
     dev = logits.device
     loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
     st = torch.empty(z.rows, 5, dtype=torch.float32, device=dev) if stats else None
-    n = lib.dtl_distill_scratch(z.rows, z.vocab)
-    scratch = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    n = _distill_scratch(z.rows, z.vocab)
+    scratch = _scratch(n, dev)
     _call(dev, lib.dtl_distill, C.byref(z), C.byref(t), temperature, _ptr(loss), _ptr(st), _ptr(scratch), n)
     return loss, ids, log_probs, st
 
@@ -207,7 +229,7 @@ class _Distill(torch.autograd.Function):
         logits, ids, log_probs, stats = ctx.saved_tensors
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         z = _logits_view(logits)
-        t, ids, log_probs = _teacher(logits, ids, log_probs, ctx.rest)
+        t = _teacher_view(ids, log_probs, ctx.rest)
         g = g.contiguous()
         _call(logits.device, lib.dtl_distill_backward, C.byref(z), C.byref(t), ctx.temperature, _ptr(stats), _ptr(g),
               _ptr(grad), z.vocab)
@@ -250,8 +272,8 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
             raise ValueError("out must have the shape, type and device of logits")
         stride = _logits_view(out, "out").stride
     loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
-    n = lib.dtl_distill_scratch(z.rows, z.vocab)
-    scratch = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    n = _distill_scratch(z.rows, z.vocab)
+    scratch = _scratch(n, dev)
     _call(dev, lib.dtl_distill_step, C.byref(z), C.byref(t), float(temperature), _ptr(weights), _ptr(loss),
           out.data_ptr(), stride, _ptr(scratch), n)
     return loss, out

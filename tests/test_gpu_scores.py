@@ -150,10 +150,9 @@ def test_scores_over_vocabularies(hip, rows, vocab, dtype):
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("kind", ["masked", "equal", "lowest", "lowest_mask", "sorted", "few", "sure", "zeros", "huge",
                                   "mixed"])
-@pytest.mark.parametrize("rows", [4, 260])  # in parts and by whole rows
-def test_scores_of_logits_that_go_wrong(hip, rows, kind, dtype):
+@pytest.mark.parametrize("rows,vocab", [(4, 60001), (260, 5003)])  # in parts and by whole rows
+def test_scores_of_logits_that_go_wrong(hip, rows, vocab, kind, dtype):
     rng = np.random.default_rng(len(kind))
-    vocab = 5003
     z = make(rng, rows, vocab, kind)
     if dtype == "f16" and "lowest" in kind:
         z = np.maximum(z, -65504.0)
@@ -185,11 +184,11 @@ def test_tokens_out_of_the_vocabulary(hip):
 def test_rows_give_the_same_bits_alone_and_among_others(hip, dtype):
     """Row by row, in parts, whole, misaligned: a row's results depend on the row."""
     rng = np.random.default_rng(8)
-    vocab, rows = 10001, 300
+    vocab, rows = 60001, 180
     z = make(rng, rows, vocab)
     tokens = pick_tokens(rng, z)
     all_ = run_scores(hip, Logits(hip, z, dtype), tokens, 0.7, 40)
-    for lo, hi, pad, offset in ((0, 1, 0, 0), (7, 8, 3, 2), (100, 120, 1, 6), (20, 299, 64, 0)):
+    for lo, hi, pad, offset in ((0, 1, 0, 0), (7, 8, 3, 2), (100, 120, 1, 6), (12, 179, 64, 0)):
         offset = offset * 2 if dtype == "f32" else offset
         part = run_scores(hip, Logits(hip, z[lo:hi], dtype, pad, offset), tokens[lo:hi], 0.7, 40)
         for k in ("lp", "h", "stats", "lps"):
@@ -262,13 +261,13 @@ def make_teacher(rng, z, k, rest=True):
 
 def run_distill(hip, lg, ids, v, T, rest, weights, wide=True, pad=0, offset=0, in_place=False):
     """(loss, gradient by the step, loss, gradient by forward and backward)"""
-    from detllm_amd._lib import Teacher, f32p
+    from detllm_amd._lib import Teacher
 
     dt, size, _ = DTYPES[lg.dtype]
     bits = np.dtype(f"u{size}")
     R = lg.rows
     dv = hip.put(v.astype(np.float32))
-    t = Teacher(hip.put(ids.astype(np.int64 if wide else np.int32)), 8 if wide else 4, C.cast(dv, f32p), ids.shape[1],
+    t = Teacher(hip.put(ids.astype(np.int64 if wide else np.int32)), 8 if wide else 4, dv, ids.shape[1],
                 int(rest))
     w = hip.put(np.asarray(weights, np.float32))
     n = hip.dtl.dtl_distill_scratch(R, lg.vocab)
@@ -310,24 +309,25 @@ def check_distill(hip, lg, ids, v, T, rest, weights, wide=True, step=1, **kw):
 @pytest.mark.parametrize("rest", [False, True])
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("rows,vocab,k", [(1, 1, 1), (1, 2, 1), (3, 7, 4), (2, 2048, 256), (3, 2049, 17), (5, 32003, 20),
-                                          (2, 151936, 100), (1, 1 << 18, 256), (258, 4099, 31)])
+                                          (2, 151936, 100), (1, 1 << 18, 256), (258, 4099, 31), (20, 13001, 9),
+                                          (3, 30011, 64), (160, 60003, 12), (160, 151937, 40)])
 def test_distillation(hip, rows, vocab, k, dtype, rest):
     rng = np.random.default_rng(vocab + k)
     z = make(rng, rows, vocab)
     lg = Logits(hip, z, dtype, pad=2)
     ids, v = make_teacher(rng, lg.z, k)
     w = rng.uniform(-1, 2, rows).astype(np.float32)
-    check_distill(hip, lg, ids, v, 2.0, rest, w, wide=bool(k % 2), step=1 if rows < 10 else 43, pad=1,
+    check_distill(hip, lg, ids, v, 2.0, rest, w, wide=bool(k % 2), step=1 if rows < 10 else rows // 4, pad=1,
                   offset=2 * DTYPES[dtype][1])
 
 
 @pytest.mark.parametrize("rest", [False, True])
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("kind", ["masked", "equal", "lowest", "lowest_mask", "few", "sure", "mixed"])
-@pytest.mark.parametrize("rows", [6, 261])
-def test_distillation_of_logits_that_go_wrong(hip, rows, kind, dtype, rest):
+@pytest.mark.parametrize("rows,vocab", [(6, 55001), (261, 2311)])
+def test_distillation_of_logits_that_go_wrong(hip, rows, vocab, kind, dtype, rest):
     rng = np.random.default_rng(len(kind) + 1)
-    vocab, k = 2311, 12
+    k = 12
     z = make(rng, rows, vocab, kind)
     if dtype == "f16":
         z = np.where(np.isfinite(z), np.clip(z, -65504.0, 65504.0), z).astype(np.float32)
@@ -343,11 +343,11 @@ def test_distillation_of_logits_that_go_wrong(hip, rows, kind, dtype, rest):
 
 
 @pytest.mark.parametrize("rest", [False, True])
-@pytest.mark.parametrize("rows", [9, 270])
-def test_teachers_that_go_wrong(hip, rows, rest):
+@pytest.mark.parametrize("rows,vocab", [(9, 60000), (270, 1500)])
+def test_teachers_that_go_wrong(hip, rows, vocab, rest):
     """Empty slots and rows, ids twice, ids outside, broken log probabilities, lists of the whole vocabulary."""
     rng = np.random.default_rng(3)
-    vocab, k = 1500, 40
+    k = 40
     z = make(rng, rows, vocab)
     z[8] = np.nan  # an empty list: not looked at
     lg = Logits(hip, z, "f32")
@@ -372,15 +372,15 @@ def test_teachers_that_go_wrong(hip, rows, rest):
     check_distill(hip, lg, ids, v, 1.0, rest, [1.0, 0.5, 1.0])
 
 
-@pytest.mark.parametrize("rows", [3, 280])
-def test_distillation_in_place_and_by_rows(hip, rows):
+@pytest.mark.parametrize("rows,vocab", [(3, 60100), (280, 4100), (165, 50001), (161, 152001)])
+def test_distillation_in_place_and_by_rows(hip, rows, vocab):
     """The gradient over the logits themselves, and the same bits for rows alone as among others."""
     rng = np.random.default_rng(4)
-    vocab, k = 4100, 33
+    k = 33
     z = make(rng, rows, vocab)
     ids, v = make_teacher(rng, z, k)
     w = rng.uniform(0, 1, rows).astype(np.float32)
-    for dtype in DTYPES:
+    for dtype in DTYPES if vocab < 100000 else ("bf16",):
         for rest in (False, True):
             want = run_distill(hip, Logits(hip, z, dtype, pad=1), ids, v, 1.0, rest, w)
             got = run_distill(hip, Logits(hip, z, dtype, pad=1), ids, v, 1.0, rest, w, in_place=True)
@@ -396,10 +396,10 @@ def test_distillation_in_place_and_by_rows(hip, rows):
 
 def test_a_teachers_scores_into_a_students_step_in_a_graph(hip):
     """Alternatives of one model straight into the other's loss and gradient, captured and replayed."""
-    from detllm_amd._lib import Teacher, f32p
+    from detllm_amd._lib import Teacher
 
     rng = np.random.default_rng(12)
-    rows, vocab, k, T = 6, 12001, 24, 2.0
+    rows, vocab, k, T = 6, 52001, 24, 2.0
     zt, zs = make(rng, rows, vocab), make(rng, rows, vocab)
     teacher, student = Logits(hip, zt, "f32"), Logits(hip, zs, "bf16")
     f = lambda *s: hip.put(np.zeros(s, np.float32))
@@ -407,7 +407,7 @@ def test_a_teachers_scores_into_a_students_step_in_a_graph(hip):
     grad = hip.put(np.zeros((rows, vocab), np.uint16))
     s1, n1 = scratch(hip, hip.dtl.dtl_token_scores_scratch(rows, vocab, k))
     s2, n2 = scratch(hip, hip.dtl.dtl_distill_scratch(rows, vocab))
-    t = Teacher(ids, 4, C.cast(lps, f32p), k, 1)
+    t = Teacher(ids, 4, lps, k, 1)
 
     def both(stream):
         assert hip.dtl.dtl_token_scores(C.byref(teacher.c), None, 0, T, k, None, None, None, ids, lps, s1, n1, stream) == 0

@@ -17,9 +17,9 @@ P = 1 << 20  # an address that is never read
 
 def _calls(z, ids=P, id_bytes=4, v=P, k=4, T=1.0, tokens=P, token_bytes=8, top=2, out=P, stride=None, scratch=P, n=1 << 30):
     """The status of each entry point for these arguments (all refuse, or have no rows)."""
-    from detllm_amd._lib import Teacher, f32p, lib
+    from detllm_amd._lib import Teacher, lib
 
-    t = Teacher(ids, id_bytes, C.cast(v, f32p), k, 0)
+    t = Teacher(ids, id_bytes, v, k, 0)
     stride = z.vocab if stride is None else stride
     z = C.byref(z)
     return {
@@ -74,9 +74,10 @@ def test_refusals():
     _expect(INVALID, ALL[2:], _view(), ids=0)
     _expect(INVALID, ALL[2:], _view(), v=0)
     scratch = ("scores", "distill", "distill_step")
-    _expect(SMALL, scratch, _view(), n=8)
-    _expect(INVALID, scratch, _view(), scratch=0)
-    _expect(INVALID, scratch, _view(), scratch=P + 8)
+    long = _view(vocab=100000, stride=100000)
+    _expect(SMALL, scratch, long, n=8)
+    _expect(INVALID, scratch, long, scratch=0)
+    _expect(INVALID, scratch, long, scratch=P + 8)
 
 
 def test_missing_outputs_and_structs():
@@ -102,11 +103,12 @@ def test_no_rows_are_no_error():
 def test_scratch_sizes():
     from detllm_amd._lib import lib
 
-    for rows, vocab, top in ((1, 1, 0), (1, 32000, 1), (8, 151936, 20), (255, 1 << 18, 128)):
+    for rows, vocab, top in ((1, 100000, 0), (8, 151936, 20), (150, 1 << 18, 128)):
         seg = -(-vocab // 2048)
         assert lib.dtl_token_scores_scratch(rows, vocab, top) >= rows * seg * (12 + (256 if top else 0))
         assert lib.dtl_distill_scratch(rows, vocab) >= rows * seg * 12 + rows * 20
-    assert lib.dtl_token_scores_scratch(4096, 151936, 64) == 0
+    for rows, vocab in ((1, 1), (1, 32000), (4096, 151936)):
+        assert lib.dtl_token_scores_scratch(rows, vocab, 1) == 0 == lib.dtl_distill_scratch(rows, vocab)
 
 
 def test_oracle_gradients_against_differences():
