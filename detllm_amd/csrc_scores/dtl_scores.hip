@@ -18,11 +18,10 @@
 namespace dtl {
 namespace {
 
-constexpr int kRowThreads = 512;
-constexpr int kRowWaves = kRowThreads / 64;
+constexpr int kJoinThreads = 512;
 constexpr int kPartThreads = 256;
 constexpr int kPer = kScoreSeg / 64;  // logits a lane holds of a segment
-constexpr int kKeysPerThread = kScoreMaxSegs / kRowWaves;
+constexpr int kMostWaves = 16;  // of a row's workgroup
 constexpr double kLog2E = 1.4426950408889634074;
 constexpr double kLn2 = 0.6931471805599453094;
 
@@ -367,8 +366,8 @@ __device__ __forceinline__ float of_order(uint32_t k) {
 
 struct alignas(16) TopLds {
   uint32_t bins[4][256];
-  uint32_t low[kRowWaves], high[kRowWaves];
-  uint32_t counts[2][kRowWaves];
+  uint32_t low[kMostWaves], high[kMostWaves];
+  uint32_t counts[2][kMostWaves];
   uint32_t buckets, candidates, chosen;
   uint16_t ties[kScoreMaxSegs];
   uint16_t bucket[kScoreMaxTop + 64];
@@ -390,20 +389,46 @@ __device__ __forceinline__ uint32_t append(uint32_t* length, uint32_t n, int lan
 
 // How many of the workgroup's flags are set, for step `step` of a loop: the two
 // sets of counts let one barrier a step do.
+template <int WAVES>
 __device__ __forceinline__ int group_count(TopLds& t, int step, int in_wave, int wave, int lane) {
   if (lane == 0) t.counts[step & 1][wave] = in_wave;
   __syncthreads();
   int n = 0;
 #pragma unroll
-  for (int w = 0; w < kRowWaves; w++) n += t.counts[step & 1][w];
+  for (int w = 0; w < WAVES; w++) n += t.counts[step & 1][w];
   return n;
 }
 
+// A thread's keys: those of its lane in segments wave, wave + WAVES, ...
+template <int WAVES>
+struct Keys {
+  uint32_t k[kScoreMaxSegs / WAVES];
+};
+// Before the barrier that precedes select_top: the keys into registers from
+// keys[nseg * 64], the order of the largest logit of each bucket (a lane's share
+// of a segment), and what the workgroup's threads say of them.
+template <int WAVES>
+__device__ __forceinline__ void take_keys(Keys<WAVES>& key, const uint32_t* keys, int nseg, TopLds& t) {
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < kScoreMaxSegs / WAVES; i++) {
+    key.k[i] = i * WAVES + wave < nseg ? keys[i * (WAVES * 64) + tid] : 0;
+    most = max(most, key.k[i]);
+  }
+  const uint32_t low = ~wave_max(~most), high = wave_max(most);
+  if ((tid & 63) == 0) {
+    t.low[wave] = low;
+    t.high[wave] = high;
+  }
+  for (int i = tid; i < 4 * 256; i += WAVES * 64) (&t.bins[0][0])[i] = 0;
+  if (tid == 0) t.buckets = t.candidates = t.chosen = 0;
+}
+
 // The `top` largest logits of a row in order (value, then the lower index), by
-// the whole workgroup, from keys[nseg * 64]: the order of the largest logit of
-// each bucket, a lane's share of a segment.  Put the buckets in the order of
-// their largest logits: the row's `top` largest lie in the first `top` buckets,
-// since each of those holds one that is as large.  So:
+// the whole workgroup.  Put the buckets in the order of their largest logits: the
+// row's `top` largest lie in the first `top` buckets, since each of those holds
+// one that is as large.  So:
 //   1. tau, such that at least `top` buckets reach it and few more, by counting
 //      keys in 256 equal steps of an interval, then of the step that holds key
 //      `top`, four times at most, mostly once.  It starts at a key that a whole
@@ -413,32 +438,19 @@ __device__ __forceinline__ int group_count(TopLds& t, int step, int in_wave, int
 //   3. their logits from tau on, read again (32 a bucket);
 //   4. these ranked by counting, each against each.
 // All but 3 is in LDS and registers, whatever the logits hold: rows of equal
-// logits take the same steps.  keys' memory is used again for the candidates.
-// `aside` is called once between 2 and 3 and may keep one wave busy; its results
-// are there when `emit` is called.
-template <int DT, typename Aside, typename Emit>
-__device__ __forceinline__ void select_top(const char* row, int V, int nseg, int top, uint64_t* memory, TopLds& t, Aside&& aside,
-                           Emit&& emit) {
+// logits take the same steps.  `memory` holds the candidates; it may be the keys'.
+// `aside` is the first wave's, which takes no part in 3; its results are there
+// when `emit` is called.
+template <int DT, int WAVES, typename Aside, typename Emit>
+__device__ __forceinline__ void select_top(const char* row, int V, int nseg, int top, const Keys<WAVES>& keys,
+                                           uint64_t* memory, TopLds& t, Aside&& aside, Emit&& emit) {
+  constexpr int threads = WAVES * 64, per_thread = kScoreMaxSegs / WAVES;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t* keys = reinterpret_cast<const uint32_t*>(memory);
-  uint32_t key[kKeysPerThread], most = 0;
-#pragma unroll
-  for (int i = 0; i < kKeysPerThread; i++) {
-    key[i] = i * kRowWaves + wave < nseg ? keys[i * kRowThreads + tid] : 0;
-    most = max(most, key[i]);
-  }
-  const uint32_t low = ~wave_max(~most), high = wave_max(most);
-  if (lane == 0) {
-    t.low[wave] = low;
-    t.high[wave] = high;
-  }
-  for (int i = tid; i < 4 * 256; i += kRowThreads) (&t.bins[0][0])[i] = 0;
-  if (tid == 0) t.buckets = t.candidates = t.chosen = 0;
-  __syncthreads();
+  const auto& key = keys.k;
 
   uint32_t lo = 0, second = 0, hi = 0;
 #pragma unroll
-  for (int w = 0; w < kRowWaves; w++) {
+  for (int w = 0; w < WAVES; w++) {
     const uint32_t x = t.low[w];
     second = max(second, min(lo, x));
     lo = max(lo, x);
@@ -452,7 +464,7 @@ __device__ __forceinline__ void select_top(const char* row, int V, int nseg, int
   for (int step = 0; step < 4 && lo <= hi; step++) {
     const int bits = 32 - __builtin_clz((hi - lo) | 1u), shift = bits > 8 ? bits - 8 : 0;
 #pragma unroll
-    for (int i = 0; i < kKeysPerThread; i++)
+    for (int i = 0; i < per_thread; i++)
       if (key[i] >= lo && key[i] <= hi) atomicAdd(&t.bins[step][(key[i] - lo) >> shift], 1u);
     __syncthreads();
     // lane 0 has the four highest bins
@@ -485,10 +497,10 @@ __device__ __forceinline__ void select_top(const char* row, int V, int nseg, int
   int last = nseg;  // the segment up to which keys equal to tau count
   if (above + equal > top + 64) {  // then the interval is one key wide
 #pragma unroll
-    for (int i = 0; i < kKeysPerThread; i++)
-      if (i * kRowWaves + wave < nseg) {
+    for (int i = 0; i < per_thread; i++)
+      if (i * WAVES + wave < nseg) {
         const int same = __popcll(__ballot(key[i] == tau));
-        if (lane == 0) t.ties[i * kRowWaves + wave] = same;
+        if (lane == 0) t.ties[i * WAVES + wave] = same;
       }
     __syncthreads();
     last = 0;
@@ -499,18 +511,18 @@ __device__ __forceinline__ void select_top(const char* row, int V, int nseg, int
   }
   uint32_t mine = 0;
 #pragma unroll
-  for (int i = 0; i < kKeysPerThread; i++)
-    if (key[i] > tau || (key[i] == tau && i * kRowWaves + wave <= last)) mine |= 1u << i;
+  for (int i = 0; i < per_thread; i++)
+    if (key[i] > tau || (key[i] == tau && i * WAVES + wave <= last)) mine |= 1u << i;
   uint32_t at = append(&t.buckets, __popc(mine), lane);
   for (uint32_t m = mine; m; m &= m - 1)
-    t.bucket[at++] = (uint16_t)((__builtin_ctz(m) * kRowWaves + wave) * 64 + lane);
+    t.bucket[at++] = (uint16_t)((__builtin_ctz(m) * WAVES + wave) * 64 + lane);
   __syncthreads();
-  aside();
+  if (wave == 0) aside();
 
   constexpr int np = Type<DT>::kPackets, in = Type<DT>::kInPacket;
   const int work = (int)t.buckets * np;
-  for (int first = 0; first < work; first += kRowThreads) {
-    const int w = first + tid;
+  for (int first = wave == 0 ? work : 0; first < work; first += threads - 64) {
+    const int w = first + tid - 64;
     int j = 0;
     uint32_t k[in], have = 0;
     if (w < work) {
@@ -533,24 +545,24 @@ __device__ __forceinline__ void select_top(const char* row, int V, int nseg, int
 
   const uint64_t* list = memory;
   int n = t.candidates;
-  if (n > kRowThreads) {  // many equal or neighbouring ones: the `top` best by their 50 bits first
+  if (n > threads) {  // many equal or neighbouring ones: the `top` best by their 50 bits first
     uint64_t floor = 0;
     for (int bit = 49; bit >= 0; bit--) {
       const uint64_t trial = floor | (uint64_t)1 << bit;
       int in_wave = 0;
-      for (int i = tid - lane; i < n; i += kRowThreads) in_wave += __popcll(__ballot(i + lane < n && memory[i + lane] >= trial));
-      const int got = group_count(t, bit, in_wave, wave, lane);
+      for (int i = tid - lane; i < n; i += threads) in_wave += __popcll(__ballot(i + lane < n && memory[i + lane] >= trial));
+      const int got = group_count<WAVES>(t, bit, in_wave, wave, lane);
       if (got >= top) floor = trial;
       if (got == top) break;
     }
-    for (int i = tid; i < n; i += kRowThreads)
+    for (int i = tid; i < n; i += threads)
       if (memory[i] >= floor) t.best[atomicAdd(&t.chosen, 1u)] = memory[i];
     __syncthreads();
     list = t.best;
     n = top;
   }
   // eight threads count for one candidate
-  for (int first = 0; first < n; first += kRowThreads / 8) {
+  for (int first = 0; first < n; first += threads / 8) {
     const int i = first + tid / 8;
     const uint64_t one = list[min(i, n - 1)];
     int rank = 0;
@@ -570,8 +582,8 @@ __device__ __forceinline__ void select_top(const char* row, int V, int nseg, int
 // with KEYS their buckets' largest logits.  The next segment's loads are in
 // flight while one is reduced.
 template <int DT, bool ENT, bool KEYS, bool ONCE>
-__device__ __forceinline__ void read_segs(const char* row, int V, int seg0, int seg1, int wave, int waves, int lane,
-                                          float c, Part* parts, uint32_t* keys, const uint32_t* mask) {
+__device__ __forceinline__ void read_segs_as(const char* row, int V, int seg0, int seg1, int wave, int waves, int lane,
+                                             float c, Part* parts, uint32_t* keys, const uint32_t* mask) {
   int seg = seg0 + wave;
   if (seg >= seg1) return;
   Seg<DT> z, next;
@@ -589,6 +601,14 @@ __device__ __forceinline__ void read_segs(const char* row, int V, int seg0, int 
     z = next;
   }
 }
+template <int DT, bool ENT, bool KEYS>
+__device__ __forceinline__ void read_segs(const char* row, int V, int seg0, int seg1, int wave, int waves, int lane,
+                                          float c, bool once, Part* parts, uint32_t* keys, const uint32_t* mask) {
+  if (once)
+    read_segs_as<DT, ENT, KEYS, true>(row, V, seg0, seg1, wave, waves, lane, c, parts, keys, mask);
+  else
+    read_segs_as<DT, ENT, KEYS, false>(row, V, seg0, seg1, wave, waves, lane, c, parts, keys, mask);
+}
 
 // Whole rows by one workgroup each, or for few rows one part of a row each
 // (PARTS) and a second launch that joins them (JOIN).
@@ -603,6 +623,7 @@ __device__ __forceinline__ long load_index(const void* p, int wide, size_t i) {
 struct ScoreK {
   const char* z;
   size_t row_bytes, row0;  // the launch's first row
+  size_t once;             // rows below it are read past the caches
   int V, nseg, groups;
   const void* tokens;
   int wide, top;
@@ -615,26 +636,25 @@ struct ScoreK {
   uint32_t* keys;  // [rows][nseg * 64]
 };
 
-template <int DT, bool TOP, int PHASE, bool ONCE>
-__global__ __launch_bounds__(kRowThreads) void k_scores(ScoreK a) {
+template <int DT, bool TOP, int PHASE, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_scores(ScoreK a) {
   extern __shared__ uint64_t memory[];
   __shared__ Part lds_parts[PHASE == PARTS ? 1 : kScoreMaxSegs];
   __shared__ TopLds tl;
   __shared__ float row_m;
   __shared__ double row_log;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int waves = blockDim.x >> 6;
+  constexpr int waves = THREADS / 64;
   const float no = -__builtin_inff();
 
   if constexpr (PHASE == PARTS) {
     const size_t row = blockIdx.x / a.groups;
     const int g = (int)(blockIdx.x % a.groups), per = (a.nseg + a.groups - 1) / a.groups;
-    read_segs<DT, true, TOP, ONCE>(a.z + row * a.row_bytes, a.V, g * per, min(a.nseg, (g + 1) * per), wave, waves, lane, a.c,
-                             a.parts + row * a.nseg, TOP ? a.keys + row * a.nseg * 64 : nullptr, nullptr);
+    read_segs<DT, true, TOP>(a.z + row * a.row_bytes, a.V, g * per, min(a.nseg, (g + 1) * per), wave, waves, lane, a.c,
+                             false, a.parts + row * a.nseg, TOP ? a.keys + row * a.nseg * 64 : nullptr, nullptr);
     return;
   }
 
-  uint32_t* keys = reinterpret_cast<uint32_t*>(memory);
   const size_t row = a.row0 + blockIdx.x;
   const char* z = a.z + row * a.row_bytes;
   long y = -1;
@@ -643,16 +663,17 @@ __global__ __launch_bounds__(kRowThreads) void k_scores(ScoreK a) {
     y = load_index(a.tokens, a.wide, row);
     if (y >= 0 && y < a.V) zy = load_one<DT>(z, (int)y);
   }
+  Keys<TOP ? waves : kScoreMaxSegs> key;
   if constexpr (PHASE == WHOLE) {
-    read_segs<DT, true, TOP, ONCE>(z, a.V, 0, a.nseg, wave, waves, lane, a.c, lds_parts, keys, nullptr);
+    uint32_t* keys = reinterpret_cast<uint32_t*>(memory);
+    read_segs<DT, true, TOP>(z, a.V, 0, a.nseg, wave, waves, lane, a.c, row < a.once, lds_parts, keys, nullptr);
+    if constexpr (TOP) take_keys(key, keys, a.nseg, tl);  // each thread its own
   } else {
-    for (int i = threadIdx.x; i < a.nseg; i += kRowThreads) lds_parts[i] = a.parts[row * a.nseg + i];
-    if (TOP)
-      for (int i = threadIdx.x; i < a.nseg * 64; i += kRowThreads) keys[i] = a.keys[row * a.nseg * 64 + i];
+    for (int i = threadIdx.x; i < a.nseg; i += THREADS) lds_parts[i] = a.parts[row * a.nseg + i];
+    if constexpr (TOP) take_keys(key, a.keys + row * a.nseg * 64, a.nseg, tl);
   }
   __syncthreads();
   auto join = [&]() __attribute__((always_inline)) {
-    if (wave != 0) return;
     const RowStats st = join_row<DT, true>(z, a.V, a.nseg, lds_parts, nullptr, a.c, lane);
     const double l = st.bad ? (double)__builtin_nanf("") : log1p(st.r);
     const float m = st.bad ? __builtin_nanf("") : st.m;
@@ -674,11 +695,11 @@ __global__ __launch_bounds__(kRowThreads) void k_scores(ScoreK a) {
     }
   };
   if constexpr (!TOP) {
-    join();
+    if (wave == 0) join();
   } else {
     int32_t* ids = a.top_ids + row * a.top;
     float* lps = a.top_log_probs + row * a.top;
-    select_top<DT>(z, a.V, a.nseg, a.top, memory, tl, join, [&](int at, int id, float v) __attribute__((always_inline)) {
+    select_top<DT>(z, a.V, a.nseg, a.top, key, memory, tl, join, [&](int at, int id, float v) __attribute__((always_inline)) {
       const float m = row_m;
       const bool bad = !(m == m);
       ids[at] = bad ? -1 : id;
@@ -737,7 +758,7 @@ template <int DT, bool ENT>
 __global__ __launch_bounds__(kGradWaves * 64) void k_scores_grad(ScoreGradK a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const float no = -__builtin_inff();
-  const size_t row = a.row0 + blockIdx.x / a.chunks;
+  const size_t row = a.row0 + (gridDim.x - 1 - blockIdx.x) / a.chunks;  // the forward's last rows first
   const int seg0 = (int)(blockIdx.x % a.chunks) * (kGradWaves * kGradSegs) + wave;
   const char* z = a.z + row * a.row_bytes;
   char* out = a.grad + row * a.grad_bytes;
@@ -796,8 +817,8 @@ static_assert(kScoreSeg == 1 << 11, "the token's segment");
 struct DistillK {
   const char* z;
   char* grad;
-  size_t row_bytes, grad_bytes, row0;
-  int V, nseg, groups;
+  size_t row_bytes, grad_bytes, row0, once;
+  int V, nseg, groups, chunk;  // chunk: segments of a workgroup of the backward
   const void* ids;
   int wide, k;
   const float* teacher;
@@ -810,7 +831,7 @@ struct DistillK {
 };
 
 // The row's slots and their logits.
-struct Slots {
+struct alignas(16) Slots {
   int32_t id[kDistillMaxK];  // -1: empty
   float v[kDistillMaxK];
   float z[kDistillMaxK];
@@ -999,31 +1020,41 @@ template <int DT>
 __device__ __forceinline__ void grad_slot(const DistillK& a, char* out, const Slots& s, const RowGrad& g, float scale,
                                           int k) {
   const int id = s.id[k];
-  double p = 0.0;
-  for (int j = 0; j < a.k; j++)
-    if (s.id[j] == id) {
-      if (j < k) return;  // an earlier slot of the same id writes it
-      p += exp(((double)s.v[j] - g.log_hi) - g.log_lo);
+  const int4* ids = reinterpret_cast<const int4*>(s.id);
+  int before = 0, behind = 0;  // other slots of this id
+  for (int j = 0; 4 * j < a.k; j++) {
+    const int4 x = ids[j];
+    const int n = (x.x == id) + (x.y == id) + (x.z == id) + (x.w == id);
+    before += 4 * j < (k & ~3) ? n : 0;
+    behind += 4 * j > k ? n : 0;
+    if (j == k / 4) {
+      before += (x.x == id && (k & 3) > 0) + (x.y == id && (k & 3) > 1) + (x.z == id && (k & 3) > 2);
+      behind += (x.y == id && (k & 3) < 1) + (x.z == id && (k & 3) < 2) + (x.w == id && (k & 3) < 3);
     }
+  }
+  if (before) return;  // an earlier slot of the same id writes it
+  double p = exp(((double)s.v[k] - g.log_hi) - g.log_lo);
+  for (int j = k + 1; behind && j < a.k; j++)
+    if (s.id[j] == id) p += exp(((double)s.v[j] - g.log_hi) - g.log_lo);
   const float e = __builtin_amdgcn_exp2f((s.z[k] - g.m) * a.c);
   store_one<DT>(out, id, (float)((double)scale * ((double)e * g.share - p)));
 }
 
 // Losses, by whole rows or from parts.
-template <int DT, bool REST, int PHASE, bool ONCE>
-__global__ __launch_bounds__(kRowThreads) void k_distill(DistillK a) {
+template <int DT, bool REST, int PHASE, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_distill(DistillK a) {
   extern __shared__ uint32_t mask[];  // REST: [nseg * 64]
   __shared__ Part lds_parts[PHASE == PARTS ? 1 : kScoreMaxSegs];
   __shared__ Slots s;
   __shared__ SlotSums sums[kDistillMaxK / 64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int waves = blockDim.x >> 6;
+  constexpr int waves = THREADS / 64;
   const size_t row = PHASE == PARTS ? blockIdx.x / a.groups : a.row0 + blockIdx.x;
   const char* z = a.z + row * a.row_bytes;
   const float w = a.weights ? a.weights[row] : 1.0f;
 
   if (REST)
-    for (int i = threadIdx.x; i < a.nseg * 64; i += blockDim.x) mask[i] = 0;
+    for (int i = threadIdx.x; i < a.nseg * 64; i += THREADS) mask[i] = 0;
   load_slots<DT, REST>(s, a, row, z);
   __syncthreads();
   // a row that does not count, or has no slots in use, is not read
@@ -1035,16 +1066,16 @@ __global__ __launch_bounds__(kRowThreads) void k_distill(DistillK a) {
     }
     if constexpr (PHASE == PARTS) {
       const int g = (int)(blockIdx.x % a.groups), per = (a.nseg + a.groups - 1) / a.groups;
-      read_segs<DT, false, false, ONCE>(z, a.V, g * per, min(a.nseg, (g + 1) * per), wave, waves, lane, a.c,
-                                        a.parts + row * a.nseg, nullptr, REST ? mask : nullptr);
+      read_segs<DT, false, false>(z, a.V, g * per, min(a.nseg, (g + 1) * per), wave, waves, lane, a.c, false,
+                                  a.parts + row * a.nseg, nullptr, REST ? mask : nullptr);
       return;
     }
     sum_slots<REST>(s, sums, waves, a.inv_t);
     if constexpr (PHASE == WHOLE) {
-      read_segs<DT, false, false, ONCE>(z, a.V, 0, a.nseg, wave, waves, lane, a.c, lds_parts, nullptr,
-                                        REST ? mask : nullptr);
+      read_segs<DT, false, false>(z, a.V, 0, a.nseg, wave, waves, lane, a.c, row < a.once, lds_parts, nullptr,
+                                  REST ? mask : nullptr);
     } else {
-      for (int i = threadIdx.x; i < a.nseg; i += kRowThreads) lds_parts[i] = a.parts[row * a.nseg + i];
+      for (int i = threadIdx.x; i < a.nseg; i += THREADS) lds_parts[i] = a.parts[row * a.nseg + i];
     }
   }
   if constexpr (PHASE == PARTS) return;
@@ -1170,14 +1201,12 @@ __global__ __launch_bounds__(THREADS) void k_distill_step(DistillK a) {
 
 // The gradient alone, from the stats of the forward: workgroups of one chunk of
 // a row each.
-constexpr int kDistillChunk = 16;  // segments
-
 template <int DT>
 __global__ __launch_bounds__(kGradWaves * 64) void k_distill_grad(DistillK a) {
   __shared__ Slots s;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const size_t row = a.row0 + blockIdx.x / a.groups;
-  const int seg0 = (int)(blockIdx.x % a.groups) * kDistillChunk, seg1 = min(a.nseg, seg0 + kDistillChunk);
+  const size_t row = a.row0 + (gridDim.x - 1 - blockIdx.x) / a.groups;  // the forward's last rows first
+  const int seg0 = (int)(blockIdx.x % a.groups) * a.chunk, seg1 = min(a.nseg, seg0 + a.chunk);
   const char* z = a.z + row * a.row_bytes;
   char* out = a.grad + row * a.grad_bytes;
   const float weight = a.weights ? a.weights[row] : 1.0f;
@@ -1199,7 +1228,7 @@ __global__ __launch_bounds__(kGradWaves * 64) void k_distill_grad(DistillK a) {
   const int k = threadIdx.x, id = s.id[k];
   if (!zero && id >= seg0 * kScoreSeg && id < seg1 * kScoreSeg) grad_slot<DT>(a, out, s, g, scale, k);
 }
-static_assert(kGradWaves * 64 == kDistillMaxK && kRowThreads >= kDistillMaxK && kPartThreads >= kDistillMaxK,
+static_assert(kGradWaves * 64 == kDistillMaxK && kPartThreads >= kDistillMaxK,
               "a thread a slot");
 
 // ---- launches ---------------------------------------------------------------------------
@@ -1223,7 +1252,7 @@ int part_groups(size_t rows, int nseg) {
 }
 
 // A launch of `per_row` workgroups a row; of many rows several, of as many as
-// keep the launch's threads below 2^32 (a row has 16 workgroups of 256 at most).
+// keep the launch's threads below 2^32 (a row has 32 workgroups of 256 at most).
 constexpr size_t kRowsPerLaunch = 1u << 18;
 template <typename K>
 void launch_rows(void (*kernel)(K), size_t rows, int per_row, int threads, size_t lds, hipStream_t s, K k) {
@@ -1235,10 +1264,19 @@ void launch_rows(void (*kernel)(K), size_t rows, int per_row, int threads, size_
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Reads that bypass the caches reach 7.0 TB/s instead of 6.2 on 1.24 GB of
-// logits, but leave nothing behind: a backward pass over 32 MB of them takes 18.6
-// us instead of 15.0.  So only where the logits are larger than the cache.
-bool read_once(size_t rows, size_t row_bytes) { return rows * row_bytes > (size_t)256 << 20; }
+// Rows to read past the caches: those reads reach 7.0 TB/s instead of 6.2 on 1.24
+// GB of logits, but leave nothing behind, and a backward pass over 32 MB of
+// logits then takes 18.6 us instead of 15.0.  So where the logits are larger than
+// the memory-side cache of 256 MB, and if a backward pass may follow (it starts
+// with the last rows) all but the last 192 MB.
+size_t rows_once(size_t rows, size_t row_bytes, bool again) {
+  if (rows * row_bytes <= (size_t)256 << 20) return 0;
+  return rows;
+}
+
+// Whole rows go to workgroups of sixteen waves where there are too few rows for
+// several workgroups a compute unit, which reads faster the more waves it has.
+bool wide_rows(size_t rows, int nseg) { return rows <= 256 && nseg > 8; }
 
 template <typename F>
 void by_bool(bool b, F&& f) {
@@ -1293,15 +1331,18 @@ void launch_token_scores(const ScoreArgs& a, hipStream_t s) {
       constexpr int DT = decltype(dt)::value;
       constexpr bool TOP = decltype(with_top)::value;
       if (whole_rows(a.rows, k.nseg)) {
-        launch_rows(read_once(a.rows, k.row_bytes) ? k_scores<DT, TOP, WHOLE, true> : k_scores<DT, TOP, WHOLE, false>,
-                    a.rows, 1, kRowThreads, lds, s, k);
+        k.once = rows_once(a.rows, k.row_bytes, a.stats != nullptr);
+        if (wide_rows(a.rows, k.nseg))
+          launch_rows(k_scores<DT, TOP, WHOLE, 1024>, a.rows, 1, 1024, lds, s, k);
+        else
+          launch_rows(k_scores<DT, TOP, WHOLE, 512>, a.rows, 1, 512, lds, s, k);
         return;
       }
       k.groups = part_groups(a.rows, k.nseg);
       k.parts = static_cast<Part*>(a.scratch);
       k.keys = reinterpret_cast<uint32_t*>(static_cast<char*>(a.scratch) + round256(a.rows * k.nseg * sizeof(Part)));
-      launch_rows(k_scores<DT, TOP, PARTS, false>, a.rows, k.groups, kPartThreads, 0, s, k);
-      launch_rows(k_scores<DT, TOP, JOIN, false>, a.rows, 1, kRowThreads, lds, s, k);
+      launch_rows(k_scores<DT, TOP, PARTS, kPartThreads>, a.rows, k.groups, kPartThreads, 0, s, k);
+      launch_rows(k_scores<DT, TOP, JOIN, kJoinThreads>, a.rows, 1, kJoinThreads, lds, s, k);
     });
   });
 }
@@ -1363,7 +1404,10 @@ size_t distill_scratch_bytes(size_t rows, size_t vocab, bool step) {
 void launch_distill_grad(const DistillArgs& a, hipStream_t s) {
   if (a.rows == 0) return;
   DistillK k = distill_kernel_args(a);
-  k.groups = (k.nseg + kDistillChunk - 1) / kDistillChunk;
+  // each workgroup loads the row's slots: no more of them than fill the chip
+  k.chunk = kGradWaves;
+  while (k.chunk < 4 * kGradWaves && a.rows * k.nseg / k.chunk > 4096) k.chunk += kGradWaves;
+  k.groups = (k.nseg + k.chunk - 1) / k.chunk;
   by_type(a.dtype, [&](auto dt) {
     launch_rows(k_distill_grad<decltype(dt)::value>, a.rows, k.groups, kGradWaves * 64, 0, s, k);
   });
@@ -1374,19 +1418,25 @@ template <int DT, bool REST, int NS, bool LONGER, int THREADS>
 void launch_step_as(const DistillK& k, size_t rows, hipStream_t s) {
   launch_rows(k_distill_step<DT, REST, NS, LONGER, THREADS>, rows, 1, THREADS, REST ? (size_t)k.nseg * 256 : 0, s, k);
 }
-// A step of whole rows.  Eight waves and two segments a wave in registers leave
-// room for two or three workgroups a compute unit, one reading while another
-// writes; us of 4096 rows with sixteen waves and every segment held / eight and
-// two / eight and three: vocabularies of 32000 bf16 189 / 135 / -, 49152 bf16 233
-// / 174 / 200, 151936 bf16 773 / 538 / 515, 32000 f32 286 / 202 / -, 49152 f32 337
-// / 314 / 329; 2048 rows of 151936 f32 - / 556 / -.
+// A step of whole rows.  Workgroups that hold only part of a long row leave room
+// for two or three of them a compute unit, one reading while another writes; us
+// by segments held a wave x waves:
+//   4096 rows of 32000 bf16   2 x 8 (all) 109, 4 x 4 (all) 111, 1 x 16 (all) 175
+//   4096 rows of 49152 bf16   2 x 8 158, 3 x 8 (all) 158, 1 x 8 168, 2 x 16 225
+//   4096 rows of 151936 bf16  4 x 8 515, 3 x 8 523, 2 x 8 543, 1 x 8 562, 5 x 16 (all) 601
+//   4096 rows of 32000 f32    2 x 8 (all) 188, 4 x 4 (all) 203, 1 x 16 (all) 234
+//   4096 rows of 49152 f32    2 x 8 308, 1 x 8 317, 3 x 8 323, 2 x 16 320
+//   2048 rows of 151936 f32   2 x 16 509, 3 x 8 520, 2 x 8 547, 1 x 8 546, 2 x 4 683
 template <int DT, bool REST>
 void launch_step(const DistillK& k, size_t rows, hipStream_t s) {
   if (k.nseg <= 4) return launch_step_as<DT, REST, 1, false, 256>(k, rows, s);
   if (k.nseg <= 8) return launch_step_as<DT, REST, 1, false, 512>(k, rows, s);
   if (k.nseg <= 16) return launch_step_as<DT, REST, 2, false, 512>(k, rows, s);
-  if (DT == DTL_F32 || k.nseg <= 32) return launch_step_as<DT, REST, 2, true, 512>(k, rows, s);
-  if constexpr (DT != DTL_F32) launch_step_as<DT, REST, 3, true, 512>(k, rows, s);
+  if (k.nseg <= 32) return launch_step_as<DT, REST, 2, true, 512>(k, rows, s);
+  if constexpr (DT == DTL_F32)
+    launch_step_as<DT, REST, 2, true, 1024>(k, rows, s);
+  else
+    launch_step_as<DT, REST, 4, true, 512>(k, rows, s);
 }
 }  // namespace
 
@@ -1394,6 +1444,7 @@ void launch_distill(const DistillArgs& a, hipStream_t s) {
   if (a.rows == 0) return;
   DistillK k = distill_kernel_args(a);
   const size_t lds = a.rest ? (size_t)k.nseg * 256 : 0;
+  k.once = a.grad ? 0 : rows_once(a.rows, k.row_bytes, a.stats != nullptr);
   by_type(a.dtype, [&](auto dt) {
     by_bool(a.rest, [&](auto with_rest) {
       constexpr int DT = decltype(dt)::value;
@@ -1401,17 +1452,18 @@ void launch_distill(const DistillArgs& a, hipStream_t s) {
       if (whole_rows(a.rows, k.nseg)) {
         if (a.grad)
           launch_step<DT, REST>(k, a.rows, s);
+        else if (wide_rows(a.rows, k.nseg))
+          launch_rows(k_distill<DT, REST, WHOLE, 1024>, a.rows, 1, 1024, lds, s, k);
         else
-          launch_rows(read_once(a.rows, k.row_bytes) ? k_distill<DT, REST, WHOLE, true> : k_distill<DT, REST, WHOLE, false>,
-                      a.rows, 1, kRowThreads, lds, s, k);
+          launch_rows(k_distill<DT, REST, WHOLE, 512>, a.rows, 1, 512, lds, s, k);
         return;
       }
       k.groups = part_groups(a.rows, k.nseg);
       k.parts = static_cast<Part*>(a.scratch);
       if (a.grad)
         k.stats = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + round256(a.rows * k.nseg * sizeof(Part)));
-      launch_rows(k_distill<DT, REST, PARTS, false>, a.rows, k.groups, kPartThreads, lds, s, k);
-      launch_rows(k_distill<DT, REST, JOIN, false>, a.rows, 1, kRowThreads, lds, s, k);
+      launch_rows(k_distill<DT, REST, PARTS, kPartThreads>, a.rows, k.groups, kPartThreads, lds, s, k);
+      launch_rows(k_distill<DT, REST, JOIN, kJoinThreads>, a.rows, 1, kJoinThreads, lds, s, k);
     });
   });
   if (a.grad && !whole_rows(a.rows, k.nseg)) {
