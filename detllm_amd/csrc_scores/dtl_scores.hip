@@ -545,7 +545,7 @@ __device__ __forceinline__ void select_top(const char* row, int V, int nseg, int
 
   const uint64_t* list = memory;
   int n = t.candidates;
-  if (n > threads) {  // many equal or neighbouring ones: the `top` best by their 50 bits first
+  if (n > 512) {  // many equal or neighbouring ones: the `top` best by their 50 bits first
     uint64_t floor = 0;
     for (int bit = 49; bit >= 0; bit--) {
       const uint64_t trial = floor | (uint64_t)1 << bit;
@@ -716,6 +716,7 @@ struct ScoreGradK {
   char* grad;
   size_t row_bytes, grad_bytes, row0;
   int V, nseg, chunks;
+  bool past;  // write past the caches
   const void* tokens;
   int wide;
   float c;
@@ -723,11 +724,13 @@ struct ScoreGradK {
   const float *stats, *entropy, *g, *h;
 };
 
-// Segments a wave takes one after another; a workgroup has kGradWaves waves.
-constexpr int kGradWaves = 4, kGradSegs = 2;
+// Waves of a gradient's workgroup, each with one segment: us of 4096 rows of 151936
+// bf16 with one / two / four segments a wave 450 / 471 / 478.
+constexpr int kGradWaves = 4;
 
-template <int DT, bool ONCE, typename F>
-__device__ __forceinline__ void write_seg(const Seg<DT>& z, char* out, int seg, int lane, int V, F&& f) {
+// PAST: past the caches' usual policy, see write_past.
+template <int DT, bool PAST, typename F>
+__device__ __forceinline__ void write_seg_as(const Seg<DT>& z, char* out, int seg, int lane, int V, F&& f) {
   constexpr int in = Type<DT>::kInPacket;
   const bool whole = seg * kScoreSeg + kScoreSeg <= V;
 #pragma unroll
@@ -742,7 +745,7 @@ __device__ __forceinline__ void write_seg(const Seg<DT>& z, char* out, int seg, 
       p[d] = DT == DTL_F32 ? bits_of<DT>(v[d]) : bits_of<DT>(v[2 * d % in]) | bits_of<DT>(v[(2 * d + 1) % in]) << 16;
     if (whole || j + in <= V) {
       auto* to = reinterpret_cast<typename Type<DT>::mem*>(out + (size_t)j * Type<DT>::kBytes);
-      if (ONCE)
+      if (PAST)
         __builtin_nontemporal_store(p, to);
       else
         *to = p;
@@ -754,12 +757,21 @@ __device__ __forceinline__ void write_seg(const Seg<DT>& z, char* out, int seg, 
   }
 }
 
+template <int DT, typename F>
+__device__ __forceinline__ void write_seg(const Seg<DT>& z, char* out, int seg, int lane, int V, bool past, F&& f) {
+  if (past)
+    write_seg_as<DT, true>(z, out, seg, lane, V, f);
+  else
+    write_seg_as<DT, false>(z, out, seg, lane, V, f);
+}
+
 template <int DT, bool ENT>
 __global__ __launch_bounds__(kGradWaves * 64) void k_scores_grad(ScoreGradK a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const float no = -__builtin_inff();
   const size_t row = a.row0 + (gridDim.x - 1 - blockIdx.x) / a.chunks;  // the forward's last rows first
-  const int seg0 = (int)(blockIdx.x % a.chunks) * (kGradWaves * kGradSegs) + wave;
+  const int seg = (int)(blockIdx.x % a.chunks) * kGradWaves + wave;
+  if (seg >= a.nseg) return;
   const char* z = a.z + row * a.row_bytes;
   char* out = a.grad + row * a.grad_bytes;
   const long y = a.tokens ? load_index(a.tokens, a.wide, row) : -1;
@@ -768,7 +780,7 @@ __global__ __launch_bounds__(kGradWaves * 64) void k_scores_grad(ScoreGradK a) {
   const double r = a.stats[2 * row + 1], p0 = 1.0 / (1.0 + r);
   // padding, and rows whose mask leaves nothing: zeros, whatever they hold
   const bool zero = (g == 0.0 && h == 0.0) || m == no;
-  const bool bad = y >= a.V, here = y >= 0 && !bad && !zero && ((int)(y >> 11) - seg0) % kGradWaves == 0;
+  const bool bad = y >= a.V, here = y >= 0 && !bad && !zero && (int)(y / kScoreSeg) == seg;
   double l = 0.0, hh = 0.0;
   if (ENT || here) {
     l = log1p(r);
@@ -781,27 +793,21 @@ __global__ __launch_bounds__(kGradWaves * 64) void k_scores_grad(ScoreGradK a) {
     // log p of a masked token is -inf and its p log p is 0
     at_y = (float)(a.inv_t * (-g * expm1(lp) - (ENT && h != 0.0 && lp > -1e30 ? h * exp(lp) * (t + hh) : 0.0)));
   }
-#pragma unroll
-  for (int i = 0; i < kGradSegs; i++) {
-    const int seg = seg0 + i * kGradWaves;
-    if (seg >= a.nseg) break;
-    Seg<DT> s;
-    if (zero) {
-      write_seg<DT, false>(s, out, seg, lane, a.V, [](float, int) { return 0.0f; });
-      continue;
-    }
-    load_seg<DT, false>(s, z, seg, lane, a.V);
-    auto value_of = [&](float v) {
-      const float t = (v - m) * a.c, e = __builtin_amdgcn_exp2f(t);
-      return e * (ENT ? __builtin_fmaf(B, fmaxf(t, kLowest), A) : A);
-    };
-    if (y >> 11 == seg)
-      write_seg<DT, false>(s, out, seg, lane, a.V, [&](float v, int j) { return j == (int)y ? at_y : value_of(v); });
-    else
-      write_seg<DT, false>(s, out, seg, lane, a.V, [&](float v, int) { return value_of(v); });
+  Seg<DT> s;
+  if (zero) {
+    write_seg<DT>(s, out, seg, lane, a.V, a.past, [](float, int) { return 0.0f; });
+    return;
   }
+  load_seg<DT, false>(s, z, seg, lane, a.V);
+  auto value_of = [&](float v) {
+    const float t = (v - m) * a.c, e = __builtin_amdgcn_exp2f(t);
+    return e * (ENT ? __builtin_fmaf(B, fmaxf(t, kLowest), A) : A);
+  };
+  if (here)
+    write_seg<DT>(s, out, seg, lane, a.V, a.past, [&](float v, int j) { return j == (int)y ? at_y : value_of(v); });
+  else
+    write_seg<DT>(s, out, seg, lane, a.V, a.past, [&](float v, int) { return value_of(v); });
 }
-static_assert(kScoreSeg == 1 << 11, "the token's segment");
 
 // ---- distillation ------------------------------------------------------------------------
 
@@ -818,7 +824,8 @@ struct DistillK {
   const char* z;
   char* grad;
   size_t row_bytes, grad_bytes, row0, once;
-  int V, nseg, groups, chunk;  // chunk: segments of a workgroup of the backward
+  int V, nseg, groups;
+  bool past;  // write past the caches
   const void* ids;
   int wide, k;
   const float* teacher;
@@ -998,17 +1005,17 @@ __device__ __forceinline__ RowGrad join_distill(const DistillK& a, const RowStat
 }
 
 // Gradient of a segment for every j as if outside the list.
-template <int DT, bool ONCE>
+template <int DT>
 __device__ __forceinline__ void grad_seg(const DistillK& a, const Seg<DT>& s, char* out, const RowGrad& g, float scale,
                                          int seg, int lane) {
   const float A = scale * (g.share - g.outside);
-  write_seg<DT, ONCE>(s, out, seg, lane, a.V,
-                      [&](float v, int) { return __builtin_amdgcn_exp2f((v - g.m) * a.c) * A; });
+  write_seg<DT>(s, out, seg, lane, a.V, a.past,
+                [&](float v, int) { return __builtin_amdgcn_exp2f((v - g.m) * a.c) * A; });
 }
 template <int DT>
 __device__ __forceinline__ void zero_seg(char* out, int seg, int lane, int V) {
   Seg<DT> s;
-  write_seg<DT, false>(s, out, seg, lane, V, [](float, int) { return 0.0f; });
+  write_seg_as<DT, false>(s, out, seg, lane, V, [](float, int) { return 0.0f; });
 }
 __device__ __forceinline__ bool grad_is_zero(const RowGrad& g, float scale) {
   return scale == 0.0f || g.m == -__builtin_inff();
@@ -1180,7 +1187,7 @@ __global__ __launch_bounds__(THREADS) void k_distill_step(DistillK a) {
       if (zero)
         zero_seg<DT>(out, seg, lane, a.V);
       else
-        grad_seg<DT, true>(a, held[i], out, g, scale, seg, lane);
+        grad_seg<DT>(a, held[i], out, g, scale, seg, lane);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -1191,7 +1198,7 @@ __global__ __launch_bounds__(THREADS) void k_distill_step(DistillK a) {
       } else {
         Seg<DT> x;
         load_seg<DT, false>(x, z, seg, lane, a.V);
-        grad_seg<DT, true>(a, x, out, g, scale, seg, lane);
+        grad_seg<DT>(a, x, out, g, scale, seg, lane);
       }
     }
   __syncthreads();
@@ -1199,14 +1206,14 @@ __global__ __launch_bounds__(THREADS) void k_distill_step(DistillK a) {
   if (!zero && k < a.k && s.id[k] >= 0) grad_slot<DT>(a, out, s, g, scale, k);
 }
 
-// The gradient alone, from the stats of the forward: workgroups of one chunk of
-// a row each.
+// The gradient alone, from the stats of the forward: workgroups of four segments
+// of a row each (2048 rows of 151936 f32: 447 us, 467 with sixteen).
 template <int DT>
 __global__ __launch_bounds__(kGradWaves * 64) void k_distill_grad(DistillK a) {
   __shared__ Slots s;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const size_t row = a.row0 + (gridDim.x - 1 - blockIdx.x) / a.groups;  // the forward's last rows first
-  const int seg0 = (int)(blockIdx.x % a.groups) * a.chunk, seg1 = min(a.nseg, seg0 + a.chunk);
+  const int seg0 = (int)(blockIdx.x % a.groups) * kGradWaves, seg = seg0 + wave;
   const char* z = a.z + row * a.row_bytes;
   char* out = a.grad + row * a.grad_bytes;
   const float weight = a.weights ? a.weights[row] : 1.0f;
@@ -1215,18 +1222,18 @@ __global__ __launch_bounds__(kGradWaves * 64) void k_distill_grad(DistillK a) {
   __syncthreads();
   const float scale = slots_state(s) ? weight * a.T : 0.0f;
   const bool zero = grad_is_zero(g, scale);
-  for (int seg = seg0 + wave; seg < seg1; seg += kGradWaves) {
+  if (seg < a.nseg) {
     if (zero) {
       zero_seg<DT>(out, seg, lane, a.V);
     } else {
       Seg<DT> x;
       load_seg<DT, false>(x, z, seg, lane, a.V);
-      grad_seg<DT, false>(a, x, out, g, scale, seg, lane);
+      grad_seg<DT>(a, x, out, g, scale, seg, lane);
     }
   }
   __syncthreads();
   const int k = threadIdx.x, id = s.id[k];
-  if (!zero && id >= seg0 * kScoreSeg && id < seg1 * kScoreSeg) grad_slot<DT>(a, out, s, g, scale, k);
+  if (!zero && id >= seg0 * kScoreSeg && id < (seg0 + kGradWaves) * kScoreSeg) grad_slot<DT>(a, out, s, g, scale, k);
 }
 static_assert(kGradWaves * 64 == kDistillMaxK && kPartThreads >= kDistillMaxK,
               "a thread a slot");
@@ -1274,8 +1281,15 @@ size_t rows_once(size_t rows, size_t row_bytes, bool again) {
   return rows;
 }
 
-// Whole rows go to workgroups of sixteen waves where there are too few rows for
-// several workgroups a compute unit, which reads faster the more waves it has.
+// Gradients larger than the memory-side cache are written past it: 423 instead of
+// 450 us for 4096 rows of 151936 bf16, 408 instead of 426 for 2048 of f32.
+bool write_past(size_t rows, size_t row_bytes) { return rows * row_bytes > (size_t)256 << 20; }
+
+// Whole rows go to workgroups of one, four or eight waves by their length (us of
+// 16384 rows of 1000 bf16 with one / four / eight: scores 30 / - / 80, with 20
+// alternatives - / 149 / 225, losses - / 57 / 93), and of sixteen where there are
+// too few rows for several workgroups a compute unit, which reads faster the more
+// waves it has (64 rows of 32000 f32 6.6 instead of 7.1).
 bool wide_rows(size_t rows, int nseg) { return rows <= 256 && nseg > 8; }
 
 template <typename F>
@@ -1324,6 +1338,7 @@ void launch_token_scores(const ScoreArgs& a, hipStream_t s) {
   size_t lds = 0;
   if (a.top) {
     lds = candidate_bytes(a.top);
+    if (lds > (size_t)k.nseg * kScoreSeg * 8) lds = (size_t)k.nseg * kScoreSeg * 8;  // a short row has no more
     if (lds < (size_t)k.nseg * 256) lds = (size_t)k.nseg * 256;
   }
   by_type(a.dtype, [&](auto dt) {
@@ -1332,10 +1347,15 @@ void launch_token_scores(const ScoreArgs& a, hipStream_t s) {
       constexpr bool TOP = decltype(with_top)::value;
       if (whole_rows(a.rows, k.nseg)) {
         k.once = rows_once(a.rows, k.row_bytes, a.stats != nullptr);
-        if (wide_rows(a.rows, k.nseg))
+        if (!TOP && k.nseg == 1) {
+          if constexpr (!TOP) launch_rows(k_scores<DT, false, WHOLE, 64>, a.rows, 1, 64, lds, s, k);
+        } else if (k.nseg <= 4) {
+          launch_rows(k_scores<DT, TOP, WHOLE, 256>, a.rows, 1, 256, lds, s, k);
+        } else if (wide_rows(a.rows, k.nseg)) {
           launch_rows(k_scores<DT, TOP, WHOLE, 1024>, a.rows, 1, 1024, lds, s, k);
-        else
+        } else {
           launch_rows(k_scores<DT, TOP, WHOLE, 512>, a.rows, 1, 512, lds, s, k);
+        }
         return;
       }
       k.groups = part_groups(a.rows, k.nseg);
@@ -1356,7 +1376,8 @@ void launch_token_scores_grad(const ScoreGradArgs& a, hipStream_t s) {
   k.grad_bytes = a.grad_stride * type_bytes(a.dtype);
   k.V = a.vocab;
   k.nseg = segments(a.vocab);
-  k.chunks = (k.nseg + kGradWaves * kGradSegs - 1) / (kGradWaves * kGradSegs);
+  k.chunks = (k.nseg + kGradWaves - 1) / kGradWaves;
+  k.past = write_past(a.rows, k.grad_bytes);
   k.tokens = a.tokens;
   k.wide = a.wide;
   k.c = (float)(kLog2E / a.temperature);
@@ -1391,6 +1412,7 @@ DistillK distill_kernel_args(const DistillArgs& a) {
   k.inv_t = 1.0 / a.temperature;
   k.loss = a.loss;
   k.stats = a.stats;
+  k.past = write_past(a.rows, k.grad_bytes);
   return k;
 }
 }  // namespace
@@ -1404,10 +1426,7 @@ size_t distill_scratch_bytes(size_t rows, size_t vocab, bool step) {
 void launch_distill_grad(const DistillArgs& a, hipStream_t s) {
   if (a.rows == 0) return;
   DistillK k = distill_kernel_args(a);
-  // each workgroup loads the row's slots: no more of them than fill the chip
-  k.chunk = kGradWaves;
-  while (k.chunk < 4 * kGradWaves && a.rows * k.nseg / k.chunk > 4096) k.chunk += kGradWaves;
-  k.groups = (k.nseg + k.chunk - 1) / k.chunk;
+  k.groups = (k.nseg + kGradWaves - 1) / kGradWaves;
   by_type(a.dtype, [&](auto dt) {
     launch_rows(k_distill_grad<decltype(dt)::value>, a.rows, k.groups, kGradWaves * 64, 0, s, k);
   });
@@ -1452,6 +1471,8 @@ void launch_distill(const DistillArgs& a, hipStream_t s) {
       if (whole_rows(a.rows, k.nseg)) {
         if (a.grad)
           launch_step<DT, REST>(k, a.rows, s);
+        else if (k.nseg <= 4)
+          launch_rows(k_distill<DT, REST, WHOLE, 256>, a.rows, 1, 256, lds, s, k);
         else if (wide_rows(a.rows, k.nseg))
           launch_rows(k_distill<DT, REST, WHOLE, 1024>, a.rows, 1, 1024, lds, s, k);
         else
