@@ -1514,12 +1514,17 @@ int launch_status() {
 
 constexpr size_t kMostRows = 1u << 24;
 
+// One row has no stride; others do not overlap, and their bytes can be counted.
+bool stride_ok(const dtl_logits* z, size_t stride) {
+  return z->rows <= 1 || (stride >= z->vocab && stride <= ((size_t)1 << 48) / z->rows);
+}
+
 int check_logits(const dtl_logits* z) {
   if (!z) return DTL_ERR_INVALID_ARGUMENT;
   if (z->dtype != DTL_F32 && z->dtype != DTL_BF16 && z->dtype != DTL_F16) return DTL_ERR_INVALID_ARGUMENT;
   if (z->vocab == 0) return DTL_ERR_CDF_EMPTY;
   if (z->vocab > (size_t)kScoreMaxVocab) return DTL_ERR_CDF_TOO_MANY_SYMBOLS;
-  if (z->rows > kMostRows || (z->rows > 1 && z->stride < z->vocab) || z->stride > (size_t)1 << 40) return DTL_ERR_SHAPE;
+  if (z->rows > kMostRows || !stride_ok(z, z->stride)) return DTL_ERR_SHAPE;
   if (z->rows == 0) return DTL_OK;
   if (!z->data || reinterpret_cast<uintptr_t>(z->data) % type_bytes(z->dtype)) return DTL_ERR_INVALID_ARGUMENT;
   return DTL_OK;
@@ -1527,7 +1532,7 @@ int check_logits(const dtl_logits* z) {
 bool index_bytes_ok(int n) { return n == 4 || n == 8; }
 bool temperature_ok(float t) { return t >= kScoreMinTemperature && t <= kScoreMaxTemperature; }
 int check_grad(const dtl_logits* z, const void* grad, size_t stride) {
-  if (z->rows > 1 && (stride < z->vocab || stride > (size_t)1 << 40)) return DTL_ERR_SHAPE;
+  if (!stride_ok(z, stride)) return DTL_ERR_SHAPE;
   if (z->rows && (!grad || reinterpret_cast<uintptr_t>(grad) % type_bytes(z->dtype))) return DTL_ERR_INVALID_ARGUMENT;
   return DTL_OK;
 }

@@ -5,7 +5,9 @@ rows say of given tokens (log probability, entropy, top alternatives), and the
 loss that moves a student towards a teacher's top alternatives, both with
 gradients.  The calls enqueue the library's kernels (dtl_token_scores*,
 dtl_distill* of include/detllm.h, which define every result) on the current
-stream of the logits' device, do not wait, and can be captured into a graph.
+stream of the logits' device, do not wait, and can be captured into a graph (a
+captured backward needs a leaf of its own, `logits.detach().requires_grad_()`: one
+whose eager graph is still alive belongs to that graph's stream).
 
     teacher = scores.token_scores(teacher_logits, tokens, top=32, temperature=2.0)
     loss = scores.distill_loss(student_logits, teacher.top_ids, teacher.top_log_probs,
@@ -24,7 +26,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import check, lib
+from ._lib import DetllmError, check, lib
 
 
 def _one_hip_runtime() -> None:
@@ -133,6 +135,8 @@ def _scratch(n: int, device: torch.device) -> Optional[torch.Tensor]:
 
 def _scores(logits, tokens, top, temperature, stats):
     z = _logits_view(logits)
+    if not 0 <= top <= min(MAX_TOP, z.vocab):
+        raise DetllmError(1, "token_scores: top")
     lead, dev = logits.shape[:-1], logits.device
     log_probs = torch.empty(lead, dtype=torch.float32, device=dev) if tokens is not None else None
     entropy = torch.empty(lead, dtype=torch.float32, device=dev)
@@ -258,13 +262,14 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
     loops that know the rows' weights (1 / rows for a mean, 0 for padding; None:
     ones) before the loss.  One pass instead of a forward and a backward; pass the
     gradient on with `logits.backward(grad)`.  out: where the gradient goes, of the
-    logits' shape and type; the logits themselves if they are not needed again."""
+    logits' shape and type; the logits themselves if nothing needs them again."""
     z = _logits_view(logits)
     t, teacher_ids, teacher_log_probs = _teacher(logits, teacher_ids, teacher_log_probs, rest)
     dev = logits.device
     if weights is not None:
         weights = _beside(weights, logits, logits.shape[:-1], _FLOAT, "weights")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         stride = z.vocab
     else:
@@ -276,4 +281,6 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
     scratch = _scratch(n, dev)
     _call(dev, lib.dtl_distill_step, C.byref(z), C.byref(t), float(temperature), _ptr(weights), _ptr(loss),
           out.data_ptr(), stride, _ptr(scratch), n)
+    if given:  # autograd is told that it was written
+        torch.autograd.graph.increment_version(out)
     return loss, out

@@ -204,7 +204,7 @@ def test_refusals():
                 torch.empty(300, 4, device=DEV).t()):
         with pytest.raises(ValueError):
             scores.distill_loss_and_grad(z, ids, v, out=out)
-    for kw, status in ((dict(top=129), 1), (dict(top=301), 1), (dict(temperature=0.0), 42)):
+    for kw, status in ((dict(top=129), 1), (dict(top=301), 1), (dict(top=-1), 1), (dict(temperature=0.0), 42)):
         with pytest.raises(DetllmError) as e:
             scores.token_scores(z, tok, **kw)
         assert e.value.status == status
@@ -218,9 +218,57 @@ def test_refusals():
         x.zero_()
     with pytest.raises(RuntimeError):
         s.backward()
+    x = leaf * 1
+    s = (x * x).sum()
+    scores.distill_loss_and_grad(x, ids, v, out=x)  # over what s needs
+    with pytest.raises(RuntimeError):
+        s.backward()
     g, = torch.autograd.grad(scores.distill_loss(leaf, ids, v).sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+def test_logits_larger_than_the_cache():
+    """Beyond 256 MB, rows of odd length: read and written past the caches, the same bits."""
+    R, V, k = 900, 151937, 5
+    z = torch.empty(R, V, dtype=torch.bfloat16, device=DEV).normal_()
+    few = [slice(0, 3), slice(449, 451), slice(R - 2, R)]
+    tokens = torch.randint(0, V, (R,), device=DEV)
+    leaf = z.requires_grad_()
+    w = torch.rand(R, device=DEV)
+
+    def work(rows):
+        x = leaf[rows]
+        got = scores.token_scores(x, tokens[rows], top=k)
+        loss = scores.distill_loss(x, got.top_ids, got.top_log_probs - 0.2, rest=True)
+        g, = torch.autograd.grad([got.log_probs, got.entropy], [x], [w[rows], -w[rows]], retain_graph=True)
+        d, = torch.autograd.grad([loss], [x], [w[rows]])
+        step = scores.distill_loss_and_grad(x.detach(), got.top_ids, got.top_log_probs - 0.2, w[rows], rest=True)
+        return [t.detach() for t in (*got, loss, g, d, *step)]
+
+    whole = work(slice(None))
+    for rows in few:
+        for a, b in zip(whole, work(rows)):
+            assert torch.equal(a[rows], b)
+    i = 450
+    want, tol = rows64.scores_grad(rows_of(z[i:i + 1])[0], int(tokens[i]), 1.0, float(w[i]), -float(w[i]),
+                                   float(whole[1][i]), "bf16")
+    near(whole[5][i], want, tol, "gradient")
+
+
+def test_more_rows_than_a_launch():
+    R, V = (1 << 18) + 5, 70
+    z = logits(40, 64, V, dtype="f16").repeat(R // 64 + 1, 1)[:R].contiguous().requires_grad_()
+    tokens = (torch.arange(R, device=DEV) % 64) % V
+    got = scores.token_scores(z, tokens, top=2)
+    loss = scores.distill_loss(z, got.top_ids, got.top_log_probs)
+    ones = torch.ones(R, device=DEV)
+    grad, = torch.autograd.grad([got.log_probs, got.entropy, loss], [z], [ones, ones, ones])
+    step = scores.distill_loss_and_grad(z.detach(), got.top_ids, got.top_log_probs)
+    for t in (*got, loss, grad, *step):
+        t = t.detach().reshape(R, -1)
+        assert torch.equal(t[64:], t[:-64])
+    check_scores(z[:3], tokens[:3], type(got)(*(t[:3] for t in got)), 1.0, 2)
 
 
 def test_rows_past_32_bits():
