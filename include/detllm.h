@@ -276,7 +276,8 @@ int dtl_status_from_bits(int bits);
  * (log probability: -log2 of it is the ideal code length; entropy; the most
  * likely alternatives), and the loss that moves a smaller model towards such
  * alternatives, with gradients.  Their arithmetic is their own (32-bit sums in
- * a fixed order, hardware 2^x); no payload depends on them.  A row's results
+ * a fixed order, hardware 2^x, whose results below 2^-126 are 0); no payload
+ * depends on them.  A row's results
  * are the same bits whatever the other rows and however many there are.
  *
  * Pointers are device memory of the current device, the work is enqueued on
@@ -340,7 +341,7 @@ size_t dtl_distill_scratch(size_t rows, size_t vocab);
 /* loss[row] = T^2 (sum_k p_k (log p_k - log q[id_k]) + rest (log rest - log
  * q_rest)), q = softmax(logits / T) and q_rest = 1 - q over the listed ids; the
  * last term only with teacher->rest and where a logit outside the list is not
- * masked.  A row without slots in use: 0, and its logits are not read.  A
+ * masked.  A row without slots in use: 0, whatever its logits hold.  A
  * masked logit that the teacher gives mass to: +inf.  An id >= vocab, a v that
  * is NaN or +inf, a logit that is NaN or +inf: NaN.  stats ([rows][5] floats,
  * may be NULL) is what dtl_distill_backward needs. */
@@ -354,7 +355,8 @@ int dtl_distill_backward(const dtl_logits *logits, const dtl_teacher *teacher, f
                          void *stream);
 /* Both in one call for row weights known beforehand (NULL: ones): loss[row] is
  * weights[row] times dtl_distill's, grad the gradient of their sum.  Reads the
- * logits from memory once.  A row of weight 0 is not read: loss 0, gradient 0. */
+ * logits once (of rows past 32768 logits a part again, mostly from the caches).
+ * A row of weight 0 is not read: loss 0, gradient 0. */
 int dtl_distill_step(const dtl_logits *logits, const dtl_teacher *teacher, float temperature,
                      const float *weights, float *loss, void *grad, size_t grad_stride, void *scratch,
                      size_t scratch_bytes, void *stream);
