@@ -1241,12 +1241,13 @@ static_assert(kGradWaves * 64 == kDistillMaxK && kPartThreads >= kDistillMaxK,
 // ---- launches ---------------------------------------------------------------------------
 
 // Whether a row is one workgroup's.  Few long rows would leave compute units idle
-// and go to several workgroups each, with a second launch to join them.  us by
-// whole rows / in parts, scores of bf16: 1 row of 32000 6.2 / 6.6, of 151936 15.1 /
-// 7.0; 64 rows 15.8 / 10.2, 128 rows 18.0 / 15.8, 255 rows 20.0 / 23.2; of 262144
-// 128 rows 27.0 / 20.5, 255 rows 28.7 / 32.3; a step of 64 rows of 151936 29.7 /
-// 25.8, 128 rows 32.1 / 34.1.
-bool whole_rows(size_t rows, int nseg) { return nseg <= 24 || rows >= 160; }
+// and go to several workgroups each, with a second launch to join them.  us on the
+// device by whole rows / in parts, scores of bf16: 1 row of 32000 5.6 / 6.6, of
+// 60000 7.9 / 6.7 (and one launch less on the host), of 151936 13.3 / 6.7; of
+// 151936 64 rows 14.0 / 10.0, 100 rows 14.8 / 11.8, 128 rows 15.5 / 15.1, 159 rows
+// 16.5 / 17.5; with 20 alternatives 128 rows 21.1 / 21.3; losses of 128 rows 14.3 /
+// 15.0, of f32 18.1 / 20.4.
+bool whole_rows(size_t rows, int nseg) { return nseg <= 32 || rows >= 128; }
 
 int segments(size_t vocab) { return (int)((vocab + kScoreSeg - 1) / kScoreSeg); }
 

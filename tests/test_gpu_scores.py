@@ -150,7 +150,7 @@ def test_scores_over_vocabularies(hip, rows, vocab, dtype):
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("kind", ["masked", "equal", "lowest", "lowest_mask", "sorted", "few", "sure", "zeros", "huge",
                                   "mixed"])
-@pytest.mark.parametrize("rows,vocab", [(4, 60001), (260, 5003)])  # in parts and by whole rows
+@pytest.mark.parametrize("rows,vocab", [(4, 70001), (260, 5003)])  # in parts and by whole rows
 def test_scores_of_logits_that_go_wrong(hip, rows, vocab, kind, dtype):
     rng = np.random.default_rng(len(kind))
     z = make(rng, rows, vocab, kind)
@@ -184,7 +184,7 @@ def test_tokens_out_of_the_vocabulary(hip):
 def test_rows_give_the_same_bits_alone_and_among_others(hip, dtype):
     """Row by row, in parts, whole, misaligned: a row's results depend on the row."""
     rng = np.random.default_rng(8)
-    vocab, rows = 60001, 180
+    vocab, rows = 70001, 180
     z = make(rng, rows, vocab)
     tokens = pick_tokens(rng, z)
     all_ = run_scores(hip, Logits(hip, z, dtype), tokens, 0.7, 40)
@@ -324,7 +324,7 @@ def test_distillation(hip, rows, vocab, k, dtype, rest):
 @pytest.mark.parametrize("rest", [False, True])
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("kind", ["masked", "equal", "lowest", "lowest_mask", "few", "sure", "mixed"])
-@pytest.mark.parametrize("rows,vocab", [(6, 55001), (261, 2311)])
+@pytest.mark.parametrize("rows,vocab", [(6, 71001), (261, 2311)])
 def test_distillation_of_logits_that_go_wrong(hip, rows, vocab, kind, dtype, rest):
     rng = np.random.default_rng(len(kind) + 1)
     k = 12
@@ -343,7 +343,7 @@ def test_distillation_of_logits_that_go_wrong(hip, rows, vocab, kind, dtype, res
 
 
 @pytest.mark.parametrize("rest", [False, True])
-@pytest.mark.parametrize("rows,vocab", [(9, 60000), (270, 1500)])
+@pytest.mark.parametrize("rows,vocab", [(9, 70000), (270, 1500)])
 def test_teachers_that_go_wrong(hip, rows, vocab, rest):
     """Empty slots and rows, ids twice, ids outside, broken log probabilities, lists of the whole vocabulary."""
     rng = np.random.default_rng(3)
@@ -372,7 +372,7 @@ def test_teachers_that_go_wrong(hip, rows, vocab, rest):
     check_distill(hip, lg, ids, v, 1.0, rest, [1.0, 0.5, 1.0])
 
 
-@pytest.mark.parametrize("rows,vocab", [(3, 60100), (280, 4100), (165, 50001), (161, 152001)])
+@pytest.mark.parametrize("rows,vocab", [(3, 70100), (280, 4100), (165, 50001), (161, 152001)])
 def test_distillation_in_place_and_by_rows(hip, rows, vocab):
     """The gradient over the logits themselves, and the same bits for rows alone as among others."""
     rng = np.random.default_rng(4)
@@ -399,7 +399,7 @@ def test_a_teachers_scores_into_a_students_step_in_a_graph(hip):
     from detllm_amd._lib import Teacher
 
     rng = np.random.default_rng(12)
-    rows, vocab, k, T = 6, 52001, 24, 2.0
+    rows, vocab, k, T = 6, 68001, 24, 2.0
     zt, zs = make(rng, rows, vocab), make(rng, rows, vocab)
     teacher, student = Logits(hip, zt, "f32"), Logits(hip, zs, "bf16")
     f = lambda *s: hip.put(np.zeros(s, np.float32))
