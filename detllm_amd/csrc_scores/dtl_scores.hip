@@ -1290,7 +1290,12 @@ bool write_past(size_t rows, size_t row_bytes) { return rows * row_bytes > (size
 // 16384 rows of 1000 bf16 with one / four / eight: scores 30 / - / 80, with 20
 // alternatives - / 149 / 225, losses - / 57 / 93), and of sixteen where there are
 // too few rows for several workgroups a compute unit, which reads faster the more
-// waves it has (64 rows of 32000 f32 6.6 instead of 7.1).
+// waves it has (64 rows of 32000 f32 6.6 instead of 7.1).  Scores of many rows of
+// middle length take four waves too, more rows side by side for the selection to
+// hide behind: 4096 rows with 20 alternatives, four / eight waves: of 16000 f32 63 /
+// 87, of 32000 f32 104 / 131, of 49152 bf16 96 / 101, 100000 bf16 159 / 157; 400 rows of
+// 32000 bf16 17.7 / 15.8; with 128 alternatives the candidates' LDS leaves room for
+// too few (of 151936 bf16 360 / 269).
 bool wide_rows(size_t rows, int nseg) { return rows <= 256 && nseg > 8; }
 
 template <typename F>
@@ -1350,7 +1355,7 @@ void launch_token_scores(const ScoreArgs& a, hipStream_t s) {
         k.once = rows_once(a.rows, k.row_bytes, a.stats != nullptr);
         if (!TOP && k.nseg == 1) {
           if constexpr (!TOP) launch_rows(k_scores<DT, false, WHOLE, 64>, a.rows, 1, 64, lds, s, k);
-        } else if (k.nseg <= 4) {
+        } else if (k.nseg <= 4 || (a.rows >= 1024 && k.nseg <= 48 && a.top <= 32)) {
           launch_rows(k_scores<DT, TOP, WHOLE, 256>, a.rows, 1, 256, lds, s, k);
         } else if (wide_rows(a.rows, k.nseg)) {
           launch_rows(k_scores<DT, TOP, WHOLE, 1024>, a.rows, 1, 1024, lds, s, k);

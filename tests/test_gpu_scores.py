@@ -133,6 +133,16 @@ def pick_tokens(rng, z):
     return t
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_many_rows_of_middle_length(hip, dtype):
+    rng = np.random.default_rng(21)
+    z = make(rng, 1030, 9500)
+    z[::7] = np.round(z[::7])  # ties among the alternatives
+    lg = Logits(hip, z, dtype, pad=1)
+    check_scores(hip, lg, pick_tokens(rng, lg.z), 1.0, 32, step=49)
+    check_scores(hip, lg, pick_tokens(rng, lg.z), 2.0, 100, step=113)
+
+
 SHAPES = [(1, 1), (1, 2), (3, 7), (2, 63), (1, 2047), (2, 2048), (3, 2049), (5, 32003), (2, 49152), (1, 151936),
           (1, 1 << 18)]
 
