@@ -21,7 +21,7 @@ namespace {
 constexpr int kJoinThreads = 512;
 constexpr int kPartThreads = 256;
 constexpr int kPer = kScoreSeg / 64;  // logits a lane holds of a segment
-constexpr int kMostWaves = 16;  // of a row's workgroup
+constexpr int kMostWaves = 16;        // of a row's workgroup
 constexpr double kLog2E = 1.4426950408889634074;
 constexpr double kLn2 = 0.6931471805599453094;
 
@@ -49,13 +49,6 @@ template <int DT>
 struct Seg {  // a lane's logits of a segment: packets of 16 bytes, 64 lanes apart
   packet w[Type<DT>::kPackets];
 };
-
-// Where logit i of a lane lies in its segment.
-template <int DT>
-__device__ __forceinline__ int place(int i, int lane) {
-  constexpr int n = Type<DT>::kInPacket;
-  return i / n * (64 * n) + lane * n + i % n;
-}
 
 template <int DT>
 __device__ __forceinline__ float value(const packet& p, int i) {
@@ -112,7 +105,7 @@ __device__ __forceinline__ packet load_packet(const char* row, int j, int V) {
 }
 
 // ONCE: past the caches' usual policy, for logits that do not fit the 256 MB
-// memory-side cache anyway (see read_once).
+// memory-side cache anyway (see read_past).
 template <int DT, bool ONCE>
 __device__ __forceinline__ void load_seg(Seg<DT>& s, const char* row, int seg, int lane, int V) {
   constexpr int n = Type<DT>::kInPacket;
@@ -623,7 +616,7 @@ __device__ __forceinline__ long load_index(const void* p, int wide, size_t i) {
 struct ScoreK {
   const char* z;
   size_t row_bytes, row0;  // the launch's first row
-  size_t once;             // rows below it are read past the caches
+  bool once;               // read past the caches
   int V, nseg, groups;
   const void* tokens;
   int wide, top;
@@ -666,7 +659,7 @@ __global__ __launch_bounds__(THREADS) void k_scores(ScoreK a) {
   Keys<TOP ? waves : kScoreMaxSegs> key;
   if constexpr (PHASE == WHOLE) {
     uint32_t* keys = reinterpret_cast<uint32_t*>(memory);
-    read_segs<DT, true, TOP>(z, a.V, 0, a.nseg, wave, waves, lane, a.c, row < a.once, lds_parts, keys, nullptr);
+    read_segs<DT, true, TOP>(z, a.V, 0, a.nseg, wave, waves, lane, a.c, a.once, lds_parts, keys, nullptr);
     if constexpr (TOP) take_keys(key, keys, a.nseg, tl);  // each thread its own
   } else {
     for (int i = threadIdx.x; i < a.nseg; i += THREADS) lds_parts[i] = a.parts[row * a.nseg + i];
@@ -823,9 +816,9 @@ __global__ __launch_bounds__(kGradWaves * 64) void k_scores_grad(ScoreGradK a) {
 struct DistillK {
   const char* z;
   char* grad;
-  size_t row_bytes, grad_bytes, row0, once;
+  size_t row_bytes, grad_bytes, row0;
   int V, nseg, groups;
-  bool past;  // write past the caches
+  bool once, past;  // read (a loss alone), write past the caches
   const void* ids;
   int wide, k;
   const float* teacher;
@@ -1079,7 +1072,7 @@ __global__ __launch_bounds__(THREADS) void k_distill(DistillK a) {
     }
     sum_slots<REST>(s, sums, waves, a.inv_t);
     if constexpr (PHASE == WHOLE) {
-      read_segs<DT, false, false>(z, a.V, 0, a.nseg, wave, waves, lane, a.c, row < a.once, lds_parts, nullptr,
+      read_segs<DT, false, false>(z, a.V, 0, a.nseg, wave, waves, lane, a.c, a.once, lds_parts, nullptr,
                                   REST ? mask : nullptr);
     } else {
       for (int i = threadIdx.x; i < a.nseg; i += THREADS) lds_parts[i] = a.parts[row * a.nseg + i];
@@ -1272,15 +1265,12 @@ void launch_rows(void (*kernel)(K), size_t rows, int per_row, int threads, size_
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Rows to read past the caches: those reads reach 7.0 TB/s instead of 6.2 on 1.24
-// GB of logits, but leave nothing behind, and a backward pass over 32 MB of
-// logits then takes 18.6 us instead of 15.0.  So where the logits are larger than
-// the memory-side cache of 256 MB, and if a backward pass may follow (it starts
-// with the last rows) all but the last 192 MB.
-size_t rows_once(size_t rows, size_t row_bytes, bool again) {
-  if (rows * row_bytes <= (size_t)256 << 20) return 0;
-  return rows;
-}
+// Logits larger than the memory-side cache of 256 MB are read past it: 7.0 TB/s
+// instead of 6.2 on 1.24 GB.  Smaller ones are not: it leaves nothing behind, and a
+// backward pass over 32 MB then takes 18.6 us instead of 15.0.  (Leaving the last 192
+// MB of larger ones to a backward pass made the forward as much slower, 238 instead
+// of 205 us, as the backward faster.)
+bool read_past(size_t rows, size_t row_bytes) { return rows * row_bytes > (size_t)256 << 20; }
 
 // Gradients larger than the memory-side cache are written past it: 423 instead of
 // 450 us for 4096 rows of 151936 bf16, 408 instead of 426 for 2048 of f32.
@@ -1352,7 +1342,7 @@ void launch_token_scores(const ScoreArgs& a, hipStream_t s) {
       constexpr int DT = decltype(dt)::value;
       constexpr bool TOP = decltype(with_top)::value;
       if (whole_rows(a.rows, k.nseg)) {
-        k.once = rows_once(a.rows, k.row_bytes, a.stats != nullptr);
+        k.once = read_past(a.rows, k.row_bytes);
         if (!TOP && k.nseg == 1) {
           if constexpr (!TOP) launch_rows(k_scores<DT, false, WHOLE, 64>, a.rows, 1, 64, lds, s, k);
         } else if (k.nseg <= 4 || (a.rows >= 1024 && k.nseg <= 48 && a.top <= 32)) {
@@ -1469,7 +1459,7 @@ void launch_distill(const DistillArgs& a, hipStream_t s) {
   if (a.rows == 0) return;
   DistillK k = distill_kernel_args(a);
   const size_t lds = a.rest ? (size_t)k.nseg * 256 : 0;
-  k.once = a.grad ? 0 : rows_once(a.rows, k.row_bytes, a.stats != nullptr);
+  k.once = read_past(a.rows, k.row_bytes);
   by_type(a.dtype, [&](auto dt) {
     by_bool(a.rest, [&](auto with_rest) {
       constexpr int DT = decltype(dt)::value;
