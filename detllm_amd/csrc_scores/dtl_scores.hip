@@ -1014,6 +1014,13 @@ __device__ __forceinline__ bool grad_is_zero(const RowGrad& g, float scale) {
   return scale == 0.0f || g.m == -__builtin_inff();
 }
 
+// Before the slots' gradients: every store of the row's is done, not only issued
+// (a barrier by itself leaves stores of other waves in flight).
+__device__ __forceinline__ void wait_for_stores() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
 // The gradient at slot k's id, by the first slot of each distinct id.  Its
 // logit is the slots': the gradient may lie over the logits.
 template <int DT>
@@ -1194,7 +1201,7 @@ __global__ __launch_bounds__(THREADS) void k_distill_step(DistillK a) {
         grad_seg<DT>(a, x, out, g, scale, seg, lane);
       }
     }
-  __syncthreads();
+  wait_for_stores();
   const int k = threadIdx.x;
   if (!zero && k < a.k && s.id[k] >= 0) grad_slot<DT>(a, out, s, g, scale, k);
 }
@@ -1224,7 +1231,7 @@ __global__ __launch_bounds__(kGradWaves * 64) void k_distill_grad(DistillK a) {
       grad_seg<DT>(a, x, out, g, scale, seg, lane);
     }
   }
-  __syncthreads();
+  wait_for_stores();
   const int k = threadIdx.x, id = s.id[k];
   if (!zero && id >= seg0 * kScoreSeg && id < (seg0 + kGradWaves) * kScoreSeg) grad_slot<DT>(a, out, s, g, scale, k);
 }
