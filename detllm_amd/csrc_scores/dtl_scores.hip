@@ -229,8 +229,8 @@ __device__ __forceinline__ float lane_max(const Seg<DT>& z) {
 }
 
 // The sums of a segment.  NEAR: t from one fused z c - mc, mc the rounded m c
-// (the sums are then relative to mc and are brought back to m c at the end);
-// otherwise from z - m, where z c or m c could overflow.
+// (the sums are then relative to mc and are brought back to m c at the end by
+// 2^-d, d = m c - mc of up to half an ulp of mc); otherwise from z - m.
 template <int DT, bool ENT, bool NEAR>
 __device__ __forceinline__ void seg_sums(const Seg<DT>& z, float m, float c, float& sum, float& weighted) {
   float s[4] = {}, u[4] = {};
@@ -255,7 +255,9 @@ template <int DT, bool ENT>
 __device__ __forceinline__ Part seg_part(const Seg<DT>& z, float most, float c) {
   Part p{wave_max(most), 0.0f, 0.0f};
   const float m = p.m == -__builtin_inff() ? 0.0f : p.m;
-  if (__builtin_fabsf(m) < 0x1p60f)  // m c < 2^75
+  // |d| <= 2^-5 there, so that taking it through the sums costs less than a
+  // rounding.  From |m c| = 2^32 on it can pass 128, where 2^d overflows.
+  if (__builtin_fabsf(m * c) < 0x1p20f)
     seg_sums<DT, ENT, true>(z, m, c, p.s, p.u);
   else
     seg_sums<DT, ENT, false>(z, m, c, p.s, p.u);
