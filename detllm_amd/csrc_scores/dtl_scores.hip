@@ -952,11 +952,15 @@ __device__ __forceinline__ RowGrad join_distill(const DistillK& a, const RowStat
     if (sums[i].sum > 0.0) v0 = fmax(v0, sums[i].v0);
     z0 = fmax(z0, sums[i].z0);
   }
-  // total of e relative to m, the row's largest logit; left: without the list
-  double total = 1.0 + st.r, left = 0.0, m = st.m;
+  // total of e relative to m, the row's largest logit; left: without the list,
+  // which may be far below the list's: log left has no underflow
+  double total = 1.0 + st.r, left = 0.0, log_left = 0.0, m = st.m;
   if (REST) {
     m = fmax(m, z0);
-    if (st.m != no) left = exp((st.m - m) * a.inv_t) * (1.0 + st.r);
+    if (st.m != no) {
+      left = exp((st.m - m) * a.inv_t) * (1.0 + st.r);
+      log_left = (st.m - m) * a.inv_t + log1p(st.r);
+    }
     total = left;
   }
   if (m == no) {  // every logit masked: no q to compare with, nothing to move
@@ -985,15 +989,15 @@ __device__ __forceinline__ RowGrad join_distill(const DistillK& a, const RowStat
   }
   double term = own - cross * a.inv_t + mass * log_total;
   double rest = 0.0;
-  if (REST && left > 0.0) {
+  if (REST && st.m != no) {
     rest = fmax(0.0, 1.0 - mass);
-    if (rest > 0.0) term += rest * (log(rest) - (log(left) - log_total));
+    if (rest > 0.0) term += rest * (log(rest) - (log_left - log_total));
   }
   *loss = (float)((double)a.T * a.T * term);
   RowGrad g;
   g.m = (float)m;
   g.share = (float)((mass + rest) / total);
-  g.outside = rest > 0.0 ? (float)(rest / left) : 0.0f;
+  g.outside = rest > 0.0 && left > 0.0 ? (float)(rest / left) : 0.0f;
   g.log_hi = (float)log_sum;
   g.log_lo = (float)(log_sum - g.log_hi);
   return g;

@@ -3,7 +3,9 @@ they take, through the C ABI, against the definitions in 64 bits."""
 import numpy as np
 import pytest
 
+import lists64
 import rows64
+from rows64 import DTYPES
 from test_gpu_scores import (Logits, _free, check_scores, hip, make, make_teacher, near, pick_tokens,  # noqa: F401
                              run_distill, run_scores, run_scores_grad)
 
@@ -92,3 +94,71 @@ def test_gradients_of_far_logits(hip, dtype, value, T):
                 dtol = dtol + lost_distill(T, w[i], dz)
                 near(dist[1][i], dz, dtol, f"gradient of row {i} by the step")
                 near(dist[3][i], dz, dtol, f"gradient of row {i} by the backward")
+
+
+# ---- lists whose logits lie far above the others ---------------------------------------
+
+
+# in parts; whole rows whose step holds all or a part of them; few rows of middle length
+PHASES = [(4, 70001), (130, 9001), (133, 70001), (129, 151937), (5, 40003)]
+
+
+def apart(rng, rows, vocab, k, gap, T):
+    """Rows whose k listed logits lie gap * T above the largest other one."""
+    z = (rng.normal(0, 1, (rows, vocab)) * T).astype(np.float32)
+    z -= z.max(1, keepdims=True)
+    z[:, rng.random(vocab) < 0.1] = -np.inf
+    ids = np.stack([rng.permutation(vocab)[:k] for _ in range(rows)])
+    np.put_along_axis(z, ids, ((gap + rng.uniform(0, 3, (rows, k))) * T).astype(np.float32), 1)
+    p = rng.dirichlet(np.ones(k), rows) * rng.choice([0.5, 0.9, 0.999], (rows, 1))
+    return z, ids, np.log(p).astype(np.float32)
+
+
+def check_rest(hip, z, ids, v, T, dtype, loss=True, gradient=True):
+    rows = len(z)
+    lg = Logits(hip, z, dtype, pad=1)
+    w = np.random.default_rng(33).uniform(0.1, 2, rows).astype(np.float32)
+    print(f"distill with rest {rows} x {z.shape[1]} {dtype} T {T}", flush=True)
+    step, grad, alone, grad2 = run_distill(hip, lg, ids, v, T, True, w)
+    for i in range(0, rows, 1 if rows < 10 else 31):
+        want, tol, dz, dtol = lists64.distill_rest(lg.z[i], ids[i], v[i], T, float(w[i]), dtype)
+        if loss:
+            near(step[i], want, tol, f"loss of row {i}")
+            want, tol, _, _ = lists64.distill_rest(lg.z[i], ids[i], v[i], T, 1.0, dtype)
+            near(alone[i], want, tol, f"loss of row {i} alone")
+        if gradient:
+            near(grad[i], dz, dtol, f"gradient of row {i} by the step")
+            near(grad2[i], dz, dtol, f"gradient of row {i} by the backward")
+
+
+APART = [(0.5, 1.0), (50, 1.0), (95, 1.0), (95, 0.1), (300, 1.0), (300, 0.01), (800, 1.0), (2000, 1.0), (2000, 0.01), (9e4, 1e-4)]
+MASKS = [(-100.0, 1.0), (-1e4, 1.0), (-65504.0, 2.0), (-65504.0, 1e-4), (float(np.finfo(np.float32).min), 1.0),
+         (float(np.finfo(np.float32).min), 1e-4)]
+
+
+def masked(rng, rows, vocab, value):
+    """Everything outside the list at a finite mask."""
+    z = make(rng, rows, vocab)
+    ids = np.stack([rng.permutation(vocab)[:20] for _ in range(rows)])
+    listed = np.take_along_axis(z, ids, 1)
+    z[:] = value
+    np.put_along_axis(z, ids, listed, 1)
+    p = rng.dirichlet(np.ones(20), rows) * 0.9
+    return z, ids, np.log(p).astype(np.float32)
+
+
+def far_lists(hip, rows, vocab, dtype, **what):
+    rng = np.random.default_rng(34)
+    every = 1 if rows * vocab < 2000000 else 3
+    for gap, T in APART[::every]:
+        check_rest(hip, *apart(rng, rows, vocab, 20, gap, T), T, dtype, **what)
+    for value, T in MASKS[::every]:
+        if dtype == "f16":
+            value = max(value, -65504.0)
+        check_rest(hip, *masked(rng, rows, vocab, value), T, dtype, **what)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,vocab", PHASES)
+def test_losses_of_lists_far_above_the_rest(hip, rows, vocab, dtype):
+    far_lists(hip, rows, vocab, dtype, gradient=False)
