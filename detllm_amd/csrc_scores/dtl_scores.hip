@@ -811,8 +811,10 @@ __global__ __launch_bounds__(kGradWaves * 64) void k_scores_grad(ScoreGradK a) {
 //   one is the teacher's mass outside the list.
 // loss = w T^2 (sum p_k (log p_k - log q_k) + rest (log rest - log q_rest)); the
 // last term only where a logit outside the list is unmasked.
-// dz_j = w T (e_j share - p_j) with share = (sum p + rest) / sum of e, and for j
-// outside the list e_j (share - rest / sum of e outside) instead.
+// dz_j = w T (e_j share - p_j) with share = (sum p + rest) / sum of e.  For j
+// outside the list both terms are relative to the largest logit there, which may
+// lie far below the list's: with e'_j = 2^((z_j - out_m) c) <= 1 and out_a =
+// share e^((out_m - m) / T) - rest / sum of e', dz_j = w T e'_j out_a.
 // The slots' terms are formed in 64 bits: the loss is a small difference of
 // large ones.
 struct DistillK {
@@ -828,7 +830,7 @@ struct DistillK {
   float c, T;
   double inv_t;
   float* loss;
-  float* stats;  // [rows][kDistillStats]: RowGrad
+  float* stats;  // [rows][kDistillStats]: put_stats
   Part* parts;
 };
 
@@ -925,12 +927,28 @@ __device__ __forceinline__ void sum_slots(const Slots& s, SlotSums* sums, int wa
   }
 }
 
-// What a row's gradient needs besides its logits: m, share, rest / sum outside,
-// and the log of the teacher's sum as a float and what it leaves.
+// What a row's gradient needs besides its logits: m and share for the list's,
+// out_m and out_a for the others, and the log of the teacher's sum as a float and
+// what it leaves (with rest 0: p = e^v).
 struct RowGrad {
-  float m, share, outside, log_hi, log_lo;
+  float m, share, out_m, out_a, log_hi, log_lo;
 };
-static_assert(sizeof(RowGrad) == kDistillStats * sizeof(float), "stats");
+
+// From the forward to the backward: without rest out_m is m and out_a is share.
+template <bool REST>
+__device__ __forceinline__ void put_stats(float* stats, size_t row, const RowGrad& g) {
+  float* s = stats + row * kDistillStats;
+  s[0] = g.m;
+  s[1] = g.share;
+  s[2] = REST ? g.out_m : g.log_hi;
+  s[3] = REST ? g.out_a : g.log_lo;
+  s[4] = 0.0f;
+}
+template <bool REST>
+__device__ __forceinline__ RowGrad get_stats(const float* stats, size_t row) {
+  const float* s = stats + row * kDistillStats;
+  return REST ? RowGrad{s[0], s[1], s[2], s[3], 0.0f, 0.0f} : RowGrad{s[0], s[1], s[0], s[1], s[2], s[3]};
+}
 
 // The row's loss (times T^2) and what its gradient needs, from the row's stats
 // (with rest those outside the list) and the slots' sums.
@@ -943,7 +961,7 @@ __device__ __forceinline__ RowGrad join_distill(const DistillK& a, const RowStat
   }
   if (st.bad || (state & BROKEN)) {
     *loss = nan;
-    return RowGrad{nan, nan, nan, nan, nan};
+    return RowGrad{nan, nan, nan, nan, nan, nan};
   }
   constexpr int n = kDistillMaxK / 64;
   double v0 = no, z0 = no;
@@ -952,20 +970,19 @@ __device__ __forceinline__ RowGrad join_distill(const DistillK& a, const RowStat
     if (sums[i].sum > 0.0) v0 = fmax(v0, sums[i].v0);
     z0 = fmax(z0, sums[i].z0);
   }
-  // total of e relative to m, the row's largest logit; left: without the list,
-  // which may be far below the list's: log left has no underflow
-  double total = 1.0 + st.r, left = 0.0, log_left = 0.0, m = st.m;
+  // total of e relative to m, the row's largest logit.  With rest st has the sums
+  // without the list; down: from its maximum to m, and log left, the log of what
+  // the others have of the total, without down's underflow.
+  double total = 1.0 + st.r, down = 1.0, log_left = 0.0, m = st.m;
   if (REST) {
     m = fmax(m, z0);
-    if (st.m != no) {
-      left = exp((st.m - m) * a.inv_t) * (1.0 + st.r);
-      log_left = (st.m - m) * a.inv_t + log1p(st.r);
-    }
-    total = left;
+    down = st.m == no ? 0.0 : exp((st.m - m) * a.inv_t);
+    log_left = (st.m - m) * a.inv_t + log1p(st.r);
+    total = down * (1.0 + st.r);
   }
   if (m == no) {  // every logit masked: no q to compare with, nothing to move
     *loss = __builtin_inff();
-    return RowGrad{no, 0.0f, 0.0f, 0.0f, 0.0f};
+    return RowGrad{no, 0.0f, no, 0.0f, 0.0f, 0.0f};
   }
   double mass = 0.0, own = 0.0, cross = 0.0;  // sum of p, p v and p (z - m)
 #pragma unroll
@@ -997,19 +1014,22 @@ __device__ __forceinline__ RowGrad join_distill(const DistillK& a, const RowStat
   RowGrad g;
   g.m = (float)m;
   g.share = (float)((mass + rest) / total);
-  g.outside = rest > 0.0 && left > 0.0 ? (float)(rest / left) : 0.0f;
+  // where every logit outside is masked e' is 0 as long as out_m is finite
+  g.out_m = REST && st.m == no ? g.m : st.m;
+  g.out_a = (float)(down * ((mass + rest) / total) - rest / (1.0 + st.r));
   g.log_hi = (float)log_sum;
   g.log_lo = (float)(log_sum - g.log_hi);
   return g;
 }
 
-// Gradient of a segment for every j as if outside the list.
+// Gradient of a segment for every j as if outside the list (a listed logit's may
+// be anything: its slot writes it again).
 template <int DT>
 __device__ __forceinline__ void grad_seg(const DistillK& a, const Seg<DT>& s, char* out, const RowGrad& g, float scale,
                                          int seg, int lane) {
-  const float A = scale * (g.share - g.outside);
+  const float A = scale * g.out_a;
   write_seg<DT>(s, out, seg, lane, a.V, a.past,
-                [&](float v, int) { return __builtin_amdgcn_exp2f((v - g.m) * a.c) * A; });
+                [&](float v, int) { return __builtin_amdgcn_exp2f((v - g.out_m) * a.c) * A; });
 }
 template <int DT>
 __device__ __forceinline__ void zero_seg(char* out, int seg, int lane, int V) {
@@ -1100,7 +1120,7 @@ __global__ __launch_bounds__(THREADS) void k_distill(DistillK a) {
   const RowGrad g = join_distill<REST>(a, st, sums, state, &loss);
   if (lane == 0) {
     a.loss[row] = state ? w * loss : 0.0f;
-    if (a.stats) reinterpret_cast<RowGrad*>(a.stats)[row] = g;
+    if (a.stats) put_stats<REST>(a.stats, row, g);
   }
 }
 
@@ -1214,7 +1234,7 @@ __global__ __launch_bounds__(THREADS) void k_distill_step(DistillK a) {
 
 // The gradient alone, from the stats of the forward: workgroups of four segments
 // of a row each (2048 rows of 151936 f32: 447 us, 467 with sixteen).
-template <int DT>
+template <int DT, bool REST>
 __global__ __launch_bounds__(kGradWaves * 64) void k_distill_grad(DistillK a) {
   __shared__ Slots s;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1223,7 +1243,7 @@ __global__ __launch_bounds__(kGradWaves * 64) void k_distill_grad(DistillK a) {
   const char* z = a.z + row * a.row_bytes;
   char* out = a.grad + row * a.grad_bytes;
   const float weight = a.weights ? a.weights[row] : 1.0f;
-  const RowGrad g = reinterpret_cast<const RowGrad*>(a.stats)[row];
+  const RowGrad g = get_stats<REST>(a.stats, row);
   load_slots<DT, false>(s, a, row, z);
   __syncthreads();
   const float scale = slots_state(s) ? weight * a.T : 0.0f;
@@ -1429,7 +1449,7 @@ DistillK distill_kernel_args(const DistillArgs& a) {
 // Parts, and for a step of few rows the stats between its launches.
 size_t distill_scratch_bytes(size_t rows, size_t vocab, bool step) {
   if (whole_rows(rows, segments(vocab))) return 0;
-  return round256(rows * segments(vocab) * sizeof(Part)) + (step ? rows * sizeof(RowGrad) : 0);
+  return round256(rows * segments(vocab) * sizeof(Part)) + (step ? rows * kDistillStats * sizeof(float) : 0);
 }
 
 void launch_distill_grad(const DistillArgs& a, hipStream_t s) {
@@ -1437,7 +1457,9 @@ void launch_distill_grad(const DistillArgs& a, hipStream_t s) {
   DistillK k = distill_kernel_args(a);
   k.groups = (k.nseg + kGradWaves - 1) / kGradWaves;
   by_type(a.dtype, [&](auto dt) {
-    launch_rows(k_distill_grad<decltype(dt)::value>, a.rows, k.groups, kGradWaves * 64, 0, s, k);
+    constexpr int DT = decltype(dt)::value;
+    launch_rows(a.rest ? k_distill_grad<DT, true> : k_distill_grad<DT, false>, a.rows, k.groups, kGradWaves * 64, 0, s,
+                k);
   });
 }
 

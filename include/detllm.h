@@ -348,7 +348,8 @@ size_t dtl_distill_scratch(size_t rows, size_t vocab);
 int dtl_distill(const dtl_logits *logits, const dtl_teacher *teacher, float temperature, float *loss,
                 float *stats, void *scratch, size_t scratch_bytes, void *stream);
 /* The gradient of the logits (as in dtl_token_scores_backward) for the gradient
- * of each row's loss.  Zero in rows whose gradient is zero, that have no slot in
+ * of each row's loss; teacher (its rest too), temperature and stats are the
+ * forward's.  Zero in rows whose gradient is zero, that have no slot in
  * use or whose logits are all masked. */
 int dtl_distill_backward(const dtl_logits *logits, const dtl_teacher *teacher, float temperature,
                          const float *stats, const float *grad_loss, void *grad, size_t grad_stride,

@@ -162,3 +162,9 @@ def far_lists(hip, rows, vocab, dtype, **what):
 @pytest.mark.parametrize("rows,vocab", PHASES)
 def test_losses_of_lists_far_above_the_rest(hip, rows, vocab, dtype):
     far_lists(hip, rows, vocab, dtype, gradient=False)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,vocab", PHASES)
+def test_gradients_of_lists_far_above_the_rest(hip, rows, vocab, dtype):
+    far_lists(hip, rows, vocab, dtype, loss=False)
