@@ -7,7 +7,8 @@ gradients.  The calls enqueue the library's kernels (dtl_token_scores*,
 dtl_distill* of include/detllm.h, which define every result) on the current
 stream of the logits' device, do not wait, and can be captured into a graph (a
 captured backward needs a leaf of its own, `logits.detach().requires_grad_()`: one
-whose eager graph is still alive belongs to that graph's stream).
+whose eager graph is still alive belongs to that graph's stream).  Reverse mode only:
+tensors with a forward-mode tangent and torch.jit.trace are refused.
 
     teacher = scores.token_scores(teacher_logits, tokens, top=32, temperature=2.0)
     loss = scores.distill_loss(student_logits, teacher.top_ids, teacher.top_log_probs,
@@ -24,6 +25,7 @@ from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import DetllmError, check, lib
@@ -56,14 +58,28 @@ class TokenScores(NamedTuple):
     top_log_probs: Optional[torch.Tensor]
 
 
-def _need_logits(t: torch.Tensor, name: str = "logits") -> None:
+def _no_tangent(t: torch.Tensor, name: str) -> None:
+    """The kernels see a tensor's values alone: the tangent of a dual tensor would be
+    lost, and torch takes a missing one for zero."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{name} has a tangent: there is no forward-mode derivative")
+
+
+# Without its wrapper, as _device_now below.
+_tracing = getattr(torch._C, "_is_tracing", None) or torch.jit.is_tracing
+
+
+def _need_logits(t: torch.Tensor) -> None:
+    """What a call asks of its logits first, before autograd unpacks them."""
     if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES:
-        raise TypeError(f"{name} must be a float32, bfloat16 or float16 tensor")
+        raise TypeError("logits must be a float32, bfloat16 or float16 tensor")
+    _no_tangent(t, "logits")
+    if _tracing():
+        raise RuntimeError("calls of the library cannot be recorded by torch.jit.trace")
 
 
 def _logits_view(t: torch.Tensor, name: str = "logits") -> _lib.Logits:
     """The tensor's rows as a dtl_logits."""
-    _need_logits(t, name)
     if not t.is_cuda:
         raise ValueError(f"{name} must be on the GPU")
     shape, strides = t.shape, t.stride()
@@ -89,6 +105,7 @@ def _logits_view(t: torch.Tensor, name: str = "logits") -> _lib.Logits:
 def _beside(t: torch.Tensor, logits: torch.Tensor, shape, dtypes, name: str) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
         raise TypeError(f"{name} must be a tensor of {' or '.join(str(d) for d in dtypes)}")
+    _no_tangent(t, name)
     if t.device != logits.device:
         raise ValueError(f"{name} and logits are on different devices")
     if t.shape != shape:
@@ -130,6 +147,14 @@ def _scratch(n: int, device: torch.device) -> Optional[torch.Tensor]:
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
+def _incoming(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """The gradient that a backward is given."""
+    if g is None:
+        return None
+    _no_tangent(g, "the gradient")
+    return g.contiguous()
+
+
 # ---- scores ------------------------------------------------------------------
 
 
@@ -169,8 +194,8 @@ class _TokenScores(torch.autograd.Function):
     def backward(ctx, g, h, _ids, _lps):
         logits, tokens, stats, entropy = ctx.saved_tensors
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        g = None if g is None else g.contiguous()
-        h = None if h is None else h.contiguous()
+        g = _incoming(g)
+        h = _incoming(h)
         z = _logits_view(logits)
         _call(logits.device, lib.dtl_token_scores_backward, C.byref(z), _ptr(tokens),
               0 if tokens is None else tokens.element_size(), ctx.temperature, _ptr(stats), _ptr(entropy), _ptr(g),
@@ -234,7 +259,7 @@ class _Distill(torch.autograd.Function):
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         z = _logits_view(logits)
         t = _teacher_view(ids, log_probs, ctx.rest)
-        g = g.contiguous()
+        g = _incoming(g)
         _call(logits.device, lib.dtl_distill_backward, C.byref(z), C.byref(t), ctx.temperature, _ptr(stats), _ptr(g),
               _ptr(grad), z.vocab)
         return grad, None, None, None, None
@@ -246,9 +271,9 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_log_pr
     and teacher_log_probs[..., k] (k up to 256), differentiable in the logits.
 
     teacher_log_probs (float32) are at this temperature, as token_scores with
-    the same temperature gives them.  rest=False compares within the list's
-    renormalised probabilities; rest=True keeps them as they are and compares
-    what lies outside the list as one more outcome."""
+    the same temperature gives them, and constants to autograd.  rest=False
+    compares within the list's renormalised probabilities; rest=True keeps them as
+    they are and compares what lies outside the list as one more outcome."""
     _need_logits(logits)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _Distill.apply(logits, teacher_ids, teacher_log_probs, float(temperature), bool(rest))
@@ -263,6 +288,7 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
     ones) before the loss.  One pass instead of a forward and a backward; pass the
     gradient on with `logits.backward(grad)`.  out: where the gradient goes, of the
     logits' shape and type; the logits themselves if nothing needs them again."""
+    _need_logits(logits)
     z = _logits_view(logits)
     t, teacher_ids, teacher_log_probs = _teacher(logits, teacher_ids, teacher_log_probs, rest)
     dev = logits.device
@@ -275,6 +301,7 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
     else:
         if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev:
             raise ValueError("out must have the shape, type and device of logits")
+        _no_tangent(out, "out")
         stride = _logits_view(out, "out").stride
     loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
     n = _distill_scratch(z.rows, z.vocab)
