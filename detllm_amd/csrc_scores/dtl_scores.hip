@@ -1086,12 +1086,15 @@ __global__ __launch_bounds__(THREADS) void k_distill(DistillK a) {
   const char* z = a.z + row * a.row_bytes;
   const float w = a.weights ? a.weights[row] : 1.0f;
 
-  if (REST)
-    for (int i = threadIdx.x; i < a.nseg * 64; i += THREADS) mask[i] = 0;
-  load_slots<DT, REST>(s, a, row, z);
-  __syncthreads();
   // a row that does not count, or has no slots in use, is not read
-  const int state = w == 0.0f ? 0 : slots_state(s);
+  int state = 0;
+  if (w != 0.0f) {
+    if (REST)
+      for (int i = threadIdx.x; i < a.nseg * 64; i += THREADS) mask[i] = 0;
+    load_slots<DT, REST>(s, a, row, z);
+    __syncthreads();
+    state = slots_state(s);
+  }
   if (state) {
     if (REST) {
       if (threadIdx.x < kDistillMaxK && s.id[threadIdx.x] >= 0) mask_bit<DT>(mask, s.id[threadIdx.x]);
@@ -1243,6 +1246,10 @@ __global__ __launch_bounds__(kGradWaves * 64) void k_distill_grad(DistillK a) {
   const char* z = a.z + row * a.row_bytes;
   char* out = a.grad + row * a.grad_bytes;
   const float weight = a.weights ? a.weights[row] : 1.0f;
+  if (weight == 0.0f) {  // a row that does not count is not read
+    if (seg < a.nseg) zero_seg<DT>(out, seg, lane, a.V);
+    return;
+  }
   const RowGrad g = get_stats<REST>(a.stats, row);
   load_slots<DT, false>(s, a, row, z);
   __syncthreads();

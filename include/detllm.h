@@ -356,8 +356,9 @@ int dtl_distill_backward(const dtl_logits *logits, const dtl_teacher *teacher, f
                          void *stream);
 /* Both in one call for row weights known beforehand (NULL: ones): loss[row] is
  * weights[row] times dtl_distill's, grad the gradient of their sum.  Reads the
- * logits once (of rows past 32768 logits a part again, mostly from the caches).
- * A row of weight 0 is not read: loss 0, gradient 0. */
+ * logits once (of rows past 32768 logits a part again, mostly from the caches;
+ * fewer than 128 rows past 65536 logits twice).  A row of weight 0 is not read,
+ * nor are its ids and log probabilities: loss 0, gradient 0. */
 int dtl_distill_step(const dtl_logits *logits, const dtl_teacher *teacher, float temperature,
                      const float *weights, float *loss, void *grad, size_t grad_stride, void *scratch,
                      size_t scratch_bytes, void *stream);

@@ -168,3 +168,23 @@ def test_losses_of_lists_far_above_the_rest(hip, rows, vocab, dtype):
 @pytest.mark.parametrize("rows,vocab", PHASES)
 def test_gradients_of_lists_far_above_the_rest(hip, rows, vocab, dtype):
     far_lists(hip, rows, vocab, dtype, loss=False)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("rows,vocab", [(6, 70001), (6, 5003), (130, 70001)])
+def test_rows_of_weight_0(hip, rows, vocab, rest):
+    """Whatever they, their list and their stats hold: zeros, and the others as without them."""
+    rng = np.random.default_rng(35)
+    z = make(rng, rows, vocab)
+    ids, v = make_teacher(rng, z, 7)
+    w = rng.uniform(0.5, 1, rows).astype(np.float32)
+    off = np.arange(rows) % 3 == 1
+    w[off] = 0.0
+    want = run_distill(hip, Logits(hip, z, "f32"), ids, v, 1.0, rest, w)
+    z[off, ::5] = np.nan
+    ids[off, 0], ids[off, 1], v[off, 2] = vocab, 1 << 30, np.nan
+    got = run_distill(hip, Logits(hip, z, "f32"), ids, v, 1.0, rest, w)
+    for a, b in zip(got, want):
+        assert np.array_equal(a[~off], b[~off])
+    assert not got[0][off].any() and not got[1][off].any() and not got[3][off].any()
+    assert np.isnan(got[2][off]).all()  # the loss alone knows no weights
