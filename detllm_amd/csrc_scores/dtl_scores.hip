@@ -1569,10 +1569,30 @@ int check_logits(const dtl_logits* z) {
 }
 bool index_bytes_ok(int n) { return n == 4 || n == 8; }
 bool temperature_ok(float t) { return t >= kScoreMinTemperature && t <= kScoreMaxTemperature; }
+
+// Whether a row of the gradient lies over a part of the logits' rows other than
+// itself: logits would be overwritten that another wave has yet to read.  Rows may
+// interleave (two halves of one matrix, say).
+bool overlap(const dtl_logits* z, const void* grad, size_t grad_stride) {
+  const size_t n = type_bytes(z->dtype), row = z->vocab * n, zs = z->stride * n, gs = grad_stride * n, last = z->rows - 1;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(z->data), g = reinterpret_cast<uintptr_t>(grad);
+  if (last == 0) return a != g && a < g + row && g < a + row;
+  if (a == g && zs == gs) return false;
+  if (a >= g + last * gs + row || g >= a + last * zs + row) return false;
+  for (size_t i = 0; i <= last; i++) {  // against the last of the gradient's rows that begins before this one's end
+    const uintptr_t at = a + i * zs;
+    if (at + row <= g) continue;
+    const size_t j = (at + row - 1 - g) / gs;
+    if (at < g + (j < last ? j : last) * gs + row) return true;
+  }
+  return false;
+}
+
 int check_grad(const dtl_logits* z, const void* grad, size_t stride) {
   if (!stride_ok(z, stride)) return DTL_ERR_SHAPE;
-  if (z->rows && (!grad || reinterpret_cast<uintptr_t>(grad) % type_bytes(z->dtype))) return DTL_ERR_INVALID_ARGUMENT;
-  return DTL_OK;
+  if (z->rows == 0) return DTL_OK;
+  if (!grad || reinterpret_cast<uintptr_t>(grad) % type_bytes(z->dtype)) return DTL_ERR_INVALID_ARGUMENT;
+  return overlap(z, grad, stride) ? DTL_ERR_INVALID_ARGUMENT : DTL_OK;
 }
 
 DistillArgs distill_args(const dtl_logits* z, const dtl_teacher* t, float temperature) {

@@ -287,7 +287,8 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
     loops that know the rows' weights (1 / rows for a mean, 0 for padding; None:
     ones) before the loss.  One pass instead of a forward and a backward; pass the
     gradient on with `logits.backward(grad)`.  out: where the gradient goes, of the
-    logits' shape and type; the logits themselves if nothing needs them again."""
+    logits' shape and type; the logits themselves if nothing needs them again, but
+    not memory that holds other rows' or only a part of them."""
     _need_logits(logits)
     z = _logits_view(logits)
     t, teacher_ids, teacher_log_probs = _teacher(logits, teacher_ids, teacher_log_probs, rest)

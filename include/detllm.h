@@ -313,8 +313,8 @@ int dtl_token_scores(const dtl_logits *logits, const void *tokens, int token_byt
                      size_t top, float *log_probs, float *entropy, float *stats, int32_t *top_ids,
                      float *top_log_probs, void *scratch, size_t scratch_bytes, void *stream);
 /* The gradient of the logits (their type, row i at grad + i * grad_stride
- * elements; may be the logits themselves at the same stride) for the gradients
- * of log_probs and of entropy, either of which may be NULL.  stats and entropy
+ * elements; may be the logits themselves at the same stride, or lie between their
+ * rows, but not over a part of them) for the gradients of log_probs and of entropy, either of which may be NULL.  stats and entropy
  * are the forward's.  Zero in rows whose gradients are zero (padding's is) or
  * whose logits are all masked, whatever else they hold; NaN in rows that gave
  * NaN. */

@@ -102,3 +102,20 @@ def test_saved_tensors_through_hooks():
     assert torch.equal(got, want)
     got, = torch.autograd.grad(checkpoint(loss, leaf, use_reentrant=False), leaf)
     assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_out_over_a_part_of_the_logits_is_refused():
+    from detllm_amd._lib import DetllmError
+
+    wide = torch.randn(4, 100, device=GPU)
+    ids, v = torch.arange(6, dtype=torch.int32, device=GPU).repeat(3, 1), torch.full((3, 6), -2.0, device=GPU)
+    for z, out in ((wide[:3, :50], wide[:3, 1:51]), (wide[:3], wide[1:]), (wide[:3, :50], wide.view(-1)[:150].view(3, 50))):
+        with pytest.raises(DetllmError) as e:
+            scores.distill_loss_and_grad(z, ids, v, out=out)
+        assert e.value.status == 42
+    want = scores.distill_loss_and_grad(wide[:3, :50], ids, v)[1]
+    _, got = scores.distill_loss_and_grad(wide[:3, :50], ids, v, out=wide[:3, 50:])
+    assert torch.equal(got, want) and torch.equal(wide[:3, 50:], want)
+    scores.distill_loss_and_grad(wide[:3, :50], ids, v, out=wide[:3, :50])
+    assert torch.equal(wide[:3, :50], want)
