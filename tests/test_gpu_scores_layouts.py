@@ -52,3 +52,19 @@ def test_gradients_between_the_rows_of_the_logits(hip, rows, vocab, dtype):
     assert hip.dtl.dtl_distill(C.byref(lg), C.byref(t), 1.0, loss, stats, sc, n, hip.stream) == 0
     assert hip.dtl.dtl_distill_backward(C.byref(lg), C.byref(t), 1.0, stats, dw, right, stride, hip.stream) == 0
     assert np.array_equal(gradient(), want[4]) and np.array_equal(hip.get(loss, np.float32, rows), want[3])
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("rows,vocab", [(129, 152001), (140, 66001), (5, 60001), (130, 33001), (3, 9001)])
+def test_steps_in_place(hip, rows, vocab, dtype, rest):
+    """Every shape of the step, its gradient over the logits: of rows held whole, held in part, in parts."""
+    rng = np.random.default_rng(42)
+    z = make(rng, rows, vocab)
+    ids, v = make_teacher(rng, z, 25)
+    w = rng.uniform(0.5, 1, rows).astype(np.float32)
+    want = run_distill(hip, Logits(hip, z, dtype, pad=1), ids, v, 0.5, rest, w)
+    got = run_distill(hip, Logits(hip, z, dtype, pad=1), ids, v, 0.5, rest, w, in_place=True)
+    for a, b in zip(got, want):
+        assert np.array_equal(a, b)
+    assert np.array_equal(want[1], want[3])

@@ -188,3 +188,76 @@ def test_rows_of_weight_0(hip, rows, vocab, rest):
         assert np.array_equal(a[~off], b[~off])
     assert not got[0][off].any() and not got[1][off].any() and not got[3][off].any()
     assert np.isnan(got[2][off]).all()  # the loss alone knows no weights
+
+
+# ---- every temperature -----------------------------------------------------------------
+
+
+EVERY_T = [1e-4, 0.1, 1.0, 1e4]
+SPLIT_AND_WHOLE = [(4, 70001), (130, 5003)]
+KINDS = ["text", "sure", "masked", "lowest_mask", "huge"]
+
+
+def logits_of(hip, rng, rows, vocab, kind, dtype):
+    z = make(rng, rows, vocab, kind)
+    if dtype == "f16":
+        z = np.where(np.isfinite(z), np.clip(z, -65504.0, 65504.0), z).astype(np.float32)
+    return Logits(hip, z, dtype, pad=3)
+
+
+@pytest.mark.parametrize("T", EVERY_T)
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,vocab", SPLIT_AND_WHOLE)
+def test_gradients_of_scores_at_temperatures(hip, rows, vocab, dtype, T):
+    rng = np.random.default_rng(36)
+    for kind in KINDS:
+        lg = logits_of(hip, rng, rows, vocab, kind, dtype)
+        tokens = pick_tokens(rng, lg.z)
+        tokens[1] = -1
+        g, h = rng.normal(0, 1, rows).astype(np.float32), rng.normal(0, 0.3, rows).astype(np.float32)
+        print(f"gradient {rows} x {vocab} {dtype} {kind} T {T}", flush=True)
+        got = run_scores(hip, lg, tokens, T, 0)
+        grad = run_scores_grad(hip, lg, got, T, g, h, pad=1)
+        for i in range(0, rows, 1 if rows < 10 else 43):
+            want, tol = rows64.scores_grad(lg.z[i], int(tokens[i]), T, float(g[i]), float(h[i]), got["h"][i], dtype)
+            row = rows64.Row(lg.z[i], T)
+            near(grad[i], want, tol + lost_score(T, g[i], h[i], row.H, row.L), f"gradient of row {i}")
+
+
+@pytest.mark.parametrize("T", EVERY_T)
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,vocab", SPLIT_AND_WHOLE)
+def test_distillation_at_temperatures(hip, rows, vocab, dtype, T):
+    rng = np.random.default_rng(37)
+    for kind in KINDS:
+        lg = logits_of(hip, rng, rows, vocab, kind, dtype)
+        ids, v = make_teacher(rng, lg.z, 14)
+        # the teacher keeps to what is unmasked, each id once
+        v = np.where(np.isfinite(np.take_along_axis(lg.z, ids, 1)), v, -np.inf)
+        for i, row in enumerate(ids):
+            v[i, np.setdiff1d(np.arange(row.size), np.unique(row, return_index=True)[1])] = -np.inf
+        v = v.astype(np.float32)
+        w = rng.uniform(0.1, 2, rows).astype(np.float32)
+        for rest in (False, True):
+            print(f"distill {rows} x {vocab} {dtype} {kind} T {T} rest {rest}", flush=True)
+            step, grad, alone, grad2 = run_distill(hip, lg, ids, v, T, rest, w)
+            for i in range(0, rows, 1 if rows < 10 else 43):
+                if rest:
+                    loss, tol, dz, dtol = lists64.distill_rest(lg.z[i], ids[i], v[i], T, float(w[i]), dtype)
+                else:
+                    loss, tol, dz, dtol = rows64.distill(lg.z[i], ids[i], v[i], T, False, float(w[i]), dtype)
+                    dtol = dtol + lost_distill(T, w[i], dz)
+                near(step[i], loss, tol, f"loss of row {i}")
+                near(grad[i], dz, dtol, f"gradient of row {i} by the step")
+                near(grad2[i], dz, dtol, f"gradient of row {i} by the backward")
+
+
+@pytest.mark.parametrize("T", [1.0, 0.1, 0.01])
+@pytest.mark.parametrize("dtype,value", FAR[:7])
+def test_distillation_with_rest_of_far_logits(hip, dtype, value, T):
+    for rows, vocab in ((3, 70003), (130, 4100)):
+        rng = np.random.default_rng(38)
+        for kind in ("tail", "half"):
+            z = far(rng, rows, vocab, value, kind)
+            ids = np.stack([rng.permutation(2048)[:9] for _ in range(rows)])  # ordinary logits
+            check_rest(hip, z, ids, np.log(rng.dirichlet(np.ones(9), rows) * 0.8).astype(np.float32), T, dtype)

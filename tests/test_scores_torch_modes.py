@@ -1,4 +1,5 @@
-"""torch_scores_modes.py in a process of its own, where torch is loaded first."""
+"""torch_scores_modes.py and torch_scores_large.py in processes of their own, where
+torch is loaded first."""
 import subprocess
 import sys
 from pathlib import Path
@@ -8,8 +9,8 @@ import pytest
 HERE = Path(__file__).resolve().parent
 
 
-def run(which):
-    subprocess.run([sys.executable, "-u", "-m", "pytest", str(HERE / "torch_scores_modes.py"), "-v", "-m", which, "-p",
+def run(which, name="torch_scores_modes.py"):
+    subprocess.run([sys.executable, "-u", "-m", "pytest", str(HERE / name), "-v", "-m", which, "-p",
                     "no:cacheprovider", "--timeout", "60", "--timeout-method", "thread"], cwd=HERE.parent, check=True,
                    timeout=300)
 
@@ -21,3 +22,8 @@ def test_without_a_gpu():
 @pytest.mark.gpu
 def test_on_the_gpu():
     run("gpu")
+
+
+@pytest.mark.gpu
+def test_past_the_cache():
+    run("gpu", "torch_scores_large.py")
