@@ -892,7 +892,7 @@ __device__ __forceinline__ void mask_bit(uint32_t* mask, int id) {
 // What the slots alone give, a wave's share: with p proportional to e^(v - v0),
 // v0 the share's largest v (0 with rest, where p = e^v), z0 its largest logit.
 struct SlotSums {
-  double v0, sum, sum_v, sum_z;  // of e^(v - v0), and of it times v and times z - z0
+  double v0, sum, sum_v, sum_z;  // of e^(v - v0), and of it times v - v0 and times z - z0
   double z0, in;                 // rest: sum of e^((z - z0) / T) over distinct ids
 };
 
@@ -909,7 +909,7 @@ __device__ __forceinline__ void sum_slots(const Slots& s, SlotSums* sums, int wa
     }
     const double e = id >= 0 ? exp((double)v - t.v0) : 0.0;
     t.sum = wave_sum(e);
-    t.sum_v = wave_sum(e > 0.0 ? e * v : 0.0);
+    t.sum_v = wave_sum(e > 0.0 ? e * ((double)v - t.v0) : 0.0);
     const float z0 = wave_max(id >= 0 ? z : no);
     t.z0 = z0;
     t.sum_z = wave_sum(!(e > 0.0) ? 0.0 : z == no ? (double)no : e * ((double)z - z0));
@@ -928,10 +928,11 @@ __device__ __forceinline__ void sum_slots(const Slots& s, SlotSums* sums, int wa
 }
 
 // What a row's gradient needs besides its logits: m and share for the list's,
-// out_m and out_a for the others, and the log of the teacher's sum as a float and
-// what it leaves (with rest 0: p = e^v).
+// out_m and out_a for the others, and for p = e^(v - v0) / sum the list's largest v
+// and the log of the sum as a float and what it leaves (with rest all 0: p = e^v).
+// v0 is not joined with the log, which a v0 of any size would swallow.
 struct RowGrad {
-  float m, share, out_m, out_a, log_hi, log_lo;
+  float m, share, out_m, out_a, v0, log_hi, log_lo;
 };
 
 // From the forward to the backward: without rest out_m is m and out_a is share.
@@ -940,14 +941,14 @@ __device__ __forceinline__ void put_stats(float* stats, size_t row, const RowGra
   float* s = stats + row * kDistillStats;
   s[0] = g.m;
   s[1] = g.share;
-  s[2] = REST ? g.out_m : g.log_hi;
-  s[3] = REST ? g.out_a : g.log_lo;
-  s[4] = 0.0f;
+  s[2] = REST ? g.out_m : g.v0;
+  s[3] = REST ? g.out_a : g.log_hi;
+  s[4] = REST ? 0.0f : g.log_lo;
 }
 template <bool REST>
 __device__ __forceinline__ RowGrad get_stats(const float* stats, size_t row) {
   const float* s = stats + row * kDistillStats;
-  return REST ? RowGrad{s[0], s[1], s[2], s[3], 0.0f, 0.0f} : RowGrad{s[0], s[1], s[0], s[1], s[2], s[3]};
+  return REST ? RowGrad{s[0], s[1], s[2], s[3], 0.0f, 0.0f, 0.0f} : RowGrad{s[0], s[1], s[0], s[1], s[2], s[3], s[4]};
 }
 
 // The row's loss (times T^2) and what its gradient needs, from the row's stats
@@ -961,7 +962,7 @@ __device__ __forceinline__ RowGrad join_distill(const DistillK& a, const RowStat
   }
   if (st.bad || (state & BROKEN)) {
     *loss = nan;
-    return RowGrad{nan, nan, nan, nan, nan, nan};
+    return RowGrad{nan, nan, nan, nan, nan, nan, nan};
   }
   constexpr int n = kDistillMaxK / 64;
   double v0 = no, z0 = no;
@@ -982,9 +983,9 @@ __device__ __forceinline__ RowGrad join_distill(const DistillK& a, const RowStat
   }
   if (m == no) {  // every logit masked: no q to compare with, nothing to move
     *loss = __builtin_inff();
-    return RowGrad{no, 0.0f, no, 0.0f, 0.0f, 0.0f};
+    return RowGrad{no, 0.0f, no, 0.0f, 0.0f, 0.0f, 0.0f};
   }
-  double mass = 0.0, own = 0.0, cross = 0.0;  // sum of p, p v and p (z - m)
+  double mass = 0.0, own = 0.0, cross = 0.0;  // sum of p, p (v - v0) and p (z - m)
 #pragma unroll
   for (int i = 0; i < n; i++) {
     const SlotSums& x = sums[i];
@@ -992,14 +993,14 @@ __device__ __forceinline__ RowGrad join_distill(const DistillK& a, const RowStat
     const double f = x.sum > 0.0 ? exp(x.v0 - v0) : 0.0;
     if (f > 0.0) {
       mass += f * x.sum;
-      own += f * x.sum_v;
+      own += f * (x.sum_v + x.sum * (x.v0 - v0));
       cross += f * (x.sum_z + x.sum * (x.z0 - m));
     }
   }
   const double log_total = REST ? log(total) : log1p(st.r);
   double log_sum = 0.0;
   if (!REST) {
-    log_sum = v0 + log(mass);
+    log_sum = log(mass);
     cross /= mass;
     own = own / mass - log_sum;
     mass = 1.0;
@@ -1017,6 +1018,7 @@ __device__ __forceinline__ RowGrad join_distill(const DistillK& a, const RowStat
   // where every logit outside is masked e' is 0 as long as out_m is finite
   g.out_m = REST && st.m == no ? g.m : st.m;
   g.out_a = (float)(down * ((mass + rest) / total) - rest / (1.0 + st.r));
+  g.v0 = REST ? 0.0f : (float)v0;
   g.log_hi = (float)log_sum;
   g.log_lo = (float)(log_sum - g.log_hi);
   return g;
@@ -1066,9 +1068,10 @@ __device__ __forceinline__ void grad_slot(const DistillK& a, char* out, const Sl
     }
   }
   if (before) return;  // an earlier slot of the same id writes it
-  double p = exp(((double)s.v[k] - g.log_hi) - g.log_lo);
+  const auto p_of = [&](float v) { return exp(((double)v - g.v0) - g.log_hi - g.log_lo); };
+  double p = p_of(s.v[k]);
   for (int j = k + 1; behind && j < a.k; j++)
-    if (s.id[j] == id) p += exp(((double)s.v[j] - g.log_hi) - g.log_lo);
+    if (s.id[j] == id) p += p_of(s.v[j]);
   const float e = __builtin_amdgcn_exp2f((s.z[k] - g.m) * a.c);
   store_one<DT>(out, id, (float)((double)scale * ((double)e * g.share - p)));
 }

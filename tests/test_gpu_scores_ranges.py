@@ -261,3 +261,30 @@ def test_distillation_with_rest_of_far_logits(hip, dtype, value, T):
             z = far(rng, rows, vocab, value, kind)
             ids = np.stack([rng.permutation(2048)[:9] for _ in range(rows)])  # ordinary logits
             check_rest(hip, z, ids, np.log(rng.dirichlet(np.ones(9), rows) * 0.8).astype(np.float32), T, dtype)
+
+
+# ---- lists far from normalised --------------------------------------------------------
+
+
+@pytest.mark.parametrize("shift", [0.0, 1e3, -1e4, -1e9, 1e12, float(np.finfo(np.float32).min)])
+@pytest.mark.parametrize("rows,vocab,k", [(3, 70003, 20), (130, 5003, 256), (131, 40003, 64)])
+def test_lists_of_any_size(hip, rows, vocab, k, shift):
+    """Without rest a list counts up to a shift: raw logits, or nothing but masks."""
+    rng = np.random.default_rng(39)
+    lg = Logits(hip, make(rng, rows, vocab), "f32")
+    ids, _ = make_teacher(rng, lg.z, k)
+    v = rng.normal(0, 1, (rows, k)).astype(np.float32)
+    if abs(shift) < 1e30:
+        v = v + np.float32(shift)
+        v[1] = np.float32(shift)
+    else:
+        v[::2] = shift     # every slot
+        v[1::2, ::3] = shift  # some
+    w = rng.uniform(0.1, 2, rows).astype(np.float32)
+    step, grad, alone, grad2 = run_distill(hip, lg, ids, v, 1.0, False, w)
+    for i in range(0, rows, 1 if rows < 10 else 43):
+        loss, tol, dz, dtol = rows64.distill(lg.z[i], ids[i], v[i], 1.0, False, float(w[i]), "f32")
+        dtol = dtol + lost_distill(1.0, w[i], dz)
+        near(step[i], loss, tol, f"loss of row {i}")
+        near(grad[i], dz, dtol, f"gradient of row {i} by the step")
+        near(grad2[i], dz, dtol, f"gradient of row {i} by the backward")
