@@ -8,7 +8,8 @@ dtl_distill* of include/detllm.h, which define every result) on the current
 stream of the logits' device, do not wait, and can be captured into a graph (a
 captured backward needs a leaf of its own, `logits.detach().requires_grad_()`: one
 whose eager graph is still alive belongs to that graph's stream).  Reverse mode only:
-tensors with a forward-mode tangent and torch.jit.trace are refused.
+tensors with a forward-mode tangent and torch.jit.trace are refused; in a function
+given to torch.compile they stand inside torch.compiler.disable.
 
     teacher = scores.token_scores(teacher_logits, tokens, top=32, temperature=2.0)
     loss = scores.distill_loss(student_logits, teacher.top_ids, teacher.top_log_probs,

@@ -119,3 +119,21 @@ def test_out_over_a_part_of_the_logits_is_refused():
     assert torch.equal(got, want) and torch.equal(wide[:3, 50:], want)
     scores.distill_loss_and_grad(wide[:3, :50], ids, v, out=wide[:3, :50])
     assert torch.equal(wide[:3, :50], want)
+
+
+@pytest.mark.gpu
+def test_inside_a_compiled_function():
+    z, ids, v = inputs(GPU)
+
+    @torch.compiler.disable
+    def calls_of_the_library(x):
+        return scores.token_scores(x, top=2).entropy.sum() + scores.distill_loss(x, ids, v, rest=True).sum()
+
+    def loss(x):
+        return calls_of_the_library(x * 2) + x.sum()
+
+    leaf = z.clone().requires_grad_()
+    want = loss(leaf)
+    got = torch.compile(loss, backend="eager")(leaf)
+    assert torch.equal(got, want)
+    assert torch.equal(torch.autograd.grad(got, leaf)[0], torch.autograd.grad(want, leaf)[0])
