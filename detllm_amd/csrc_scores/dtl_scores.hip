@@ -1328,8 +1328,8 @@ bool write_past(size_t rows, size_t row_bytes) { return rows * row_bytes > (size
 // hide behind: 4096 rows with 20 alternatives, four / eight waves: of 16000 f32 63 /
 // 87, of 32000 f32 104 / 131, of 49152 bf16 96 / 101, 100000 bf16 159 / 157; 400 rows of
 // 32000 bf16 17.7 / 15.8; with 128 alternatives the candidates' LDS leaves room for
-// too few (of 151936 bf16 360 / 269).  Without alternatives the same rule stands,
-// measured at neither.
+// too few (of 151936 bf16 360 / 269).  Calls without alternatives follow the same
+// rule; they were not measured.
 bool wide_rows(size_t rows, int nseg) { return rows <= 256 && nseg > 8; }
 
 template <typename F>
@@ -1480,9 +1480,9 @@ void launch_step_as(const DistillK& k, size_t rows, hipStream_t s) {
   launch_rows(k_distill_step<DT, REST, NS, LONGER, THREADS>, rows, 1, THREADS, REST ? (size_t)k.nseg * 256 : 0, s, k);
 }
 // A step of whole rows, by their length alone (the figures are of 2048 rows and
-// more; fewer were not compared).  Workgroups that hold only part of a long row leave room
-// for two or three of them a compute unit, one reading while another writes; us
-// by segments held a wave x waves:
+// more; fewer were not compared).  Workgroups that hold only part of a long row
+// leave room for two or three of them a compute unit, one reading while another
+// writes; us by segments held a wave x waves:
 //   4096 rows of 32000 bf16   2 x 8 (all) 109, 4 x 4 (all) 111, 1 x 16 (all) 175
 //   4096 rows of 49152 bf16   2 x 8 158, 3 x 8 (all) 158, 1 x 8 168, 2 x 16 225
 //   4096 rows of 151936 bf16  4 x 8 515, 3 x 8 523, 2 x 8 543, 1 x 8 562, 5 x 16 (all) 601

@@ -314,10 +314,10 @@ int dtl_token_scores(const dtl_logits *logits, const void *tokens, int token_byt
                      float *top_log_probs, void *scratch, size_t scratch_bytes, void *stream);
 /* The gradient of the logits (their type, row i at grad + i * grad_stride
  * elements; may be the logits themselves at the same stride, or lie between their
- * rows, but not over a part of them) for the gradients of log_probs and of entropy, either of which may be NULL.  stats and entropy
- * are the forward's.  Zero in rows whose gradients are zero (padding's is) or
- * whose logits are all masked, whatever else they hold; NaN in rows that gave
- * NaN. */
+ * rows, but not over a part of them) for the gradients of log_probs and of
+ * entropy, either of which may be NULL.  stats and entropy are the forward's.
+ * Zero in rows whose gradients are zero (padding's is) or whose logits are all
+ * masked, whatever else they hold; NaN in rows that gave NaN. */
 int dtl_token_scores_backward(const dtl_logits *logits, const void *tokens, int token_bytes,
                               float temperature, const float *stats, const float *entropy,
                               const float *grad_log_probs, const float *grad_entropy, void *grad,
@@ -349,8 +349,8 @@ int dtl_distill(const dtl_logits *logits, const dtl_teacher *teacher, float temp
                 float *stats, void *scratch, size_t scratch_bytes, void *stream);
 /* The gradient of the logits (as in dtl_token_scores_backward) for the gradient
  * of each row's loss; teacher (its rest too), temperature and stats are the
- * forward's.  Zero in rows whose gradient is zero, that have no slot in
- * use or whose logits are all masked. */
+ * forward's.  Zero in rows whose gradient is zero, that have no slot in use or
+ * whose logits are all masked. */
 int dtl_distill_backward(const dtl_logits *logits, const dtl_teacher *teacher, float temperature,
                          const float *stats, const float *grad_loss, void *grad, size_t grad_stride,
                          void *stream);
