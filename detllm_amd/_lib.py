@@ -94,6 +94,16 @@ class Teacher(C.Structure):
     _fields_ = [("ids", C.c_void_p), ("id_bytes", C.c_int), ("log_probs", C.c_void_p), ("k", sz), ("rest", C.c_int)]
 
 
+class Adjust(C.Structure):
+    """dtl_adjust: what is done to rows of logits."""
+
+    _fields_ = [("history", C.c_void_p), ("history_bytes", C.c_int), ("history_len", sz), ("history_stride", sz),
+                ("prompt", C.c_void_p), ("repetition", C.c_float), ("presence", C.c_float), ("frequency", C.c_float),
+                ("repetitions", C.c_void_p), ("presences", C.c_void_p), ("frequencies", C.c_void_p),
+                ("bias_ids", C.c_void_p), ("bias_bytes", C.c_int), ("biases", C.c_void_p), ("bias_len", sz),
+                ("bias_stride", sz), ("allowed", C.c_void_p), ("allowed_bits", C.c_int), ("allowed_stride", sz)]
+
+
 class KernelStat(C.Structure):
     _fields_ = [
         ("name", C.c_char * 32),
@@ -148,6 +158,9 @@ _SIGS = {
                                        C.c_void_p, sz, C.c_void_p]),
     "dtl_distill_step": (C.c_int, [C.POINTER(Logits), C.POINTER(Teacher), C.c_float, C.c_void_p, C.c_void_p, C.c_void_p,
                                    sz, C.c_void_p, sz, C.c_void_p]),
+    "dtl_adjust_logits": (C.c_int, [C.POINTER(Logits), C.POINTER(Adjust), C.c_void_p, sz, C.c_void_p]),
+    "dtl_adjust_logits_backward": (C.c_int, [C.POINTER(Logits), C.POINTER(Adjust), C.c_void_p, sz, C.c_void_p, sz,
+                                             C.c_void_p]),
     "dtl_session_token_scores": (C.c_int, [C.c_void_p, sz, sz, u32p, C.c_float, sz, f32p, f32p, C.POINTER(C.c_int32),
                                            f32p]),
     "dtl_range_encoder_new": (C.c_int, [vpp]),

@@ -1,0 +1,314 @@
+// Penalties for repeated tokens, biases and masks on rows of logits, and their
+// gradient.
+//
+//   a = z;  token in the history: a = z > 0 ? z / theta : z theta;  n times behind
+//   the prompt: a -= presence + frequency n;  a += bias;  not allowed: a = -inf.
+//   dz = g (theta^-1 or theta where the token stood, 0 where it is not allowed).
+//
+// Almost every logit is only copied or masked, so the row goes through registers
+// in 16-byte packets as it is, and the few tokens of the history and the biases
+// are written over it afterwards.  Bound by memory: one read and one write of the
+// logits (in place, only the masked ones are written), an eighth of a byte of mask.
+//
+// A workgroup has a segment of a row.  It counts the history's tokens there in a
+// table in LDS, one word a logit of the segment (a direct table needs no probing,
+// and integer sums have no order); whoever touches a word first puts its place on
+// a list, and a thread an entry patches the logits.  Each segment's workgroup scans
+// the whole history, from the caches.
+#include "dtl_scores.h"
+
+#include "dtl_rows.h"
+
+namespace dtl {
+namespace {
+
+constexpr int kThreads = 256;
+
+// A table word: 13 bits of the last bias's place + 1, whether the token stands in
+// the prompt, and how often behind it.
+constexpr uint32_t kPlaceMask = (1u << 13) - 1, kInPrompt = 1u << 13, kOnce = 1u << 14;
+static_assert(kAdjustMaxBiases <= kPlaceMask && kAdjustMaxHistory < 1 << 18, "fit a table word");
+
+enum { COPY, IN_PLACE, GRAD };
+
+struct AdjustK {
+  const char* z;
+  const char* from;  // what is copied: the logits, or the gradient
+  char* out;
+  size_t z_bytes, from_bytes, out_bytes, row0;
+  int V, nseg;
+  int history_len, bias_len;  // 0 where they change nothing
+  dtl_adjust by;
+  bool past;  // written past the caches
+};
+
+template <int DT>
+__device__ __forceinline__ uint32_t allowed_bits(const AdjustK& a, size_t row, int j, int n) {
+  // of logits j .. j + n, n at most a packet's: bit i for logit j + i
+  const char* p = static_cast<const char*>(a.by.allowed) + row * a.by.allowed_stride * (a.by.allowed_bits == 1 ? 4 : 1);
+  if (a.by.allowed_bits == 1) return (uint32_t)(uint8_t)p[j >> 3] >> (j & 7);
+  constexpr int all = Type<DT>::kInPacket;
+  if (n == all) {
+    typedef uint32_t word __attribute__((aligned(1)));
+    uint32_t m = (reinterpret_cast<const word*>(p + j)[0] & 0x01010101u) * 0x01020408u >> 24 & 15;
+    if (all == 8) m |= ((reinterpret_cast<const word*>(p + j)[1] & 0x01010101u) * 0x01020408u >> 24 & 15) << 4;
+    return m;
+  }
+  uint32_t m = 0;
+  for (int i = 0; i < n; i++) m |= (uint32_t)(p[j + i] & 1) << i;
+  return m;
+}
+
+// The packet with `no` in the places whose bit is not set.
+template <int DT>
+__device__ __forceinline__ packet blend(packet p, uint32_t bits, uint32_t no) {
+#pragma unroll
+  for (int d = 0; d < 4; d++) {
+    uint32_t keep;
+    if constexpr (DT == DTL_F32)
+      keep = (uint32_t)((int32_t)(bits << (31 - d)) >> 31);
+    else
+      keep = ((uint32_t)((int32_t)(bits << (31 - 2 * d)) >> 31) & 0xffffu) |
+             ((uint32_t)((int32_t)(bits << (30 - 2 * d)) >> 31) & 0xffff0000u);
+    p[d] = (p[d] & keep) | (no & ~keep);
+  }
+  return p;
+}
+
+__device__ __forceinline__ float of_row(const float* rows, float one, size_t row) { return rows ? rows[row] : one; }
+
+template <int DT, int MODE, bool TABLE, int SEG>
+__global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
+  typedef typename Type<DT>::mem mem;
+  constexpr int n = Type<DT>::kInPacket, np = SEG / (kThreads * n), kHistory = 8;
+  constexpr uint32_t no = MODE == GRAD ? 0u : Type<DT>::kMasked;
+  static_assert(np * kThreads * n == SEG, "whole packets");
+  __shared__ __attribute__((aligned(16))) uint32_t table[TABLE ? SEG : 4];
+  __shared__ uint16_t list[TABLE ? SEG : 1];
+  __shared__ uint32_t listed;
+  const int tid = threadIdx.x;
+  const size_t row = a.row0 + blockIdx.x / a.nseg;
+  const int base = (int)(blockIdx.x % a.nseg) * SEG, end = min(a.V, base + SEG);
+  const char* from = a.from + row * a.from_bytes;
+  char* out = a.out + row * a.out_bytes;
+
+  // the history's first ids, then the segment: their loads run together
+  long ids[kHistory];
+  const size_t hrow = row * a.by.history_stride;
+  if (TABLE) {
+#pragma unroll
+    for (int i = 0; i < kHistory; i++) {
+      const int at = tid + i * kThreads;
+      ids[i] = at < a.history_len ? load_index(a.by.history, a.by.history_bytes == 8, hrow + at) : -1;
+    }
+  }
+  const bool masked = a.by.allowed != nullptr;
+  packet p[np];
+  uint32_t bits[np];
+#pragma unroll
+  for (int i = 0; i < np; i++) {
+    const int j = base + (i * kThreads + tid) * n;
+    bits[i] = ~0u;
+    if (j < end) {
+      if (masked) bits[i] = allowed_bits<DT>(a, row, j, min(n, end - j));
+      if (MODE != IN_PLACE) p[i] = load_packet<DT>(from, j, end);
+    }
+  }
+  if (TABLE) {
+    if (tid == 0) listed = 0;
+    for (int i = tid * 4; i < SEG; i += kThreads * 4) *reinterpret_cast<packet*>(table + i) = packet{0, 0, 0, 0};
+    __syncthreads();
+    auto touched = [&](uint32_t j, uint32_t before) {
+      if (before == 0) list[atomicAdd(&listed, 1u)] = (uint16_t)j;
+    };
+    if (a.bias_len) {
+      for (int k = tid; k < a.bias_len; k += kThreads) {
+        const long id = load_index(a.by.bias_ids, a.by.bias_bytes == 8, row * a.by.bias_stride + k);
+        const uint64_t j = (uint64_t)(id - base);
+        if (j < (uint64_t)(end - base)) touched((uint32_t)j, atomicMax(table + j, (uint32_t)k + 1));
+      }
+      __syncthreads();
+    }
+    if (a.history_len) {
+      const int prompt = a.by.prompt ? a.by.prompt[row] : 0;
+      auto count = [&](long id, int at) {
+        const uint64_t j = (uint64_t)(id - base);
+        if (j < (uint64_t)(end - base))
+          touched((uint32_t)j, at < prompt ? atomicOr(table + j, kInPrompt) : atomicAdd(table + j, kOnce));
+      };
+#pragma unroll
+      for (int i = 0; i < kHistory; i++) count(ids[i], tid + i * kThreads);
+      for (int at = tid + kHistory * kThreads; at < a.history_len; at += kThreads)
+        count(load_index(a.by.history, a.by.history_bytes == 8, hrow + at), at);
+    }
+  }
+
+#pragma unroll
+  for (int i = 0; i < np; i++) {
+    const int j = base + (i * kThreads + tid) * n;
+    if (j >= end) continue;
+    const int here = min(n, end - j);
+    const uint32_t all = (1u << here) - 1, on = bits[i] & all;
+    if (MODE == IN_PLACE) {
+      if (on == all) continue;
+      p[i] = on ? load_packet<DT>(from, j, end) : packet{no, no, no, no};
+    }
+    const packet w = blend<DT>(p[i], bits[i], no);
+    if (here == n) {
+      mem* to = reinterpret_cast<mem*>(out + (size_t)j * Type<DT>::kBytes);
+      if (a.past)
+        __builtin_nontemporal_store(w, to);
+      else
+        *to = w;
+    } else {
+#pragma unroll
+      for (int q = 0; q < n; q++)
+        if (q < here) {
+          if constexpr (DT == DTL_F32)
+            reinterpret_cast<uint32_t*>(out)[j + q] = w[q];
+          else
+            reinterpret_cast<uint16_t*>(out)[j + q] = (uint16_t)(w[q / 2] >> (q & 1 ? 16 : 0));
+        }
+    }
+  }
+  if (!TABLE) return;
+
+  wait_for_stores();
+  const float theta = of_row(a.by.repetitions, a.by.repetition, row);
+  const float presence = of_row(a.by.presences, a.by.presence, row);
+  const float frequency = of_row(a.by.frequencies, a.by.frequency, row);
+  for (uint32_t i = tid; i < listed; i += kThreads) {
+    const int at = list[i], j = base + at;
+    const uint32_t w = table[at], times = w / kOnce;
+    if (masked && !(allowed_bits<DT>(a, row, j, 1) & 1)) continue;
+    // the source is as it was: in place, only masked logits were written
+    const float z = load_one<DT>(a.z + row * a.z_bytes, j);
+    if (MODE == GRAD) {
+      const float g = load_one<DT>(from, j);
+      store_one<DT>(out, j, z > 0.0f ? g / theta : g * theta);
+      continue;
+    }
+    float v = z;
+    if (w > kPlaceMask) v = z > 0.0f ? z / theta : z * theta;
+    if (times) v -= presence + frequency * (float)times;
+    if (w & kPlaceMask) v += a.by.biases[row * a.by.bias_stride + (w & kPlaceMask) - 1];
+    store_one<DT>(out, j, v);
+  }
+}
+
+template <int DT, int MODE, int SEG>
+void launch_as(AdjustK& k, size_t rows, bool table, hipStream_t s) {
+  k.nseg = (k.V + SEG - 1) / SEG;
+  launch_rows(table ? k_adjust<DT, MODE, true, SEG> : k_adjust<DT, MODE, false, SEG>, rows, k.nseg, kThreads, 0, s, k);
+}
+
+}  // namespace
+
+int check_adjust(const dtl_adjust* by, size_t rows, size_t vocab) {
+  if (!by) return DTL_ERR_INVALID_ARGUMENT;
+  if (rows && by->history_len && !by->history) return DTL_ERR_INVALID_ARGUMENT;
+  if (rows && by->bias_len && (!by->bias_ids || !by->biases)) return DTL_ERR_INVALID_ARGUMENT;
+  if (by->history_len) {
+    if (!index_bytes_ok(by->history_bytes)) return DTL_ERR_INVALID_ARGUMENT;
+    if (by->history_len > (size_t)kAdjustMaxHistory || by->history_stride > ((size_t)1 << 40)) return DTL_ERR_SHAPE;
+    if (!by->repetitions && !(by->repetition > 0.0f && by->repetition < __builtin_inff())) return DTL_ERR_INVALID_ARGUMENT;
+    if (!by->presences && !(by->presence - by->presence == 0.0f)) return DTL_ERR_INVALID_ARGUMENT;
+    if (!by->frequencies && !(by->frequency - by->frequency == 0.0f)) return DTL_ERR_INVALID_ARGUMENT;
+  }
+  if (by->bias_len) {
+    if (!index_bytes_ok(by->bias_bytes)) return DTL_ERR_INVALID_ARGUMENT;
+    if (by->bias_len > (size_t)kAdjustMaxBiases || by->bias_stride > ((size_t)1 << 40)) return DTL_ERR_SHAPE;
+  }
+  if (by->allowed) {
+    if (by->allowed_bits != 1 && by->allowed_bits != 8) return DTL_ERR_INVALID_ARGUMENT;
+    const size_t row = by->allowed_bits == 1 ? (vocab + 31) / 32 : vocab;
+    if (rows > 1 && by->allowed_stride && by->allowed_stride < row) return DTL_ERR_SHAPE;
+    if (by->allowed_stride > ((size_t)1 << 40)) return DTL_ERR_SHAPE;
+    if (by->allowed_bits == 1 && reinterpret_cast<uintptr_t>(by->allowed) % 4) return DTL_ERR_INVALID_ARGUMENT;
+  }
+  return DTL_OK;
+}
+
+void launch_adjust(const AdjustArgs& a, hipStream_t s) {
+  if (a.rows == 0) return;
+  const size_t e = type_bytes(a.dtype);
+  AdjustK k{};
+  k.z = static_cast<const char*>(a.z);
+  k.from = static_cast<const char*>(a.grad ? a.grad : a.z);
+  k.out = static_cast<char*>(a.out);
+  k.z_bytes = a.stride * e;
+  k.from_bytes = (a.grad ? a.grad_stride : a.stride) * e;
+  k.out_bytes = a.out_stride * e;
+  k.V = a.vocab;
+  k.by = a.by;
+  const bool repeats = a.by.repetitions || a.by.repetition != 1.0f;
+  const bool counts = a.by.presences || a.by.frequencies || a.by.presence != 0.0f || a.by.frequency != 0.0f;
+  if (a.by.history && (repeats || (counts && !a.grad))) k.history_len = (int)a.by.history_len;
+  if (a.by.bias_ids && !a.grad) k.bias_len = (int)a.by.bias_len;
+  const bool table = k.history_len || k.bias_len, same = k.from == k.out;
+  if (same && !table && !a.by.allowed) return;
+  by_type(a.dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (a.grad)
+      launch_as<DT, GRAD, 8192>(k, a.rows, table, s);
+    else if (same)
+      launch_as<DT, IN_PLACE, 8192>(k, a.rows, table, s);
+    else
+      launch_as<DT, COPY, 8192>(k, a.rows, table, s);
+  });
+}
+
+}  // namespace dtl
+
+// ---- C entry points ------------------------------------------------------------------------
+
+using namespace dtl;
+
+namespace {
+AdjustArgs adjust_args(const dtl_logits* z, const dtl_adjust* by, void* out, size_t out_stride) {
+  AdjustArgs a{};
+  a.z = z->data;
+  a.stride = z->stride;
+  a.rows = z->rows;
+  a.dtype = z->dtype;
+  a.vocab = (int)z->vocab;
+  a.by = *by;
+  a.out = out;
+  a.out_stride = out_stride;
+  return a;
+}
+}  // namespace
+
+extern "C" {
+
+int dtl_adjust_logits(const dtl_logits* z, const dtl_adjust* by, void* out, size_t out_stride, void* stream) {
+  int st = check_logits(z);
+  if (!st) st = check_adjust(by, z->rows, z->vocab);
+  if (!st) st = check_grad(z, out, out_stride);
+  if (st || z->rows == 0) return st;
+  launch_adjust(adjust_args(z, by, out, out_stride), static_cast<hipStream_t>(stream));
+  return launch_status();
+}
+
+int dtl_adjust_logits_backward(const dtl_logits* z, const dtl_adjust* by, const void* grad_out, size_t grad_out_stride,
+                               void* grad, size_t grad_stride, void* stream) {
+  int st = check_logits(z);
+  if (!st) st = check_adjust(by, z->rows, z->vocab);
+  if (st) return st;
+  dtl_logits g = *z;
+  g.data = grad_out;
+  g.stride = grad_out_stride;
+  st = check_logits(&g);
+  if (!st) st = check_grad(&g, grad, grad_stride);
+  if (!st) st = check_grad(z, grad, grad_stride);
+  if (st || z->rows == 0) return st;
+  // a logit's sign is read after its gradient is written
+  if (grad == z->data) return DTL_ERR_INVALID_ARGUMENT;
+  AdjustArgs a = adjust_args(z, by, grad, grad_stride);
+  a.grad = grad_out;
+  a.grad_stride = grad_out_stride;
+  launch_adjust(a, static_cast<hipStream_t>(stream));
+  return launch_status();
+}
+
+}  // extern "C"

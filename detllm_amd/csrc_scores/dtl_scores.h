@@ -21,6 +21,8 @@ constexpr int kScoreMaxSegs = kScoreMaxVocab / kScoreSeg;
 constexpr int kScoreMaxTop = 128;
 constexpr int kDistillMaxK = 256;
 constexpr int kDistillStats = 5;
+constexpr int kAdjustMaxHistory = 1 << 17;
+constexpr int kAdjustMaxBiases = 4096;
 constexpr float kScoreMinTemperature = 1e-4f, kScoreMaxTemperature = 1e4f;
 
 struct ScoreArgs {
@@ -80,5 +82,20 @@ struct DistillArgs {
 size_t distill_scratch_bytes(size_t rows, size_t vocab, bool step);
 void launch_distill(const DistillArgs& a, hipStream_t s);
 void launch_distill_grad(const DistillArgs& a, hipStream_t s);
+
+// dtl_adjust_logits: `grad` null; dtl_adjust_logits_backward: from `grad` to `out`.
+struct AdjustArgs {
+  const void* z;
+  size_t stride;
+  size_t rows;
+  int dtype, vocab;
+  dtl_adjust by;
+  const void* grad;
+  size_t grad_stride;
+  void* out;
+  size_t out_stride;
+};
+int check_adjust(const dtl_adjust* by, size_t rows, size_t vocab);
+void launch_adjust(const AdjustArgs& a, hipStream_t s);
 
 }  // namespace dtl

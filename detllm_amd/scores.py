@@ -1,11 +1,13 @@
-"""Scores of given tokens and distillation on logits held in torch tensors.
+"""Scores of given tokens, distillation, and penalties and masks on logits held in
+torch tensors.
 
 For programs that have a model's logits on the GPU as a torch tensor: what the
-rows say of given tokens (log probability, entropy, top alternatives), and the
-loss that moves a student towards a teacher's top alternatives, both with
+rows say of given tokens (log probability, entropy, top alternatives), the
+loss that moves a student towards a teacher's top alternatives, and what is done
+to the rows before either (penalties for repeated tokens, biases, masks), all with
 gradients.  The calls enqueue the library's kernels (dtl_token_scores*,
-dtl_distill* of include/detllm.h, which define every result) on the current
-stream of the logits' device, do not wait, and can be captured into a graph (a
+dtl_distill*, dtl_adjust_logits* of include/detllm.h, which define every result) on
+the current stream of the logits' device, do not wait, and can be captured into a graph (a
 captured backward needs a leaf of its own, `logits.detach().requires_grad_()`: one
 whose eager graph is still alive belongs to that graph's stream).  Reverse mode only:
 tensors with a forward-mode tangent and torch.jit.trace are refused; in a function
@@ -23,7 +25,7 @@ from __future__ import annotations
 
 import ctypes as C
 from functools import lru_cache
-from typing import NamedTuple, Optional, Tuple
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 from torch.autograd import forward_ad
@@ -313,3 +315,148 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
     if given:  # autograd is told that it was written
         torch.autograd.graph.increment_version(out)
     return loss, out
+
+
+# ---- penalties, biases, masks -------------------------------------------------------
+
+
+def _per_row(value, logits, name):
+    """A number, or a tensor with one for each row."""
+    if isinstance(value, torch.Tensor):
+        if value.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} is a constant to autograd: detach it")
+        return 0.0, _beside(value, logits, logits.shape[:-1], _FLOAT, name)
+    return float(value), None
+
+
+def _rows_or_shared(t, logits, last, dtypes, name):
+    """A tensor of the logits' leading dimensions, or of one dimension for every row."""
+    shared = isinstance(t, torch.Tensor) and t.dim() == 1
+    return _beside(t, logits, (last,) if shared else (*logits.shape[:-1], last), dtypes, name), 0 if shared else last
+
+
+def _last(t) -> int:
+    return t.shape[-1] if isinstance(t, torch.Tensor) and t.dim() else 0
+
+
+class _By:
+    """A dtl_adjust and the tensors that it points to."""
+
+    def __init__(self, logits, vocab, history, prompt, repetition, presence, frequency, bias_ids, bias, allowed):
+        a = self.struct = _lib.Adjust()
+        lead = logits.shape[:-1]
+        rows = None
+        if history is not None:
+            history, a.history_stride = _rows_or_shared(history, logits, _last(history), _INDEX, "history")
+            a.history, a.history_bytes, a.history_len = history.data_ptr(), history.element_size(), history.shape[-1]
+            if prompt is not None:
+                prompt = _beside(prompt, logits, lead, _INDEX, "prompt").int()
+                a.prompt = prompt.data_ptr()
+        elif prompt is not None:
+            raise ValueError("prompt counts places of a history")
+        a.repetition, rows = _per_row(repetition, logits, "repetition")
+        a.presence, presences = _per_row(presence, logits, "presence")
+        a.frequency, frequencies = _per_row(frequency, logits, "frequency")
+        a.repetitions, a.presences, a.frequencies = _ptr(rows), _ptr(presences), _ptr(frequencies)
+        if (bias_ids is None) != (bias is None):
+            raise ValueError("bias_ids and bias belong together")
+        if bias is not None:
+            if isinstance(bias, torch.Tensor) and bias.requires_grad and torch.is_grad_enabled():
+                raise ValueError("bias is a constant to autograd: detach it")
+            n = _last(bias_ids)
+            bias_ids, a.bias_stride = _rows_or_shared(bias_ids, logits, n, _INDEX, "bias_ids")
+            bias = _beside(bias, logits, bias_ids.shape, _FLOAT, "bias")
+            a.bias_ids, a.bias_bytes, a.bias_len = bias_ids.data_ptr(), bias_ids.element_size(), n
+            a.biases = bias.data_ptr()
+        if allowed is not None:
+            bits = isinstance(allowed, torch.Tensor) and allowed.dtype == torch.int32
+            allowed, a.allowed_stride = _rows_or_shared(allowed, logits, -(-vocab // 32) if bits else vocab,
+                                                        (torch.int32, torch.bool), "allowed")
+            a.allowed, a.allowed_bits = allowed.data_ptr(), 1 if bits else 8
+        self.tensors = (history, prompt, rows, presences, frequencies, bias_ids, bias, allowed)
+
+    def for_backward(self):
+        """What the gradient needs: whether a token stood in the history, and the mask."""
+        history, prompt, rows, _, _, _, _, allowed = self.tensors
+        if self.struct.repetition == 1.0 and rows is None:
+            history = None
+        return history, rows if history is not None else None, allowed
+
+
+def _adjust(z, by, out, stride, device):
+    _call(device, lib.dtl_adjust_logits, C.byref(z), C.byref(by.struct), out.data_ptr(), stride)
+
+
+class _Adjust(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, by):
+        z = _logits_view(logits)
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        _adjust(z, by, out, z.vocab, logits.device)
+        history, rows, allowed = by.for_backward()
+        # without repetitions a logit's sign does not matter, only where it is
+        ctx.save_for_backward(logits if history is not None else None, history, rows, allowed)
+        ctx.like = logits.shape, logits.dtype, logits.device
+        ctx.repetition = by.struct.repetition
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        logits, history, rows, allowed = ctx.saved_tensors
+        shape, dtype, device = ctx.like
+        g = _incoming(g)
+        if history is None and allowed is None:
+            return g, None
+        grad = torch.empty(shape, dtype=dtype, device=device)
+        a = _lib.Adjust(repetition=ctx.repetition, repetitions=_ptr(rows))
+        if history is not None:
+            a.history, a.history_bytes, a.history_len = history.data_ptr(), history.element_size(), history.shape[-1]
+            a.history_stride = history.shape[-1] if history.dim() > 1 or len(shape) == 1 else 0
+        if allowed is not None:
+            a.allowed, a.allowed_bits = allowed.data_ptr(), 1 if allowed.dtype == torch.int32 else 8
+            a.allowed_stride = allowed.shape[-1] if allowed.dim() > 1 or len(shape) == 1 else 0
+        V = shape[-1]
+        gv = _lib.Logits(g.data_ptr(), _DTYPES[dtype], g.numel() // V, V, V)
+        z = gv if logits is None else _logits_view(logits)
+        _call(device, lib.dtl_adjust_logits_backward, C.byref(z), C.byref(a), gv.data, V, grad.data_ptr(), V)
+        return grad, None
+
+
+def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None, prompt: Optional[torch.Tensor] = None,
+                  repetition: Union[float, torch.Tensor] = 1.0, presence: Union[float, torch.Tensor] = 0.0,
+                  frequency: Union[float, torch.Tensor] = 0.0, bias_ids: Optional[torch.Tensor] = None,
+                  bias: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dtl_adjust_logits of logits[..., vocab]: what is done to rows before they are
+    scored, drawn from or trained on; differentiable in the logits.
+
+    history[..., n] or [n] (int64 or int32; -1 is no token): a token in it is
+    divided by `repetition` (multiplied, where its logit is negative), and loses
+    presence + frequency * its count.  The first prompt[...] places are a prompt,
+    which counts for the repetition alone.  The three are numbers, or float32 tensors
+    with one for each row.  bias_ids and bias[..., k] or [k]: what is added to listed
+    tokens (of an id listed twice the later place).  allowed: int32 words of
+    32 bits [..., ceil(vocab / 32)], or bool [..., vocab], or of one row for all;
+    what it does not allow becomes -inf.
+
+    out: where the result goes, of the logits' shape and type; the logits themselves,
+    whose unchanged places are then not written.  It has no gradient."""
+    _need_logits(logits)
+    z = _logits_view(logits)
+    by = _By(logits, z.vocab, history, prompt, repetition, presence, frequency, bias_ids, bias, allowed)
+    grad = torch.is_grad_enabled() and logits.requires_grad
+    if out is None:
+        if grad:
+            return _Adjust.apply(logits, by)
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        _adjust(z, by, out, z.vocab, logits.device)
+        return out
+    if grad or out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out has no gradient: leave it out, or call under torch.no_grad()")
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise ValueError("out must have the shape, type and device of logits")
+    _no_tangent(out, "out")
+    _adjust(z, by, out, _logits_view(out, "out").stride, logits.device)
+    torch.autograd.graph.increment_version(out)  # autograd is told that it was written
+    return out

@@ -363,6 +363,56 @@ int dtl_distill_step(const dtl_logits *logits, const dtl_teacher *teacher, float
                      const float *weights, float *loss, void *grad, size_t grad_stride, void *scratch,
                      size_t scratch_bytes, void *stream);
 
+/* ---- rows of logits before they are scored, drawn from or trained on -------
+ * No counterpart in the reference.  Conventions as for the scores above. */
+
+/* What is done to row i of logits[rows][vocab], in this order; a part whose
+ * pointer is NULL (or whose length is 0) is left out:
+ *   history  history_len ids (at most 2^17; history_bytes 4 or 8), row i at
+ *            history + i * history_stride ids (0: every row's); an id below 0 or
+ *            >= vocab is no token.  The places before prompt[i] (NULL: 0) are the
+ *            prompt's.  A token anywhere in it: z > 0 ? z / repetition :
+ *            z * repetition.  One that stands n > 0 times behind the prompt: less
+ *            presence + frequency * n.  repetitions, presences, frequencies
+ *            ([rows] each, or NULL) are taken in place of the single values.
+ *   biases   bias_len (at most 4096) ids and what is added to their logits, row i
+ *            at bias_ids + i * bias_stride and biases + i * bias_stride (0: every
+ *            row's).  Of an id that occurs twice the later place counts; an id
+ *            below 0 or >= vocab is an empty place.
+ *   allowed  a logit that is not allowed becomes -inf, whatever it was.
+ *            allowed_bits 1: bit j % 32 of the row's 32-bit word j / 32; 8: byte j
+ *            (0 or 1).  Row i at allowed + i * allowed_stride words or bytes (0:
+ *            every row's). */
+typedef struct dtl_adjust {
+    const void *history;
+    int history_bytes;
+    size_t history_len, history_stride;
+    const int32_t *prompt;
+    float repetition, presence, frequency; /* repetition > 0; 1, 0, 0 change nothing */
+    const float *repetitions, *presences, *frequencies;
+    const void *bias_ids;
+    int bias_bytes;
+    const float *biases;
+    size_t bias_len, bias_stride;
+    const void *allowed;
+    int allowed_bits;
+    size_t allowed_stride;
+} dtl_adjust;
+
+/* Writes the adjusted logits (their type, row i at out + i * out_stride elements;
+ * may be the logits themselves at the same stride, or lie between their rows, but
+ * not over a part of them).  Formed in 32 bits and rounded once; what passes a
+ * range there is infinite (the lowest float times a repetition, say). */
+int dtl_adjust_logits(const dtl_logits *logits, const dtl_adjust *by, void *out, size_t out_stride,
+                      void *stream);
+/* From the gradient of the adjusted logits (their type and shape, row i at
+ * grad_out + i * grad_out_stride) that of the logits: times 1 / repetition or
+ * repetition where a token stood in the history, 0 where a logit is not allowed,
+ * whatever grad_out holds there.  grad may be grad_out itself at the same stride,
+ * but lie over no part of the logits. */
+int dtl_adjust_logits_backward(const dtl_logits *logits, const dtl_adjust *by, const void *grad_out,
+                               size_t grad_out_stride, void *grad, size_t grad_stride, void *stream);
+
 /* logits_to_cdf / logits_to_symbol_range on caller logits (host memory):
  * uploads them and runs the same device kernels (cdf.rs:47-199). */
 int dtl_logits_to_cdf(const float *logits, size_t n, size_t tail_symbols, uint32_t *freq,
