@@ -104,6 +104,12 @@ class Adjust(C.Structure):
                 ("bias_stride", sz), ("allowed", C.c_void_p), ("allowed_bits", C.c_int), ("allowed_stride", sz)]
 
 
+class Table(C.Structure):
+    """dtl_table: rows of embeddings or of their gradient in device memory."""
+
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int), ("vocab", sz), ("width", sz), ("stride", sz)]
+
+
 class KernelStat(C.Structure):
     _fields_ = [
         ("name", C.c_char * 32),
@@ -161,6 +167,10 @@ _SIGS = {
     "dtl_adjust_logits": (C.c_int, [C.POINTER(Logits), C.POINTER(Adjust), C.c_void_p, sz, C.c_void_p]),
     "dtl_adjust_logits_backward": (C.c_int, [C.POINTER(Logits), C.POINTER(Adjust), C.c_void_p, sz, C.c_void_p, sz,
                                              C.c_void_p]),
+    "dtl_embedding": (C.c_int, [C.POINTER(Table), C.c_void_p, C.c_int, sz, C.c_float, C.c_void_p, sz, C.c_void_p]),
+    "dtl_embedding_backward_scratch": (sz, [sz, sz, sz]),
+    "dtl_embedding_backward": (C.c_int, [C.c_void_p, C.c_int, sz, C.c_void_p, C.c_int, sz, C.c_float, C.POINTER(Table),
+                                         C.c_int, C.c_void_p, sz, C.c_void_p]),
     "dtl_session_token_scores": (C.c_int, [C.c_void_p, sz, sz, u32p, C.c_float, sz, f32p, f32p, C.POINTER(C.c_int32),
                                            f32p]),
     "dtl_range_encoder_new": (C.c_int, [vpp]),

@@ -1,0 +1,619 @@
+// Embedding lookup with scaling, and the table's gradient from positions sorted by
+// token.
+//
+//   out[i] = s W[t_i];   dW[v] = s sum over t_i = v of g_i
+//
+// The gradient is bound by memory: the rows g are read once, the table is written
+// once, zeros for nearly all of it.  Adding rows with atomics would write in an order
+// of its own; here the positions are sorted by token instead (a stable radix sort of
+// two 9-bit digits, so that a token's positions keep their order), and threads sum
+// along fixed stretches of the sorted list.  A token's rows that cross a stretch's
+// end are left as partial sums, which a last launch joins.  The zeros are written
+// beside the sort, whose few workgroups wait on each other anyway.
+#include "dtl_scores.h"
+
+#include "dtl_rows.h"
+
+namespace dtl {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
+constexpr int kRounds = 8;                      // most tokens a thread of the sort has
+constexpr int kTiles = 128;                     // most workgroups of the sort
+constexpr int kPlaceBits = 13;
+constexpr int kAlone = 4096;                    // tokens that one workgroup sorts in LDS
+constexpr int kFillBytes = kSortThreads * 16 * 4;  // zeros a workgroup writes
+static_assert(kScoreMaxVocab == 1 << (2 * kDigitBits), "two digits hold a token");
+static_assert((size_t)kTiles * kRounds * kSortThreads == kEmbedMaxTokens, "the sort's workgroups hold every token");
+static_assert(kAlone <= 1 << kPlaceBits && 2 * kDigitBits + kPlaceBits <= 32, "a token and its place fit a word");
+static_assert(kAlone <= kRounds * kSortThreads, "one workgroup holds them");
+
+// ---- lookup -----------------------------------------------------------------------
+
+struct LookupK {
+  const char* table;
+  char* out;
+  const void* tokens;
+  size_t row0, n, table_bytes, out_bytes;
+  int V, D, packets, wide;
+  float scale;
+};
+
+// A thread a packet of an output row.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void k_embedding(LookupK a) {
+  typedef typename Type<DT>::mem mem;
+  constexpr int n = Type<DT>::kInPacket;
+  const uint32_t at = blockIdx.x * kThreads + threadIdx.x, r = at / (uint32_t)a.packets;
+  const int j = (int)(at - r * (uint32_t)a.packets) * n;
+  const size_t i = a.row0 + r;
+  if (i >= a.n) return;
+  const long t = load_index(a.tokens, a.wide, i);
+  char* out = a.out + i * a.out_bytes;
+  packet p{0, 0, 0, 0};
+  float v[n];
+  const bool real = t >= 0 && t < a.V;
+  if (real) p = load_packet<DT>(a.table + (size_t)t * a.table_bytes, j, a.D);
+  const float nan = __builtin_nanf("");
+#pragma unroll
+  for (int q = 0; q < n; q++) v[q] = t >= a.V ? nan : real ? value<DT>(p, q) * a.scale : 0.0f;
+  if (j + n <= a.D) {
+    packet w = p;
+    if (t >= a.V || a.scale != 1.0f) {
+#pragma unroll
+      for (int q = 0; q < 4; q++)
+        w[q] = DT == DTL_F32 ? bits_of<DT>(v[q % n]) : bits_of<DT>(v[2 * q % n]) | bits_of<DT>(v[(2 * q + 1) % n]) << 16;
+    }
+    *reinterpret_cast<mem*>(out + (size_t)j * Type<DT>::kBytes) = w;
+  } else {
+#pragma unroll
+    for (int q = 0; q < n; q++)
+      if (j + q < a.D) store_one<DT>(out, j + q, v[q]);
+  }
+}
+
+// ---- the sort ------------------------------------------------------------------------
+
+struct SortK {
+  const void* tokens;
+  int wide, V;
+  uint32_t n;       // tokens, those that are none among them
+  uint32_t tile;    // a workgroup's
+  int tiles;        // workgroups that sort; those behind them write zeros
+  uint32_t* count;  // real tokens
+  uint32_t* hist;   // [tiles][kDigits]
+  uint32_t *key0, *place0, *key1, *place1;  // after the first and the second digit
+  // zeros: rows of `fill_bytes`, of which this launch's workgroups write pieces from `piece0` on
+  char* fill;
+  size_t fill_rows, fill_bytes, fill_stride, piece0, pieces;
+};
+
+// 16 bytes a thread and step; a row's last bytes are at least an element's.
+__device__ __forceinline__ void fill_piece(const SortK& a, size_t piece) {
+  if (piece >= a.pieces) return;
+  const size_t per_row = (a.fill_bytes + 15) / 16;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    size_t at = piece * (kFillBytes / 16) + i * kSortThreads + threadIdx.x, row = 0;
+    if (a.fill_rows > 1) {
+      row = at / per_row;
+      at -= row * per_row;
+    }
+    if (row >= a.fill_rows || at >= per_row) continue;
+    char* p = a.fill + row * a.fill_stride + at * 16;
+    const size_t left = a.fill_bytes - at * 16;
+    if (left >= 16)
+      *reinterpret_cast<packet2*>(p) = packet{0, 0, 0, 0};
+    else
+      for (size_t b = 0; b < left; b += 2) *reinterpret_cast<uint16_t*>(p + b) = 0;
+  }
+}
+
+struct RankLds {
+  uint32_t count[kSortWaves][kDigits];
+  uint32_t wave_sum[kDigits / 64];
+};
+
+// The lanes of this wave with the same digit, `on` among them.
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool on) {
+  uint64_t m = __ballot(on);
+#pragma unroll
+  for (int b = 0; b < kDigitBits; b++) {
+    const uint64_t set = __ballot(digit >> b & 1);
+    m &= digit >> b & 1 ? set : ~set;
+  }
+  return m;
+}
+
+// How many of the wave's earlier items have this one's digit; counts it.
+__device__ __forceinline__ uint32_t rank_in_wave(RankLds& s, int wave, int lane, uint32_t digit, bool on) {
+  const uint64_t m = same_digit(digit, on);
+  const int first = m ? __builtin_ctzll(m) : 0;
+  uint32_t before = 0;
+  if (on && lane == first) before = atomicAdd(&s.count[wave][digit], (uint32_t)__builtin_popcountll(m));
+  before = (uint32_t)__shfl((int)before, first);
+  return before + (uint32_t)__builtin_popcountll(m & ((1ull << lane) - 1));
+}
+
+// For thread d < kDigits: the sum of `mine` over the digits before d.  All threads call it.
+__device__ __forceinline__ uint32_t scan_digits(RankLds& s, uint32_t mine, uint32_t* total) {
+  const int tid = threadIdx.x, wave = tid >> 6;
+  const uint32_t up_to = wave_scan(tid < kDigits ? mine : 0);
+  if (tid < kDigits && (tid & 63) == 63) s.wave_sum[wave] = up_to;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kDigits / 64; w++) {
+    if (w < wave) before += s.wave_sum[w];
+    all += s.wave_sum[w];
+  }
+  *total = all;
+  return before + up_to - mine;
+}
+
+// After the waves' counts: count[w][d] becomes the place of wave w's first item of
+// digit d, the digits in order from `base` (a thread a digit) on.
+__device__ __forceinline__ void place_waves(RankLds& s, uint32_t base) {
+  const int d = threadIdx.x;
+  if (d < kDigits) {
+#pragma unroll
+    for (int w = 0; w < kSortWaves; w++) {
+      const uint32_t c = s.count[w][d];
+      s.count[w][d] = base;
+      base += c;
+    }
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ void clear_counts(RankLds& s) {
+  for (int i = threadIdx.x; i < kSortWaves * kDigits; i += kSortThreads) (&s.count[0][0])[i] = 0;
+  __syncthreads();
+}
+__device__ __forceinline__ uint32_t wave_total(const RankLds& s) {
+  uint32_t sum = 0;
+  if (threadIdx.x < kDigits)
+    for (int w = 0; w < kSortWaves; w++) sum += s.count[w][threadIdx.x];
+  return sum;
+}
+
+// Up to kAlone tokens by one workgroup, both digits in LDS; the others write zeros.
+__global__ __launch_bounds__(kSortThreads) void k_sort_alone(SortK a) {
+  __shared__ RankLds s;
+  __shared__ uint32_t item[kAlone];
+  if (blockIdx.x > 0) return fill_piece(a, a.piece0 + blockIdx.x - 1);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int rounds = kAlone / kSortThreads;
+  const uint32_t per_wave = 64 * ((a.n + kSortThreads - 1) / kSortThreads);
+  uint32_t mine[rounds], rank[rounds], all = a.n;
+#pragma unroll
+  for (int pass = 0; pass < 2; pass++) {
+    clear_counts(s);
+#pragma unroll
+    for (int r = 0; r < rounds; r++) {
+      const uint32_t at = wave * per_wave + r * 64 + lane;
+      const bool in = (uint32_t)r * 64 < per_wave && at < all;
+      bool on = in;
+      if (pass == 0) {
+        const long t = in ? load_index(a.tokens, a.wide, at) : -1;
+        on = t >= 0 && t < a.V;
+        mine[r] = (uint32_t)t << kPlaceBits | at;
+      } else if (in) {
+        mine[r] = item[at];
+      }
+      const uint32_t digit = mine[r] >> (kPlaceBits + pass * kDigitBits) & (kDigits - 1);
+      rank[r] = rank_in_wave(s, wave, lane, digit, on);
+      if (!on) rank[r] = ~0u;
+    }
+    __syncthreads();
+    uint32_t total;
+    const uint32_t base = scan_digits(s, wave_total(s), &total);
+    place_waves(s, base);
+#pragma unroll
+    for (int r = 0; r < rounds; r++) {
+      if (rank[r] == ~0u) continue;
+      const uint32_t at = s.count[wave][mine[r] >> (kPlaceBits + pass * kDigitBits) & (kDigits - 1)] + rank[r];
+      if (pass == 0) {
+        item[at] = mine[r];
+      } else {
+        a.key1[at] = mine[r] >> kPlaceBits;
+        a.place1[at] = mine[r] & ((1u << kPlaceBits) - 1);
+      }
+    }
+    all = total;
+    __syncthreads();
+  }
+  if (tid == 0) *a.count = all;
+}
+
+// Of more tokens: how often each digit stands in each tile,
+template <int PASS>
+__global__ __launch_bounds__(kSortThreads) void k_sort_count(SortK a) {
+  __shared__ uint32_t count[kDigits];
+  if ((int)blockIdx.x >= a.tiles) return fill_piece(a, a.piece0 + blockIdx.x - a.tiles);
+  const int tid = threadIdx.x;
+  for (int i = tid; i < kDigits; i += kSortThreads) count[i] = 0;
+  __syncthreads();
+  const uint32_t n = PASS == 0 ? a.n : *a.count, first = blockIdx.x * a.tile;
+  for (uint32_t i = tid; i < a.tile; i += kSortThreads) {
+    const uint32_t at = first + i;
+    if (at >= n) break;
+    const long t = PASS == 0 ? load_index(a.tokens, a.wide, at) : (long)a.key0[at];
+    if (t >= 0 && t < a.V) atomicAdd(count + ((uint32_t)t >> (PASS * kDigitBits) & (kDigits - 1)), 1u);
+  }
+  __syncthreads();
+  for (int i = tid; i < kDigits; i += kSortThreads) a.hist[(size_t)blockIdx.x * kDigits + i] = count[i];
+}
+
+// and each token to its place: behind the smaller digits, the same digit in the tiles
+// before, and in this tile before it.  Every workgroup sums the counts for itself.
+template <int PASS>
+__global__ __launch_bounds__(kSortThreads) void k_sort_place(SortK a) {
+  __shared__ RankLds s;
+  if ((int)blockIdx.x >= a.tiles) return fill_piece(a, a.piece0 + blockIdx.x - a.tiles);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint32_t before = 0, all = 0;
+  if (tid < kDigits)
+#pragma unroll 8
+    for (int t = 0; t < a.tiles; t++) {
+      const uint32_t c = a.hist[(size_t)t * kDigits + tid];
+      if (t < (int)blockIdx.x) before += c;
+      all += c;
+    }
+  const uint32_t n = PASS == 0 ? a.n : *a.count, first = blockIdx.x * a.tile, per_wave = a.tile / kSortWaves;
+  clear_counts(s);
+  uint32_t key[kRounds], place[kRounds], rank[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; r++) {
+    rank[r] = ~0u;
+    if ((uint32_t)r * 64 >= per_wave) continue;
+    const uint32_t at = first + wave * per_wave + r * 64 + lane;
+    const bool in = at < n;
+    const long t = !in ? -1 : PASS == 0 ? load_index(a.tokens, a.wide, at) : (long)a.key0[at];
+    const bool on = t >= 0 && t < a.V;
+    key[r] = (uint32_t)t;
+    place[r] = PASS == 0 ? at : in ? a.place0[at] : 0;
+    const uint32_t k = rank_in_wave(s, wave, lane, key[r] >> (PASS * kDigitBits) & (kDigits - 1), on);
+    if (on) rank[r] = k;
+  }
+  __syncthreads();
+  uint32_t total;
+  const uint32_t base = scan_digits(s, all, &total);
+  place_waves(s, base + before);
+  uint32_t *to_key = PASS == 0 ? a.key0 : a.key1, *to_place = PASS == 0 ? a.place0 : a.place1;
+#pragma unroll
+  for (int r = 0; r < kRounds; r++) {
+    if (rank[r] == ~0u) continue;
+    const uint32_t at = s.count[wave][key[r] >> (PASS * kDigitBits) & (kDigits - 1)] + rank[r];
+    to_key[at] = key[r];
+    to_place[at] = place[r];
+  }
+  if (PASS == 0 && blockIdx.x == 0 && tid == 0) *a.count = total;
+}
+
+// ---- sums along the sorted list --------------------------------------------------------
+
+struct SumK {
+  const char* g;
+  char* grad;
+  size_t g_bytes, grad_bytes;
+  const uint32_t *key, *place, *count;
+  float* partial;  // [stretches][2][packets * kInPacket]: of the token that came in, of the one that goes out
+  int D, packets, add;
+  uint32_t stretch, stretches;
+  float scale;
+};
+
+// scale * v to the table's row (or on top of it).
+template <int DT, int OUT>
+__device__ __forceinline__ void finish(const SumK& a, uint32_t token, int j, const float* v) {
+  constexpr int n = Type<DT>::kInPacket, m = Type<OUT>::kInPacket;
+  typedef typename Type<OUT>::mem mem;
+  char* row = a.grad + (size_t)token * a.grad_bytes;
+#pragma unroll
+  for (int h = 0; h < n; h += m) {
+    const int jh = j + h;
+    if (jh + m <= a.D) {
+      mem* to = reinterpret_cast<mem*>(row + (size_t)jh * Type<OUT>::kBytes);
+      float w[m];
+      packet old{0, 0, 0, 0};
+      if (a.add) old = *to;
+#pragma unroll
+      for (int q = 0; q < m; q++) w[q] = v[h + q] * a.scale + (a.add ? value<OUT>(old, q) : 0.0f);
+      packet p;
+#pragma unroll
+      for (int q = 0; q < 4; q++)
+        p[q] = OUT == DTL_F32 ? bits_of<OUT>(w[q % m]) : bits_of<OUT>(w[2 * q % m]) | bits_of<OUT>(w[(2 * q + 1) % m]) << 16;
+      *to = p;
+    } else {
+#pragma unroll
+      for (int q = 0; q < m; q++)
+        if (jh + q < a.D) store_one<OUT>(row, jh + q, v[h + q] * a.scale + (a.add ? load_one<OUT>(row, jh + q) : 0.0f));
+    }
+  }
+}
+
+// A thread a stretch and packet of columns.
+template <int DT, int OUT>
+__global__ __launch_bounds__(kThreads) void k_embedding_sum(SumK a) {
+  constexpr int n = Type<DT>::kInPacket, kAhead = 8;
+  const uint32_t at = blockIdx.x * kThreads + threadIdx.x, c = at / (uint32_t)a.packets;
+  const int col = (int)(at - c * (uint32_t)a.packets), j = col * n;
+  const uint32_t all = *a.count, first = c * a.stretch, end = min(all, first + a.stretch);
+  if (c >= a.stretches || first >= all) return;
+  float* partial = a.partial + (size_t)c * 2 * a.packets * n + j;
+  uint32_t now = a.key[first];
+  bool came = first > 0 && a.key[first - 1] == now;
+  float sum[n] = {};
+  auto keep = [&](bool out) {  // the sum so far, for the join
+    float* p = partial + (out ? (size_t)a.packets * n : 0);
+#pragma unroll
+    for (int q = 0; q < n; q += 4) *reinterpret_cast<float4*>(p + q) = make_float4(sum[q], sum[q + 1], sum[q + 2], sum[q + 3]);
+  };
+  for (uint32_t p = first; p < end; p += kAhead) {
+    uint32_t key[kAhead], place[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; i += 4) {  // the lists are padded to whole stretches
+      const uint4 k = *reinterpret_cast<const uint4*>(a.key + p + i), l = *reinterpret_cast<const uint4*>(a.place + p + i);
+      key[i] = k.x, key[i + 1] = k.y, key[i + 2] = k.z, key[i + 3] = k.w;
+      place[i] = l.x, place[i + 1] = l.y, place[i + 2] = l.z, place[i + 3] = l.w;
+    }
+    packet x[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; i++)
+      if (p + i < end) x[i] = load_packet<DT>(a.g + (size_t)place[i] * a.g_bytes, j, a.D);
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) {
+      if (p + i >= end) break;
+      if (key[i] != now) {
+        if (came)
+          keep(false);
+        else
+          finish<DT, OUT>(a, now, j, sum);
+        came = false;
+        now = key[i];
+#pragma unroll
+        for (int q = 0; q < n; q++) sum[q] = 0.0f;
+      }
+#pragma unroll
+      for (int q = 0; q < n; q++) sum[q] += value<DT>(x[i], q);
+    }
+  }
+  const bool goes = end < all && a.key[end] == now;
+  if (came)
+    keep(false);
+  else if (goes)
+    keep(true);
+  else
+    finish<DT, OUT>(a, now, j, sum);
+}
+
+// The tokens that go out of a stretch where they began: a thread a stretch and packet.
+template <int DT, int OUT>
+__global__ __launch_bounds__(kThreads) void k_embedding_join(SumK a) {
+  constexpr int n = Type<DT>::kInPacket;
+  const uint32_t at = blockIdx.x * kThreads + threadIdx.x, c = at / (uint32_t)a.packets;
+  const int j = (int)(at - c * (uint32_t)a.packets) * n;
+  const uint32_t all = *a.count, first = c * a.stretch, end = first + a.stretch;
+  if (c >= a.stretches || end >= all) return;
+  const uint32_t token = a.key[end];
+  if (a.key[end - 1] != token || (first > 0 && a.key[first - 1] == token)) return;
+  const size_t one = (size_t)a.packets * n;
+  const float* p = a.partial + (size_t)c * 2 * one + one + j;
+  double sum[n];
+#pragma unroll
+  for (int q = 0; q < n; q++) sum[q] = p[q];
+  for (uint32_t d = c + 1; d * a.stretch < all && a.key[d * a.stretch] == token; d++) {
+    p = a.partial + (size_t)d * 2 * one + j;
+#pragma unroll
+    for (int q = 0; q < n; q++) sum[q] += p[q];
+  }
+  float v[n];
+#pragma unroll
+  for (int q = 0; q < n; q++) v[q] = (float)sum[q];
+  finish<DT, OUT>(a, token, j, v);
+}
+
+// ---- launches ---------------------------------------------------------------------------
+
+int packets_of(size_t width, int dtype) { return (int)((width * type_bytes(dtype) + 15) / 16); }
+
+// Positions a thread sums: as few as keep the chip's threads busy.
+uint32_t stretch_of(size_t n, size_t packets) {
+  uint32_t s = 8;
+  while (s < 1024 && n * packets / s > (1u << 18)) s *= 2;
+  return s;
+}
+
+struct Layout {  // of the scratch
+  uint32_t stretch, stretches, tile;
+  int tiles;
+  size_t list, hist, key0, place0, key1, place1, partial, bytes;
+};
+Layout layout_of(size_t n, size_t width) {
+  Layout l{};
+  // the gradient's type is not known here: 16-bit rows have the fewest packets and the
+  // longest stretches, f32 ones the most
+  l.tile = (uint32_t)(((n + kTiles - 1) / kTiles + kSortThreads - 1) / kSortThreads * kSortThreads);
+  l.tiles = (int)((n + l.tile - 1) / (l.tile ? l.tile : 1));
+  l.list = (n + 1023) / 1024 * 1024 * 4;
+  l.hist = 256;
+  l.key0 = l.hist + (size_t)kTiles * kDigits * 4;
+  l.place0 = l.key0 + l.list;
+  l.key1 = l.place0 + l.list;
+  l.place1 = l.key1 + l.list;
+  l.partial = l.place1 + l.list;
+  l.bytes = l.partial;
+  for (int e : {DTL_F32, DTL_BF16}) {
+    const size_t packets = packets_of(width, e), stretch = stretch_of(n, packets);
+    const size_t need = l.partial + (n + stretch - 1) / stretch * 2 * packets * (e == DTL_F32 ? 4 : 8) * 4;
+    if (need > l.bytes) l.bytes = need;
+  }
+  return l;
+}
+
+}  // namespace
+}  // namespace dtl
+
+// ---- C entry points ------------------------------------------------------------------------
+
+using namespace dtl;
+
+namespace {
+
+// As for rows of logits.
+bool spacing_ok(size_t rows, size_t width, size_t stride) {
+  return rows <= 1 || (stride >= width && stride <= ((size_t)1 << 48) / rows);
+}
+
+bool dtype_ok(int t) { return t == DTL_F32 || t == DTL_BF16 || t == DTL_F16; }
+
+int check_table(const dtl_table* t) {
+  if (!t || !dtype_ok(t->dtype)) return DTL_ERR_INVALID_ARGUMENT;
+  if (t->vocab == 0) return DTL_ERR_CDF_EMPTY;
+  if (t->vocab > (size_t)kScoreMaxVocab) return DTL_ERR_CDF_TOO_MANY_SYMBOLS;
+  if (t->width == 0 || t->width > kEmbedMaxWidth) return DTL_ERR_SHAPE;
+  if (!spacing_ok(t->vocab, t->width, t->stride)) return DTL_ERR_SHAPE;
+  if (!t->data || reinterpret_cast<uintptr_t>(t->data) % type_bytes(t->dtype)) return DTL_ERR_INVALID_ARGUMENT;
+  return DTL_OK;
+}
+int check_rows(const void* p, int dtype, size_t n, size_t width, size_t stride) {
+  if (!spacing_ok(n, width, stride)) return DTL_ERR_SHAPE;
+  return n && (!p || reinterpret_cast<uintptr_t>(p) % type_bytes(dtype)) ? DTL_ERR_INVALID_ARGUMENT : DTL_OK;
+}
+// From a tensor's first row to the end of its last.
+size_t extent(size_t n, size_t width, size_t stride, int dtype) {
+  return n ? ((n - 1) * stride + width) * type_bytes(dtype) : 0;
+}
+bool apart(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x + na <= y || y + nb <= x;
+}
+template <typename K>
+void launch_threads(void (*kernel)(K), size_t threads, hipStream_t s, const K& k) {
+  launch_kernel(kernel, dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, k);
+}
+
+}  // namespace
+
+extern "C" {
+
+int dtl_embedding(const dtl_table* t, const void* tokens, int token_bytes, size_t n, float scale, void* out,
+                  size_t out_stride, void* stream) {
+  int st = check_table(t);
+  if (st) return st;
+  if (n > kMostRows) return DTL_ERR_SHAPE;
+  if (!index_bytes_ok(token_bytes) || (n && !tokens)) return DTL_ERR_INVALID_ARGUMENT;
+  st = check_rows(out, t->dtype, n, t->width, out_stride);
+  if (st || n == 0) return st;
+  if (!apart(out, extent(n, t->width, out_stride, t->dtype), t->data, extent(t->vocab, t->width, t->stride, t->dtype)))
+    return DTL_ERR_INVALID_ARGUMENT;
+  LookupK k{};
+  k.table = static_cast<const char*>(t->data);
+  k.out = static_cast<char*>(out);
+  k.tokens = tokens;
+  k.n = n;
+  k.table_bytes = t->stride * type_bytes(t->dtype);
+  k.out_bytes = out_stride * type_bytes(t->dtype);
+  k.V = (int)t->vocab;
+  k.D = (int)t->width;
+  k.packets = packets_of(t->width, t->dtype);
+  k.wide = token_bytes == 8;
+  k.scale = scale;
+  const size_t most = ((size_t)1 << 31) / k.packets;  // rows a launch
+  by_type(t->dtype, [&](auto dt) {
+    for (k.row0 = 0; k.row0 < n; k.row0 += most)
+      launch_threads(k_embedding<decltype(dt)::value>, (n - k.row0 < most ? n - k.row0 : most) * k.packets,
+                     static_cast<hipStream_t>(stream), k);
+  });
+  return launch_status();
+}
+
+size_t dtl_embedding_backward_scratch(size_t n, size_t vocab, size_t width) {
+  if (n > kEmbedMaxTokens || vocab > (size_t)kScoreMaxVocab || width > kEmbedMaxWidth) return 0;
+  return layout_of(n, width).bytes;
+}
+
+int dtl_embedding_backward(const void* tokens, int token_bytes, size_t n, const void* grad_out, int grad_dtype,
+                           size_t grad_out_stride, float scale, const dtl_table* grad, int add, void* scratch,
+                           size_t scratch_bytes, void* stream) {
+  int st = check_table(grad);
+  if (st) return st;
+  if (!dtype_ok(grad_dtype) || (grad->dtype != grad_dtype && grad->dtype != DTL_F32)) return DTL_ERR_INVALID_ARGUMENT;
+  if (n > kEmbedMaxTokens) return DTL_ERR_SHAPE;
+  if (!index_bytes_ok(token_bytes) || (n && !tokens)) return DTL_ERR_INVALID_ARGUMENT;
+  st = check_rows(grad_out, grad_dtype, n, grad->width, grad_out_stride);
+  if (st) return st;
+  const Layout l = layout_of(n, grad->width);
+  if (scratch_bytes < l.bytes) return DTL_ERR_BUFFER_TOO_SMALL;
+  if (!scratch || reinterpret_cast<uintptr_t>(scratch) % 16) return DTL_ERR_INVALID_ARGUMENT;
+  const size_t e = type_bytes(grad->dtype), all = extent(grad->vocab, grad->width, grad->stride, grad->dtype);
+  if (n && !apart(grad->data, all, grad_out, extent(n, grad->width, grad_out_stride, grad_dtype)))
+    return DTL_ERR_INVALID_ARGUMENT;
+  if (n == 0 && add) return DTL_OK;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* mem = static_cast<char*>(scratch);
+
+  SortK k{};
+  k.tokens = tokens;
+  k.wide = token_bytes == 8;
+  k.V = (int)grad->vocab;
+  k.n = (uint32_t)n;
+  k.tile = l.tile;
+  k.count = reinterpret_cast<uint32_t*>(mem);
+  k.hist = reinterpret_cast<uint32_t*>(mem + l.hist);
+  k.key0 = reinterpret_cast<uint32_t*>(mem + l.key0);
+  k.place0 = reinterpret_cast<uint32_t*>(mem + l.place0);
+  k.key1 = reinterpret_cast<uint32_t*>(mem + l.key1);
+  k.place1 = reinterpret_cast<uint32_t*>(mem + l.place1);
+  if (!add) {
+    const bool whole = grad->vocab == 1 || grad->stride == grad->width;
+    k.fill = static_cast<char*>(grad->data);
+    k.fill_rows = whole ? 1 : grad->vocab;
+    k.fill_bytes = (whole ? grad->vocab : 1) * grad->width * e;
+    k.fill_stride = grad->stride * e;
+    k.pieces = (k.fill_rows * ((k.fill_bytes + 15) / 16) * 16 + kFillBytes - 1) / kFillBytes;
+  }
+  if (n <= (size_t)kAlone) {
+    launch_kernel(k_sort_alone, dim3((unsigned)(1 + k.pieces)), dim3(kSortThreads), 0, s, k);
+  } else {
+    k.tiles = l.tiles;
+    const size_t quarter = (k.pieces + 3) / 4;
+    void (*const steps[])(SortK) = {k_sort_count<0>, k_sort_place<0>, k_sort_count<1>, k_sort_place<1>};
+    for (auto step : steps) {
+      launch_kernel(step, dim3((unsigned)(k.tiles + quarter)), dim3(kSortThreads), 0, s, k);
+      k.piece0 += quarter;
+    }
+  }
+  if (n) {
+    SumK u{};
+    u.g = static_cast<const char*>(grad_out);
+    u.grad = static_cast<char*>(grad->data);
+    u.g_bytes = grad_out_stride * type_bytes(grad_dtype);
+    u.grad_bytes = grad->stride * e;
+    u.key = k.key1;
+    u.place = k.place1;
+    u.count = k.count;
+    u.partial = reinterpret_cast<float*>(mem + l.partial);
+    u.D = (int)grad->width;
+    u.packets = packets_of(grad->width, grad_dtype);
+    u.add = add != 0;
+    u.stretch = stretch_of(n, u.packets);
+    u.stretches = (uint32_t)((n + u.stretch - 1) / u.stretch);
+    u.scale = scale;
+    const size_t threads = (size_t)u.stretches * u.packets;
+    by_type(grad_dtype, [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      by_bool(grad->dtype == DTL_F32, [&](auto wide) {
+        constexpr int OUT = decltype(wide)::value ? DTL_F32 : DT;
+        launch_threads(k_embedding_sum<DT, OUT>, threads, s, u);
+        if (u.stretches > 1) launch_threads(k_embedding_join<DT, OUT>, threads, s, u);
+      });
+    });
+  }
+  return launch_status();
+}
+
+}  // extern "C"

@@ -413,6 +413,34 @@ int dtl_adjust_logits(const dtl_logits *logits, const dtl_adjust *by, void *out,
 int dtl_adjust_logits_backward(const dtl_logits *logits, const dtl_adjust *by, const void *grad_out,
                                size_t grad_out_stride, void *grad, size_t grad_stride, void *stream);
 
+/* ---- the two ends of a student's training step ------------------------------
+ * No counterpart in the reference.  Conventions as for the scores above. */
+
+/* A table of embeddings or its gradient: row v at data + v * stride elements;
+ * vocab <= 2^18, width <= 2^16, any stride >= width, data aligned to an element. */
+typedef struct dtl_table {
+    void *data;
+    int dtype; /* dtl_dtype */
+    size_t vocab, width, stride;
+} dtl_table;
+
+/* out[i] = scale * table[tokens[i]] for n <= 2^24 tokens (token_bytes 4 or 8), in the
+ * table's type, row i at out + i * out_stride elements; the product is rounded once.
+ *   token < 0: padding, a row of zeros.  token >= vocab: NaN. */
+int dtl_embedding(const dtl_table *table, const void *tokens, int token_bytes, size_t n, float scale,
+                  void *out, size_t out_stride, void *stream);
+/* Scratch bytes of dtl_embedding_backward. */
+size_t dtl_embedding_backward_scratch(size_t n, size_t vocab, size_t width);
+/* The gradient of the table for that of the n <= 2^20 rows (row i at grad_out + i *
+ * grad_out_stride elements of type grad_dtype): grad[v] = scale * the sum of the rows
+ * of token v, zeros where there are none.  Padding and tokens >= vocab are not read.
+ * add != 0: added to what grad holds, whose other rows are then left alone.  grad has
+ * the rows' type or is f32, and lies over no part of them.  The sums are 32-bit ones,
+ * in an order that the tokens fix: the same inputs give the same bits. */
+int dtl_embedding_backward(const void *tokens, int token_bytes, size_t n, const void *grad_out,
+                           int grad_dtype, size_t grad_out_stride, float scale, const dtl_table *grad,
+                           int add, void *scratch, size_t scratch_bytes, void *stream);
+
 /* logits_to_cdf / logits_to_symbol_range on caller logits (host memory):
  * uploads them and runs the same device kernels (cdf.rs:47-199). */
 int dtl_logits_to_cdf(const float *logits, size_t n, size_t tail_symbols, uint32_t *freq,
