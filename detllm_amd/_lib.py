@@ -171,6 +171,11 @@ _SIGS = {
     "dtl_embedding_backward_scratch": (sz, [sz, sz, sz]),
     "dtl_embedding_backward": (C.c_int, [C.c_void_p, C.c_int, sz, C.c_void_p, C.c_int, sz, C.c_float, C.POINTER(Table),
                                          C.c_int, C.c_void_p, sz, C.c_void_p]),
+    # tensors and out: arrays of dtl_tensor (data, count, dtype and padding, 8 bytes each)
+    "dtl_grad_norm_scratch": (sz, [C.c_void_p, sz]),
+    "dtl_grad_norm": (C.c_int, [C.c_void_p, sz, C.c_int, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, sz, C.c_void_p]),
+    "dtl_clip_grads": (C.c_int, [C.c_void_p, sz, C.c_int, C.c_float, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p,
+                                 C.c_void_p, sz, C.c_void_p]),
     "dtl_session_token_scores": (C.c_int, [C.c_void_p, sz, sz, u32p, C.c_float, sz, f32p, f32p, C.POINTER(C.c_int32),
                                            f32p]),
     "dtl_range_encoder_new": (C.c_int, [vpp]),

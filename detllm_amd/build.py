@@ -39,7 +39,7 @@ SOURCES = [
 # Operators with arithmetic of their own, outside the reference's contract
 # that csrc is held to: hardware 2^x and fused multiply-adds.
 SCORES_SRC = PKG / "csrc_scores"
-SCORES_SOURCES = ["dtl_scores.hip", "dtl_adjust.hip", "dtl_embedding.hip"]
+SCORES_SOURCES = ["dtl_scores.hip", "dtl_adjust.hip", "dtl_embedding.hip", "dtl_clip.hip"]
 
 NUMERIC_FLAGS = [
     "-ffp-contract=off",

@@ -25,6 +25,7 @@ constexpr int kAdjustMaxHistory = 1 << 17;
 constexpr int kAdjustMaxBiases = 4096;
 constexpr size_t kEmbedMaxWidth = 1 << 16;
 constexpr size_t kEmbedMaxTokens = 1 << 20;  // of a gradient
+constexpr size_t kClipMaxTensors = 1 << 16;
 constexpr float kScoreMinTemperature = 1e-4f, kScoreMaxTemperature = 1e4f;
 
 struct ScoreArgs {

@@ -17,10 +17,13 @@ Reverse mode only.
 from __future__ import annotations
 
 import ctypes as C
+import math
+from array import array
 from functools import lru_cache
-from typing import Optional
+from typing import Iterable, List, Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import DetllmError, lib
@@ -135,3 +138,108 @@ def embedding_grad(tokens: torch.Tensor, grad: torch.Tensor, vocab: Optional[int
     _gradient(tokens, grad, float(scale), out, add)
     torch.autograd.graph.increment_version(out)  # autograd is told that it was written
     return out
+
+
+# ---- the gradients' norm, and clipping ---------------------------------------------------
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the tensor's elements fill their memory, in whatever order."""
+    if t.is_contiguous():
+        return True
+    n = 1
+    for stride, size in sorted((s, k) for k, s in zip(t.shape, t.stride()) if k != 1):
+        if stride != n:
+            return False
+        n *= size
+    return True
+
+
+def _tensor_list(tensors, name: str) -> Tuple[List[torch.Tensor], array]:
+    """The tensors and an array of dtl_tensor."""
+    if isinstance(tensors, torch.Tensor):
+        tensors = [tensors]
+    tensors = [t for t in tensors if t is not None]
+    dual = getattr(forward_ad, "_current_level", 0) >= 0
+    grad = torch.is_grad_enabled()
+    if _tracing():
+        raise RuntimeError("calls of the library cannot be recorded by torch.jit.trace")
+    table = array("Q")
+    device = tensors[0].device if tensors and isinstance(tensors[0], torch.Tensor) else None
+    for t in tensors:
+        dtype = _DTYPES.get(t.dtype) if isinstance(t, torch.Tensor) else None
+        if dtype is None:
+            raise TypeError(f"{name} must be float32, bfloat16 or float16 tensors")
+        if t.layout is not torch.strided:
+            raise TypeError(f"{name} must not be sparse")
+        if dual:
+            _no_tangent(t, name)
+        if not t.is_cuda or t.device != device:
+            raise ValueError(f"{name} must be on one GPU")
+        if grad and t.requires_grad:
+            raise ValueError(f"{name} need a gradient, which a norm here does not have: detach them")
+        if not (t.is_contiguous() or _dense(t)):
+            raise ValueError(f"{name} must fill their memory: call .contiguous()")
+        table.extend((t.data_ptr(), t.numel(), dtype))
+    return tensors, table
+
+
+def _norm(grads, norm_type, scale, max_norm=None, out=None):
+    grads, table = _tensor_list(grads, "grads")
+    if norm_type not in (2, math.inf):
+        raise ValueError("norm_type must be 2 or inf")
+    if not grads:
+        return torch.zeros(())
+    device = grads[0].device
+    at = None
+    if isinstance(scale, torch.Tensor):
+        if scale.dtype != torch.float32 or scale.numel() != 1 or scale.device != device:
+            raise ValueError("scale must be a number or one float32 on the gradients' device")
+        _no_tangent(scale, "scale")
+        at, scale = scale.data_ptr(), 0.0
+    written = grads
+    to = None
+    if out is not None:
+        written, to = _tensor_list(out, "out")
+        if len(written) != len(grads):
+            raise ValueError("out must have a tensor for each gradient")
+        for t, o in zip(grads, written):
+            if o.shape != t.shape or o.device != device:
+                raise ValueError("out must have the gradients' shapes and device")
+            if o.dtype != t.dtype and o.dtype != torch.float32:
+                raise TypeError("out must have the gradients' types, or be float32")
+            if o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()):
+                raise ValueError("out must have the gradients' strides")
+    address = table.buffer_info()[0]
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    need = lib.dtl_grad_norm_scratch(address, len(grads))
+    scratch = _scratch(need, device)
+    kind = int(norm_type == math.inf)
+    if max_norm is None:
+        _call(device, lib.dtl_grad_norm, address, len(grads), kind, scale, at, _ptr(norm), _ptr(scratch), need)
+        return norm
+    _call(device, lib.dtl_clip_grads, address, len(grads), kind, scale, at, max_norm,
+          None if to is None else to.buffer_info()[0], _ptr(norm), _ptr(scratch), need)
+    torch.autograd.graph.increment_version(written)  # autograd is told that they were written
+    return norm
+
+
+def grad_norm(grads: Union[torch.Tensor, Iterable[Optional[torch.Tensor]]], *, norm_type: float = 2.0,
+              scale: Union[float, torch.Tensor] = 1.0) -> torch.Tensor:
+    """dtl_grad_norm: scale times the norm over all elements of the tensors (float32,
+    bfloat16 or float16, mixed as they come; None is left out), on the device: the 2-norm,
+    summed in 64 bits, or with norm_type=inf the largest magnitude.  scale: what the
+    gradients are to be multiplied by (1 / the loss scale), a number or one float32 on
+    the device."""
+    return _norm(grads, norm_type, scale if isinstance(scale, torch.Tensor) else float(scale))
+
+
+def clip_grad_norm(grads: Union[torch.Tensor, Iterable[Optional[torch.Tensor]]], max_norm: float, *,
+                   norm_type: float = 2.0, scale: Union[float, torch.Tensor] = 1.0,
+                   out: Optional[Iterable[torch.Tensor]] = None) -> torch.Tensor:
+    """dtl_clip_grads: the gradients times scale and, where grad_norm is above max_norm,
+    times max_norm / (norm + 1e-6), in place; returns the norm on the device, without
+    waiting for it.  out: where they go instead, a tensor for each, of their shapes and
+    types or float32 (what an optimizer of float32 weights takes)."""
+    return _norm(grads, norm_type, scale if isinstance(scale, torch.Tensor) else float(scale),
+                 float(max_norm), out)

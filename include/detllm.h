@@ -441,6 +441,33 @@ int dtl_embedding_backward(const void *tokens, int token_bytes, size_t n, const 
                            int grad_dtype, size_t grad_out_stride, float scale, const dtl_table *grad,
                            int add, void *scratch, size_t scratch_bytes, void *stream);
 
+/* `count` elements in device memory, aligned to an element. */
+typedef struct dtl_tensor {
+    void *data;
+    size_t count;
+    int dtype; /* dtl_dtype */
+} dtl_tensor;
+
+/* Scratch bytes of dtl_grad_norm and dtl_clip_grads. */
+size_t dtl_grad_norm_scratch(const dtl_tensor *tensors, size_t n);
+/* *norm (device memory) = |s| times the 2-norm over all elements of the n <= 2^16
+ * tensors, or the largest magnitude where `largest` is set; s is *scale_at (device
+ * memory) or, where that is NULL, scale.  Squares are formed and added in 64 bits: none
+ * overflows or vanishes, and the same inputs give the same bits.  A NaN gives NaN, else
+ * an infinity infinity; no elements 0.  `tensors` itself is host memory, read before
+ * the call returns. */
+int dtl_grad_norm(const dtl_tensor *tensors, size_t n, int largest, float scale, const float *scale_at,
+                  float *norm, void *scratch, size_t scratch_bytes, void *stream);
+/* The same norm, and every element times s c, c = min(1, max_norm / (norm + 1e-6)), a
+ * 32-bit factor, the product rounded once: into `out` (n tensors of the same counts, of
+ * the gradients' types or f32), or in place where out is NULL, where a factor of 1
+ * writes nothing.  As the formula has it an infinite norm leaves zeros (NaN for
+ * infinities), a NaN norm NaN.  out[i] may be tensors[i] itself; other overlaps are
+ * refused. */
+int dtl_clip_grads(const dtl_tensor *tensors, size_t n, int largest, float scale, const float *scale_at,
+                   float max_norm, const dtl_tensor *out, float *norm, void *scratch,
+                   size_t scratch_bytes, void *stream);
+
 /* logits_to_cdf / logits_to_symbol_range on caller logits (host memory):
  * uploads them and runs the same device kernels (cdf.rs:47-199). */
 int dtl_logits_to_cdf(const float *logits, size_t n, size_t tail_symbols, uint32_t *freq,

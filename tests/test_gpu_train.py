@@ -8,3 +8,8 @@ from test_gpu_adjust import run_apart
 @pytest.mark.gpu
 def test_embeddings():
     run_apart("torch_embedding.py")
+
+
+@pytest.mark.gpu
+def test_gradient_norms_and_clipping():
+    run_apart("torch_clip.py")

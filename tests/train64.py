@@ -35,3 +35,20 @@ def gradient(tokens, grad, vocab, scale, dtype, old=None):
             out = np.where(touched[:, None], out + old, old)
             tol += np.where(touched[:, None], 1.01 * 2.0**-24 * np.abs(out), 0.0)
         return within(out, dtype), tol + np.where(n[:, None] > 0, rounded(out, dtype), 0.0)
+
+
+def norm(tensors, scale=1.0, largest=False):
+    """(norm, tolerance): 64-bit squares and sums are off by less than a 32-bit rounding,
+    which is the one that counts; 2^-150 where that is of the smallest numbers."""
+    with np.errstate(all="ignore"):
+        every = np.concatenate([np.zeros(1)] + [np.asarray(t, np.float64).ravel() for t in tensors])
+        v = within(abs(scale) * (np.abs(every).max() if largest else np.sqrt(np.longdouble(1) * (every * every).sum())), "f32")
+        return float(v), 1.01 * 2.0**-24 * float(np.abs(v)) + 2.0**-150
+
+
+def clipped(t, norm, max_norm, scale, dtype):
+    """(clipped, tolerance): the factor's rounding, the product's, and the type's."""
+    with np.errstate(all="ignore"):
+        c = max_norm / (norm + 1e-6)
+        out = within(within(np.asarray(t, np.float64) * (scale * (1.0 if c > 1.0 else c)), "f32"), dtype)
+        return out, 1.01 * 2.0**-23 * np.abs(out) + rounded(out, dtype) + 2.0**-149
