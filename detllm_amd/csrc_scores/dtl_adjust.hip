@@ -5,16 +5,13 @@
 //   the prompt: a -= presence + frequency n;  a += bias;  not allowed: a = -inf.
 //   dz = g (theta^-1 or theta where the token stood, 0 where it is not allowed).
 //
-// Almost every logit is only copied or masked, so the row goes through registers
-// in 16-byte packets as it is, and the few tokens of the history and the biases
-// are written over it afterwards.  Bound by memory: one read and one write of the
-// logits (in place, only the masked ones are written), an eighth of a byte of mask.
-//
-// A workgroup has a segment of a row.  It counts the history's tokens there in a
-// table in LDS, one word a logit of the segment (a direct table needs no probing,
-// and integer sums have no order); whoever touches a word first puts its place on
-// a list, and a thread an entry patches the logits.  Each segment's workgroup scans
-// the whole history, from the caches.
+// Bound by memory: one read and one write of the logits (in place, only what changes
+// is read and written), an eighth of a byte of mask.  A workgroup has a segment of a
+// row, whose logits go through registers in 16-byte packets.  It counts the history's
+// tokens there in a table in LDS, one word a logit of the segment: a direct table needs
+// no probing, and integer sums have no order.  Almost every logit is only copied or
+// masked, so a lane goes through those of its packet that the table names one by one.
+// Each segment's workgroup scans the whole history, from the caches.
 #include "dtl_scores.h"
 
 #include "dtl_rows.h"
@@ -22,7 +19,7 @@
 namespace dtl {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 
 // A table word: 13 bits of the last bias's place + 1, whether the token stands in
 // the prompt, and how often behind it.
@@ -77,30 +74,52 @@ __device__ __forceinline__ packet blend(packet p, uint32_t bits, uint32_t no) {
 
 __device__ __forceinline__ float of_row(const float* rows, float one, size_t row) { return rows ? rows[row] : one; }
 
+// An element of a packet, and its bits put back; q differs from lane to lane.
+template <int DT>
+__device__ __forceinline__ uint32_t word_of(const packet& p, int q) {
+  const int d = DT == DTL_F32 ? q : q / 2;
+  return d == 0 ? p[0] : d == 1 ? p[1] : d == 2 ? p[2] : p[3];
+}
+template <int DT>
+__device__ __forceinline__ float pick(const packet& p, int q) {
+  const uint32_t w = word_of<DT>(p, q);
+  if constexpr (DT == DTL_F32) return __builtin_bit_cast(float, w);
+  const uint32_t h = q & 1 ? w >> 16 : w & 0xffffu;
+  if constexpr (DT == DTL_BF16) return __builtin_bit_cast(float, h << 16);
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+}
+template <int DT>
+__device__ __forceinline__ void put(packet& p, int q, float v) {
+  uint32_t w = bits_of<DT>(v);
+  if constexpr (DT != DTL_F32) w = q & 1 ? (word_of<DT>(p, q) & 0xffffu) | w << 16 : (word_of<DT>(p, q) & 0xffff0000u) | w;
+  const int at = DT == DTL_F32 ? q : q / 2;
+#pragma unroll
+  for (int d = 0; d < 4; d++) p[d] = at == d ? w : p[d];
+}
+
 template <int DT, int MODE, bool TABLE, int SEG>
 __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
   typedef typename Type<DT>::mem mem;
-  constexpr int n = Type<DT>::kInPacket, np = SEG / (kThreads * n), kHistory = 8;
+  constexpr int n = Type<DT>::kInPacket, np = SEG / (kThreads * n), kHistory = 4;
   constexpr uint32_t no = MODE == GRAD ? 0u : Type<DT>::kMasked;
   static_assert(np * kThreads * n == SEG, "whole packets");
   __shared__ __attribute__((aligned(16))) uint32_t table[TABLE ? SEG : 4];
-  __shared__ uint16_t list[TABLE ? SEG : 1];
-  __shared__ uint32_t listed;
   const int tid = threadIdx.x;
   const size_t row = a.row0 + blockIdx.x / a.nseg;
   const int base = (int)(blockIdx.x % a.nseg) * SEG, end = min(a.V, base + SEG);
   const char* from = a.from + row * a.from_bytes;
   char* out = a.out + row * a.out_bytes;
 
-  // the history's first ids, then the segment: their loads run together
-  long ids[kHistory];
-  const size_t hrow = row * a.by.history_stride;
+  // the first ids of the lists, then the segment: their loads run together
+  long ids[kHistory], bias_id = -1;
+  const size_t hrow = row * a.by.history_stride, brow = row * a.by.bias_stride;
   if (TABLE) {
 #pragma unroll
     for (int i = 0; i < kHistory; i++) {
       const int at = tid + i * kThreads;
       ids[i] = at < a.history_len ? load_index(a.by.history, a.by.history_bytes == 8, hrow + at) : -1;
     }
+    if (tid < a.bias_len) bias_id = load_index(a.by.bias_ids, a.by.bias_bytes == 8, brow + tid);
   }
   const bool masked = a.by.allowed != nullptr;
   packet p[np];
@@ -114,46 +133,86 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
       if (MODE != IN_PLACE) p[i] = load_packet<DT>(from, j, end);
     }
   }
+
+  float theta = 1.0f, presence = 0.0f, frequency = 0.0f;
   if (TABLE) {
-    if (tid == 0) listed = 0;
+    theta = of_row(a.by.repetitions, a.by.repetition, row);
+    presence = of_row(a.by.presences, a.by.presence, row);
+    frequency = of_row(a.by.frequencies, a.by.frequency, row);
+    const int prompt = a.by.prompt ? a.by.prompt[row] : 0;
     for (int i = tid * 4; i < SEG; i += kThreads * 4) *reinterpret_cast<packet*>(table + i) = packet{0, 0, 0, 0};
     __syncthreads();
-    auto touched = [&](uint32_t j, uint32_t before) {
-      if (before == 0) list[atomicAdd(&listed, 1u)] = (uint16_t)j;
-    };
     if (a.bias_len) {
-      for (int k = tid; k < a.bias_len; k += kThreads) {
-        const long id = load_index(a.by.bias_ids, a.by.bias_bytes == 8, row * a.by.bias_stride + k);
+      auto place = [&](long id, int k) {
         const uint64_t j = (uint64_t)(id - base);
-        if (j < (uint64_t)(end - base)) touched((uint32_t)j, atomicMax(table + j, (uint32_t)k + 1));
-      }
+        if (j < (uint64_t)(end - base)) atomicMax(table + j, (uint32_t)k + 1);
+      };
+      place(bias_id, tid);
+      for (int k = tid + kThreads; k < a.bias_len; k += kThreads)
+        place(load_index(a.by.bias_ids, a.by.bias_bytes == 8, brow + k), k);
       __syncthreads();
     }
     if (a.history_len) {
-      const int prompt = a.by.prompt ? a.by.prompt[row] : 0;
       auto count = [&](long id, int at) {
         const uint64_t j = (uint64_t)(id - base);
-        if (j < (uint64_t)(end - base))
-          touched((uint32_t)j, at < prompt ? atomicOr(table + j, kInPrompt) : atomicAdd(table + j, kOnce));
+        if (j >= (uint64_t)(end - base)) return;
+        if (at < prompt)
+          atomicOr(table + j, kInPrompt);
+        else
+          atomicAdd(table + j, kOnce);
       };
 #pragma unroll
       for (int i = 0; i < kHistory; i++) count(ids[i], tid + i * kThreads);
+#pragma unroll 4
       for (int at = tid + kHistory * kThreads; at < a.history_len; at += kThreads)
         count(load_index(a.by.history, a.by.history_bytes == 8, hrow + at), at);
+      __syncthreads();
     }
+  }
+
+  // which of a packet's logits were touched and stay allowed
+  uint32_t hits[np];
+  packet sign[MODE == GRAD ? np : 1];
+#pragma unroll
+  for (int i = 0; i < np; i++) {
+    hits[i] = 0;
+    if (!TABLE) continue;
+    const int at = (i * kThreads + tid) * n;
+#pragma unroll
+    for (int q = 0; q < n; q += 4) {
+      const packet w = *reinterpret_cast<const packet*>(table + at + q);
+#pragma unroll
+      for (int k = 0; k < 4; k++) hits[i] |= w[k] ? 1u << (q + k) : 0u;
+    }
+    hits[i] &= bits[i];
+    if (MODE == GRAD && hits[i]) sign[i] = load_packet<DT>(a.z + row * a.z_bytes, base + at, end);
   }
 
 #pragma unroll
   for (int i = 0; i < np; i++) {
-    const int j = base + (i * kThreads + tid) * n;
+    const int at = (i * kThreads + tid) * n, j = base + at;
     if (j >= end) continue;
     const int here = min(n, end - j);
     const uint32_t all = (1u << here) - 1, on = bits[i] & all;
     if (MODE == IN_PLACE) {
-      if (on == all) continue;
+      if (on == all && !hits[i]) continue;
       p[i] = on ? load_packet<DT>(from, j, end) : packet{no, no, no, no};
     }
-    const packet w = blend<DT>(p[i], bits[i], no);
+    packet w = blend<DT>(p[i], bits[i], no);
+    for (uint32_t h = hits[i]; h; h &= h - 1) {
+      const int q = __builtin_ctz(h);
+      const uint32_t word = table[at + q], times = word / kOnce;
+      const float x = pick<DT>(w, q);
+      if (MODE == GRAD) {
+        put<DT>(w, q, pick<DT>(sign[i], q) > 0.0f ? x / theta : x * theta);
+        continue;
+      }
+      float v = x;
+      if (word > kPlaceMask) v = x > 0.0f ? x / theta : x * theta;
+      if (times) v -= presence + frequency * (float)times;
+      if (word & kPlaceMask) v += a.by.biases[brow + (word & kPlaceMask) - 1];
+      put<DT>(w, q, v);
+    }
     if (here == n) {
       mem* to = reinterpret_cast<mem*>(out + (size_t)j * Type<DT>::kBytes);
       if (a.past)
@@ -170,29 +229,6 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
             reinterpret_cast<uint16_t*>(out)[j + q] = (uint16_t)(w[q / 2] >> (q & 1 ? 16 : 0));
         }
     }
-  }
-  if (!TABLE) return;
-
-  wait_for_stores();
-  const float theta = of_row(a.by.repetitions, a.by.repetition, row);
-  const float presence = of_row(a.by.presences, a.by.presence, row);
-  const float frequency = of_row(a.by.frequencies, a.by.frequency, row);
-  for (uint32_t i = tid; i < listed; i += kThreads) {
-    const int at = list[i], j = base + at;
-    const uint32_t w = table[at], times = w / kOnce;
-    if (masked && !(allowed_bits<DT>(a, row, j, 1) & 1)) continue;
-    // the source is as it was: in place, only masked logits were written
-    const float z = load_one<DT>(a.z + row * a.z_bytes, j);
-    if (MODE == GRAD) {
-      const float g = load_one<DT>(from, j);
-      store_one<DT>(out, j, z > 0.0f ? g / theta : g * theta);
-      continue;
-    }
-    float v = z;
-    if (w > kPlaceMask) v = z > 0.0f ? z / theta : z * theta;
-    if (times) v -= presence + frequency * (float)times;
-    if (w & kPlaceMask) v += a.by.biases[row * a.by.bias_stride + (w & kPlaceMask) - 1];
-    store_one<DT>(out, j, v);
   }
 }
 
@@ -241,6 +277,7 @@ void launch_adjust(const AdjustArgs& a, hipStream_t s) {
   k.out_bytes = a.out_stride * e;
   k.V = a.vocab;
   k.by = a.by;
+  k.past = write_past(a.rows, k.out_bytes);
   const bool repeats = a.by.repetitions || a.by.repetition != 1.0f;
   const bool counts = a.by.presences || a.by.frequencies || a.by.presence != 0.0f || a.by.frequency != 0.0f;
   if (a.by.history && (repeats || (counts && !a.grad))) k.history_len = (int)a.by.history_len;

@@ -192,6 +192,10 @@ void by_type(int dtype, F&& f) {
 }
 inline size_t type_bytes(int dtype) { return dtype == DTL_F32 ? 4 : 2; }
 
+// Gradients larger than the memory-side cache are written past it: 423 instead of
+// 450 us for 4096 rows of 151936 bf16, 408 instead of 426 for 2048 of f32.
+inline bool write_past(size_t rows, size_t row_bytes) { return rows * row_bytes > (size_t)256 << 20; }
+
 // ---- entry points --------------------------------------------------------------------------
 
 inline int launch_status() {

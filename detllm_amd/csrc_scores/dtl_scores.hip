@@ -1155,10 +1155,6 @@ int part_groups(size_t rows, int nseg) {
 // of 205 us, as the backward faster.)
 bool read_past(size_t rows, size_t row_bytes) { return rows * row_bytes > (size_t)256 << 20; }
 
-// Gradients larger than the memory-side cache are written past it: 423 instead of
-// 450 us for 4096 rows of 151936 bf16, 408 instead of 426 for 2048 of f32.
-bool write_past(size_t rows, size_t row_bytes) { return rows * row_bytes > (size_t)256 << 20; }
-
 // Whole rows go to workgroups of one, four or eight waves by their length (us of
 // 16384 rows of 1000 bf16 with one / four / eight: scores 30 / - / 80, with 20
 // alternatives - / 149 / 225, losses - / 57 / 93), and of sixteen where there are
