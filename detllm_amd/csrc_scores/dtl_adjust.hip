@@ -19,8 +19,6 @@
 namespace dtl {
 namespace {
 
-constexpr int kThreads = 512;
-
 // A table word: 13 bits of the last bias's place + 1, whether the token stands in
 // the prompt, and how often behind it.
 constexpr uint32_t kPlaceMask = (1u << 13) - 1, kInPrompt = 1u << 13, kOnce = 1u << 14;
@@ -97,7 +95,14 @@ __device__ __forceinline__ void put(packet& p, int q, float v) {
   for (int d = 0; d < 4; d++) p[d] = at == d ? w : p[d];
 }
 
-template <int DT, int MODE, bool TABLE, int SEG>
+// Workgroups go to the eight dies in turn, each with a cache of its own: those of one
+// row on one die read its history into one cache instead of eight.
+__device__ __forceinline__ uint32_t by_die(uint32_t block, uint32_t blocks) {
+  const uint32_t each = blocks / 8;
+  return block < each * 8 ? block % 8 * each + block / 8 : block;
+}
+
+template <int DT, int MODE, bool TABLE, int SEG, int kThreads>
 __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
   typedef typename Type<DT>::mem mem;
   constexpr int n = Type<DT>::kInPacket, np = SEG / (kThreads * n), kHistory = 4;
@@ -105,8 +110,9 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
   static_assert(np * kThreads * n == SEG, "whole packets");
   __shared__ __attribute__((aligned(16))) uint32_t table[TABLE ? SEG : 4];
   const int tid = threadIdx.x;
-  const size_t row = a.row0 + blockIdx.x / a.nseg;
-  const int base = (int)(blockIdx.x % a.nseg) * SEG, end = min(a.V, base + SEG);
+  const uint32_t block = TABLE ? by_die(blockIdx.x, gridDim.x) : blockIdx.x;
+  const size_t row = a.row0 + block / a.nseg;
+  const int base = (int)(block % a.nseg) * SEG, end = min(a.V, base + SEG);
   const char* from = a.from + row * a.from_bytes;
   char* out = a.out + row * a.out_bytes;
 
@@ -163,9 +169,21 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
       };
 #pragma unroll
       for (int i = 0; i < kHistory; i++) count(ids[i], tid + i * kThreads);
-#pragma unroll 4
-      for (int at = tid + kHistory * kThreads; at < a.history_len; at += kThreads)
-        count(load_index(a.by.history, a.by.history_bytes == 8, hrow + at), at);
+      auto rest = [&](const auto* list) {
+        int at = tid + kHistory * kThreads;
+        for (; at + 7 * kThreads < a.history_len; at += 8 * kThreads) {
+          long more[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) more[i] = list[hrow + at + i * kThreads];
+#pragma unroll
+          for (int i = 0; i < 8; i++) count(more[i], at + i * kThreads);
+        }
+        for (; at < a.history_len; at += kThreads) count(list[hrow + at], at);
+      };
+      if (a.by.history_bytes == 8)
+        rest(static_cast<const int64_t*>(a.by.history));
+      else
+        rest(static_cast<const int32_t*>(a.by.history));
       __syncthreads();
     }
   }
@@ -196,6 +214,12 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
     const uint32_t all = (1u << here) - 1, on = bits[i] & all;
     if (MODE == IN_PLACE) {
       if (on == all && !hits[i]) continue;
+      // few to write: without reading their neighbours (256 rows of 151936 bf16, half of
+      // them with 3 % masked: 16.3 us, 20.8 with a read of every packet, 17.8 with none)
+      if (!hits[i] && here == n && __builtin_popcount(all & ~on) <= n / 2) {
+        for (uint32_t off = all & ~on; off; off &= off - 1) store_one<DT>(out, j + __builtin_ctz(off), -__builtin_inff());
+        continue;
+      }
       p[i] = on ? load_packet<DT>(from, j, end) : packet{no, no, no, no};
     }
     packet w = blend<DT>(p[i], bits[i], no);
@@ -232,10 +256,27 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
   }
 }
 
-template <int DT, int MODE, int SEG>
+template <int DT, int MODE, int SEG, int THREADS>
 void launch_as(AdjustK& k, size_t rows, bool table, hipStream_t s) {
   k.nseg = (k.V + SEG - 1) / SEG;
-  launch_rows(table ? k_adjust<DT, MODE, true, SEG> : k_adjust<DT, MODE, false, SEG>, rows, k.nseg, kThreads, 0, s, k);
+  launch_rows(table ? k_adjust<DT, MODE, true, SEG, THREADS> : k_adjust<DT, MODE, false, SEG, THREADS>, rows, k.nseg, THREADS,
+              0, s, k);
+}
+
+// A row's segments by its length and the history's.  us of 2048 logits by four waves /
+// 8192 by eight / 16384 by sixteen: 16384 rows of 1000 bf16 24 / 46 / 93, 8192 of 2500
+// 36 / 43 / 65; histories of 200, 16 rows of 32000 3.9 / 4.7 / 5.4; of 2048, 64 rows of
+// 151936 - / 11.7 / 12.7; of 8192, 512 such rows 345 / 139 / 110; of 32768, 8 of them 42 /
+// 25 / 17.  Segments of 8192 by four or sixteen waves: 2048 rows of 151936 f32 524 / 452,
+// eight 456; 4096 of bf16 514 / 545, eight 429.
+template <int DT, int MODE>
+void launch_mode(AdjustK& k, size_t rows, bool table, hipStream_t s) {
+  if (k.V <= 4096 || (rows * k.V < (1u << 21) && k.history_len <= 1024))
+    launch_as<DT, MODE, 2048, 256>(k, rows, table, s);
+  else if (k.history_len > 4096)
+    launch_as<DT, MODE, 16384, 1024>(k, rows, table, s);
+  else
+    launch_as<DT, MODE, 8192, 512>(k, rows, table, s);
 }
 
 }  // namespace
@@ -287,11 +328,11 @@ void launch_adjust(const AdjustArgs& a, hipStream_t s) {
   by_type(a.dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     if (a.grad)
-      launch_as<DT, GRAD, 8192>(k, a.rows, table, s);
+      launch_mode<DT, GRAD>(k, a.rows, table, s);
     else if (same)
-      launch_as<DT, IN_PLACE, 8192>(k, a.rows, table, s);
+      launch_mode<DT, IN_PLACE>(k, a.rows, table, s);
     else
-      launch_as<DT, COPY, 8192>(k, a.rows, table, s);
+      launch_mode<DT, COPY>(k, a.rows, table, s);
   });
 }
 
