@@ -238,11 +238,7 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
       put<DT>(w, q, v);
     }
     if (here == n) {
-      mem* to = reinterpret_cast<mem*>(out + (size_t)j * Type<DT>::kBytes);
-      if (a.past)
-        __builtin_nontemporal_store(w, to);
-      else
-        *to = w;
+      store_packet(reinterpret_cast<mem*>(out + (size_t)j * Type<DT>::kBytes), w, a.past);
     } else {
 #pragma unroll
       for (int q = 0; q < n; q++)

@@ -24,6 +24,7 @@ constexpr int kRounds = 8;                      // most tokens a thread of the s
 constexpr int kTiles = 128;                     // most workgroups of the sort
 constexpr int kPlaceBits = 13;
 constexpr int kAlone = 4096;                    // tokens that one workgroup sorts in LDS
+constexpr size_t kBusy = 1 << 20;  // threads that keep the chip busy
 constexpr int kFillBytes = kSortThreads * 16 * 4;  // zeros a workgroup writes
 static_assert(kScoreMaxVocab == 1 << (2 * kDigitBits), "two digits hold a token");
 static_assert((size_t)kTiles * kRounds * kSortThreads == kEmbedMaxTokens, "the sort's workgroups hold every token");
@@ -39,6 +40,7 @@ struct LookupK {
   size_t row0, n, table_bytes, out_bytes;
   int V, D, packets, wide;
   float scale;
+  bool past;  // written past the caches
 };
 
 // A thread a packet of an output row.
@@ -66,7 +68,7 @@ __global__ __launch_bounds__(kThreads) void k_embedding(LookupK a) {
       for (int q = 0; q < 4; q++)
         w[q] = DT == DTL_F32 ? bits_of<DT>(v[q % n]) : bits_of<DT>(v[2 * q % n]) | bits_of<DT>(v[(2 * q + 1) % n]) << 16;
     }
-    *reinterpret_cast<mem*>(out + (size_t)j * Type<DT>::kBytes) = w;
+    store_packet(reinterpret_cast<mem*>(out + (size_t)j * Type<DT>::kBytes), w, a.past);
   } else {
 #pragma unroll
     for (int q = 0; q < n; q++)
@@ -88,6 +90,7 @@ struct SortK {
   // zeros: rows of `fill_bytes`, of which this launch's workgroups write pieces from `piece0` on
   char* fill;
   size_t fill_rows, fill_bytes, fill_stride, piece0, pieces;
+  bool past;
 };
 
 // 16 bytes a thread and step; a row's last bytes are at least an element's.
@@ -105,7 +108,7 @@ __device__ __forceinline__ void fill_piece(const SortK& a, size_t piece) {
     char* p = a.fill + row * a.fill_stride + at * 16;
     const size_t left = a.fill_bytes - at * 16;
     if (left >= 16)
-      *reinterpret_cast<packet2*>(p) = packet{0, 0, 0, 0};
+      store_packet(reinterpret_cast<packet2*>(p), packet{0, 0, 0, 0}, a.past);
     else
       for (size_t b = 0; b < left; b += 2) *reinterpret_cast<uint16_t*>(p + b) = 0;
   }
@@ -234,21 +237,21 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(SortK a) {
   __shared__ uint32_t count[kDigits];
   if ((int)blockIdx.x >= a.tiles) return fill_piece(a, a.piece0 + blockIdx.x - a.tiles);
   const int tid = threadIdx.x;
-  for (int i = tid; i < kDigits; i += kSortThreads) count[i] = 0;
+  if (tid < kDigits) count[tid] = 0;
   __syncthreads();
   const uint32_t n = PASS == 0 ? a.n : *a.count, first = blockIdx.x * a.tile;
-  for (uint32_t i = tid; i < a.tile; i += kSortThreads) {
-    const uint32_t at = first + i;
-    if (at >= n) break;
-    const long t = PASS == 0 ? load_index(a.tokens, a.wide, at) : (long)a.key0[at];
+  for (uint32_t i = tid; i < a.tile && first + i < n; i += kSortThreads) {
+    const long t = PASS == 0 ? load_index(a.tokens, a.wide, first + i) : (long)a.key0[first + i];
     if (t >= 0 && t < a.V) atomicAdd(count + ((uint32_t)t >> (PASS * kDigitBits) & (kDigits - 1)), 1u);
   }
   __syncthreads();
-  for (int i = tid; i < kDigits; i += kSortThreads) a.hist[(size_t)blockIdx.x * kDigits + i] = count[i];
+  if (tid < kDigits) a.hist[(size_t)blockIdx.x * kDigits + tid] = count[tid];
 }
 
 // and each token to its place: behind the smaller digits, the same digit in the tiles
-// before, and in this tile before it.  Every workgroup sums the counts for itself.
+// before, and in this tile before it.  Every workgroup sums the counts for itself (a
+// launch that placed the first digit and counted the second with atomics took 60 us for
+// 500000 tokens, the two 24).
 template <int PASS>
 __global__ __launch_bounds__(kSortThreads) void k_sort_place(SortK a) {
   __shared__ RankLds s;
@@ -256,7 +259,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_place(SortK a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint32_t before = 0, all = 0;
   if (tid < kDigits)
-#pragma unroll 8
+#pragma unroll 16
     for (int t = 0; t < a.tiles; t++) {
       const uint32_t c = a.hist[(size_t)t * kDigits + tid];
       if (t < (int)blockIdx.x) before += c;
@@ -295,15 +298,22 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_place(SortK a) {
 
 // ---- sums along the sorted list --------------------------------------------------------
 
+// The list is cut into stretches, one a thread and packet of columns, and those of a
+// workgroup, `side` of them by `columns` packets, form a group.  A token's rows within a
+// stretch are summed and written by its thread; what crosses a stretch's end is joined
+// in LDS, what crosses a group's is left as a partial sum for the last launch.
 struct SumK {
   const char* g;
   char* grad;
   size_t g_bytes, grad_bytes;
   const uint32_t *key, *place, *count;
-  float* partial;  // [stretches][2][packets * kInPacket]: of the token that came in, of the one that goes out
+  float* partial;  // [groups][2][packets * kInPacket]: of the token that came in, of the one that goes out
   int D, packets, add;
-  uint32_t stretch, stretches;
+  int columns_log2;        // packets of a workgroup
+  uint32_t stretch;        // positions
+  uint32_t slabs, groups;  // workgroups side by side and along the list
   float scale;
+  bool past;
 };
 
 // scale * v to the table's row (or on top of it).
@@ -326,7 +336,7 @@ __device__ __forceinline__ void finish(const SumK& a, uint32_t token, int j, con
 #pragma unroll
       for (int q = 0; q < 4; q++)
         p[q] = OUT == DTL_F32 ? bits_of<OUT>(w[q % m]) : bits_of<OUT>(w[2 * q % m]) | bits_of<OUT>(w[(2 * q + 1) % m]) << 16;
-      *to = p;
+      store_packet(to, p, a.past);
     } else {
 #pragma unroll
       for (int q = 0; q < m; q++)
@@ -335,24 +345,40 @@ __device__ __forceinline__ void finish(const SumK& a, uint32_t token, int j, con
   }
 }
 
-// A thread a stretch and packet of columns.
+template <int n>
+struct alignas(16) Sum {
+  float v[n];
+};
+
+// The rows are read this once: without a place in the caches.
+template <int DT>
+__device__ __forceinline__ packet load_once(const char* row, int j, int D) {
+  if (j + Type<DT>::kInPacket > D) return load_packet<DT>(row, j, D);
+  return __builtin_nontemporal_load(reinterpret_cast<const typename Type<DT>::mem*>(row + (size_t)j * Type<DT>::kBytes));
+}
+
 template <int DT, int OUT>
 __global__ __launch_bounds__(kThreads) void k_embedding_sum(SumK a) {
   constexpr int n = Type<DT>::kInPacket, kAhead = 8;
-  const uint32_t at = blockIdx.x * kThreads + threadIdx.x, c = at / (uint32_t)a.packets;
-  const int col = (int)(at - c * (uint32_t)a.packets), j = col * n;
-  const uint32_t all = *a.count, first = c * a.stretch, end = min(all, first + a.stretch);
-  if (c >= a.stretches || first >= all) return;
-  float* partial = a.partial + (size_t)c * 2 * a.packets * n + j;
-  uint32_t now = a.key[first];
-  bool came = first > 0 && a.key[first - 1] == now;
+  // of each stretch: the sum of the token that came in, and what there is
+  __shared__ Sum<n> in[kThreads];
+  __shared__ uint8_t state[kThreads];
+  enum { CAME = 1, GOES = 2, ONE = 4 };
+  const int tid = threadIdx.x, columns = 1 << a.columns_log2, side = kThreads >> a.columns_log2;
+  const int s = tid >> a.columns_log2, c = tid & (columns - 1);
+  const uint32_t group = blockIdx.x / a.slabs;
+  const int col = (int)(blockIdx.x % a.slabs) * columns + c, j = col * n;
+  const uint32_t all = *a.count, first = (group * side + s) * a.stretch, end = min(all, first + a.stretch);
+  const bool here = col < a.packets && first < all;
+  uint32_t now = 0;
+  bool came = false, one = true;
   float sum[n] = {};
-  auto keep = [&](bool out) {  // the sum so far, for the join
-    float* p = partial + (out ? (size_t)a.packets * n : 0);
-#pragma unroll
-    for (int q = 0; q < n; q += 4) *reinterpret_cast<float4*>(p + q) = make_float4(sum[q], sum[q + 1], sum[q + 2], sum[q + 3]);
-  };
-  for (uint32_t p = first; p < end; p += kAhead) {
+  if (here) {
+    now = a.key[first];
+    came = first > 0 && a.key[first - 1] == now;
+  }
+  int what = came ? CAME : 0;
+  for (uint32_t p = first; here && p < end; p += kAhead) {
     uint32_t key[kAhead], place[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; i += 4) {  // the lists are padded to whole stretches
@@ -363,16 +389,18 @@ __global__ __launch_bounds__(kThreads) void k_embedding_sum(SumK a) {
     packet x[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; i++)
-      if (p + i < end) x[i] = load_packet<DT>(a.g + (size_t)place[i] * a.g_bytes, j, a.D);
+      if (p + i < end) x[i] = load_once<DT>(a.g + (size_t)place[i] * a.g_bytes, j, a.D);
 #pragma unroll
     for (int i = 0; i < kAhead; i++) {
       if (p + i >= end) break;
       if (key[i] != now) {
-        if (came)
-          keep(false);
-        else
+        if (came) {
+#pragma unroll
+          for (int q = 0; q < n; q++) in[tid].v[q] = sum[q];
+        } else {
           finish<DT, OUT>(a, now, j, sum);
-        came = false;
+        }
+        came = one = false;
         now = key[i];
 #pragma unroll
         for (int q = 0; q < n; q++) sum[q] = 0.0f;
@@ -381,35 +409,99 @@ __global__ __launch_bounds__(kThreads) void k_embedding_sum(SumK a) {
       for (int q = 0; q < n; q++) sum[q] += value<DT>(x[i], q);
     }
   }
-  const bool goes = end < all && a.key[end] == now;
-  if (came)
-    keep(false);
-  else if (goes)
-    keep(true);
-  else
-    finish<DT, OUT>(a, now, j, sum);
+  const bool goes = here && end < all && a.key[end] == now;
+  if (goes) what |= GOES;
+  if (one) what |= ONE;
+  if (here && !came && !goes) finish<DT, OUT>(a, now, j, sum);
+  if (came) {
+#pragma unroll
+    for (int q = 0; q < n; q++) in[tid].v[q] = sum[q];
+  }
+  state[tid] = (uint8_t)what;
+  __syncthreads();
+  if (!here) return;
+
+  // from stretch t on: adds what came in, as far as the token goes; whether past the group
+  auto follow = [&](int t) {
+    for (; t < side; t++) {
+      const int at = (t << a.columns_log2) + c;
+#pragma unroll
+      for (int q = 0; q < n; q++) sum[q] += in[at].v[q];
+      if (!(state[at] & ONE && state[at] & GOES)) return false;
+    }
+    return true;
+  };
+  float* partial = a.partial + (size_t)group * 2 * a.packets * n + j;
+  auto keep = [&](float* p) {
+#pragma unroll
+    for (int q = 0; q < n; q += 4) *reinterpret_cast<float4*>(p + q) = make_float4(sum[q], sum[q + 1], sum[q + 2], sum[q + 3]);
+  };
+  if (goes && !came) {  // it began here
+    if (follow(s + 1))
+      keep(partial + (size_t)a.packets * n);
+    else
+      finish<DT, OUT>(a, now, j, sum);
+  }
+  if (s == 0 && what & CAME) {
+#pragma unroll
+    for (int q = 0; q < n; q++) sum[q] = 0.0f;
+    follow(0);
+    keep(partial);
+  }
 }
 
-// The tokens that go out of a stretch where they began: a thread a stretch and packet.
+// The tokens that go out of a group where they began: a workgroup a group and slab, its
+// sides sharing the groups that such a token goes through.
 template <int DT, int OUT>
 __global__ __launch_bounds__(kThreads) void k_embedding_join(SumK a) {
-  constexpr int n = Type<DT>::kInPacket;
-  const uint32_t at = blockIdx.x * kThreads + threadIdx.x, c = at / (uint32_t)a.packets;
-  const int j = (int)(at - c * (uint32_t)a.packets) * n;
-  const uint32_t all = *a.count, first = c * a.stretch, end = first + a.stretch;
-  if (c >= a.stretches || end >= all) return;
+  constexpr int n = Type<DT>::kInPacket, kAhead = 4;
+  __shared__ double part[kThreads][n];
+  const int tid = threadIdx.x, columns = 1 << a.columns_log2, side = kThreads >> a.columns_log2;
+  const int s = tid >> a.columns_log2, c = tid & (columns - 1);
+  const uint32_t group = blockIdx.x / a.slabs, size = side * a.stretch;
+  const int col = (int)(blockIdx.x % a.slabs) * columns + c, j = col * n;
+  const uint32_t all = *a.count, first = group * size, end = first + size;
+  if (end >= all) return;
   const uint32_t token = a.key[end];
   if (a.key[end - 1] != token || (first > 0 && a.key[first - 1] == token)) return;
+  // the last group that it comes into
+  uint32_t last = group + 1, step = 1;
+  const uint32_t groups = (all - 1) / size;  // the last of all
+  while (last + step <= groups && a.key[(last + step) * size] == token) last += step, step *= 2;
+  for (; step; step /= 2)
+    if (last + step <= groups && a.key[(last + step) * size] == token) last += step;
   const size_t one = (size_t)a.packets * n;
-  const float* p = a.partial + (size_t)c * 2 * one + one + j;
-  double sum[n];
+  double sum[n] = {};
+  if (col < a.packets) {
+    if (s == 0) {
+      const float* p = a.partial + (size_t)group * 2 * one + one + j;
 #pragma unroll
-  for (int q = 0; q < n; q++) sum[q] = p[q];
-  for (uint32_t d = c + 1; d * a.stretch < all && a.key[d * a.stretch] == token; d++) {
-    p = a.partial + (size_t)d * 2 * one + j;
+      for (int q = 0; q < n; q++) sum[q] = p[q];
+    }
+    uint32_t d = group + 1 + s;
+    for (; d + (kAhead - 1) * side <= last; d += kAhead * side) {
+      Sum<n> x[kAhead];
 #pragma unroll
-    for (int q = 0; q < n; q++) sum[q] += p[q];
+      for (int i = 0; i < kAhead; i++) x[i] = *reinterpret_cast<const Sum<n>*>(a.partial + (size_t)(d + i * side) * 2 * one + j);
+#pragma unroll
+      for (int i = 0; i < kAhead; i++)
+#pragma unroll
+        for (int q = 0; q < n; q++) sum[q] += x[i].v[q];
+    }
+    for (; d <= last; d += side) {
+      const float* p = a.partial + (size_t)d * 2 * one + j;
+#pragma unroll
+      for (int q = 0; q < n; q++) sum[q] += p[q];
+    }
   }
+#pragma unroll
+  for (int q = 0; q < n; q++) part[tid][q] = sum[q];
+  __syncthreads();
+  if (s || col >= a.packets) return;
+  const int sides = last - group < (uint32_t)side ? (int)(last - group) : side;
+  for (int t = 1; t < sides; t++)
+#pragma unroll
+    for (int q = 0; q < n; q++) sum[q] += part[(t << a.columns_log2) + c][q];
   float v[n];
 #pragma unroll
   for (int q = 0; q < n; q++) v[q] = (float)sum[q];
@@ -418,24 +510,38 @@ __global__ __launch_bounds__(kThreads) void k_embedding_join(SumK a) {
 
 // ---- launches ---------------------------------------------------------------------------
 
+// What does not fit the memory-side cache together with what it is made of is written
+// past it, so that what is read beside it stays.  One pass of lookup and gradient, us,
+// past / not: 65536 bf16 rows of 2048 into 32000 161 / 223, 16384 of 896 into 151936
+// 80 / 88, 8192 f32 rows of 2048 into 32000 95 / 108; where it fits (2048 f32 rows of 576
+// into 49152) 37 / 30.
+bool past_caches(size_t bytes) { return bytes > (size_t)256 << 20; }
+
 int packets_of(size_t width, int dtype) { return (int)((width * type_bytes(dtype) + 15) / 16); }
 
-// Positions a thread sums: as few as keep the chip's threads busy.
-uint32_t stretch_of(size_t n, size_t packets) {
-  uint32_t s = 8;
-  while (s < 1024 && n * packets / s > (1u << 18)) s *= 2;
-  return s;
+// How a gradient of n positions by so many packets is cut.
+struct Cut {
+  int columns_log2;
+  uint32_t stretch, slabs, groups;
+};
+Cut cut_of(size_t n, size_t packets) {
+  Cut c{};
+  while (c.columns_log2 < 4 && (size_t)1 << c.columns_log2 < packets) c.columns_log2++;
+  c.slabs = (uint32_t)((packets + ((size_t)1 << c.columns_log2) - 1) >> c.columns_log2);
+  c.stretch = 8;
+  while (c.stretch < 64 && n * packets / c.stretch > kBusy) c.stretch *= 2;
+  const size_t size = (size_t)c.stretch * (kThreads >> c.columns_log2);
+  c.groups = (uint32_t)((n + size - 1) / size);
+  return c;
 }
 
 struct Layout {  // of the scratch
-  uint32_t stretch, stretches, tile;
+  uint32_t tile;
   int tiles;
   size_t list, hist, key0, place0, key1, place1, partial, bytes;
 };
 Layout layout_of(size_t n, size_t width) {
   Layout l{};
-  // the gradient's type is not known here: 16-bit rows have the fewest packets and the
-  // longest stretches, f32 ones the most
   l.tile = (uint32_t)(((n + kTiles - 1) / kTiles + kSortThreads - 1) / kSortThreads * kSortThreads);
   l.tiles = (int)((n + l.tile - 1) / (l.tile ? l.tile : 1));
   l.list = (n + 1023) / 1024 * 1024 * 4;
@@ -446,9 +552,9 @@ Layout layout_of(size_t n, size_t width) {
   l.place1 = l.key1 + l.list;
   l.partial = l.place1 + l.list;
   l.bytes = l.partial;
-  for (int e : {DTL_F32, DTL_BF16}) {
-    const size_t packets = packets_of(width, e), stretch = stretch_of(n, packets);
-    const size_t need = l.partial + (n + stretch - 1) / stretch * 2 * packets * (e == DTL_F32 ? 4 : 8) * 4;
+  for (int e : {DTL_F32, DTL_BF16}) {  // whichever the rows are
+    const size_t packets = packets_of(width, e);
+    const size_t need = l.partial + cut_of(n, packets).groups * 2 * packets * (e == DTL_F32 ? 4 : 8) * 4;
     if (need > l.bytes) l.bytes = need;
   }
   return l;
@@ -522,6 +628,7 @@ int dtl_embedding(const dtl_table* t, const void* tokens, int token_bytes, size_
   k.packets = packets_of(t->width, t->dtype);
   k.wide = token_bytes == 8;
   k.scale = scale;
+  k.past = past_caches((n + (n < t->vocab ? n : t->vocab)) * t->width * type_bytes(t->dtype));
   const size_t most = ((size_t)1 << 31) / k.packets;  // rows a launch
   by_type(t->dtype, [&](auto dt) {
     for (k.row0 = 0; k.row0 < n; k.row0 += most)
@@ -568,6 +675,7 @@ int dtl_embedding_backward(const void* tokens, int token_bytes, size_t n, const 
   k.place0 = reinterpret_cast<uint32_t*>(mem + l.place0);
   k.key1 = reinterpret_cast<uint32_t*>(mem + l.key1);
   k.place1 = reinterpret_cast<uint32_t*>(mem + l.place1);
+  k.past = past_caches(grad->vocab * grad->width * e + n * grad->width * type_bytes(grad_dtype));
   if (!add) {
     const bool whole = grad->vocab == 1 || grad->stride == grad->width;
     k.fill = static_cast<char*>(grad->data);
@@ -600,16 +708,20 @@ int dtl_embedding_backward(const void* tokens, int token_bytes, size_t n, const 
     u.D = (int)grad->width;
     u.packets = packets_of(grad->width, grad_dtype);
     u.add = add != 0;
-    u.stretch = stretch_of(n, u.packets);
-    u.stretches = (uint32_t)((n + u.stretch - 1) / u.stretch);
+    const Cut cut = cut_of(n, u.packets);
+    u.columns_log2 = cut.columns_log2;
+    u.stretch = cut.stretch;
+    u.slabs = cut.slabs;
+    u.groups = cut.groups;
     u.scale = scale;
-    const size_t threads = (size_t)u.stretches * u.packets;
+    u.past = k.past;
+    const size_t threads = (size_t)cut.groups * cut.slabs * kThreads;
     by_type(grad_dtype, [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
       by_bool(grad->dtype == DTL_F32, [&](auto wide) {
         constexpr int OUT = decltype(wide)::value ? DTL_F32 : DT;
         launch_threads(k_embedding_sum<DT, OUT>, threads, s, u);
-        if (u.stretches > 1) launch_threads(k_embedding_join<DT, OUT>, threads, s, u);
+        if (cut.groups > 1) launch_threads(k_embedding_join<DT, OUT>, threads, s, u);
       });
     });
   }

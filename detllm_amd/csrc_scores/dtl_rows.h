@@ -78,6 +78,19 @@ __device__ __forceinline__ packet load_packet(const char* row, int j, int V) {
   return p;
 }
 
+// Past the caches or not.  The two stores are kept apart: the compiler would make one
+// of them, without the hint.
+template <typename M>
+__device__ __forceinline__ void store_packet(M* to, const packet& p, bool past) {
+  if (past) {
+    asm volatile("");
+    __builtin_nontemporal_store(p, to);
+    asm volatile("");
+  } else {
+    *to = p;
+  }
+}
+
 __device__ __forceinline__ long load_index(const void* p, int wide, size_t i) {
   return wide ? (long)reinterpret_cast<const int64_t*>(p)[i] : (long)reinterpret_cast<const int32_t*>(p)[i];
 }

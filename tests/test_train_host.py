@@ -62,7 +62,7 @@ def test_embedding_scratch():
 
     f = lib.dtl_embedding_backward_scratch
     for n, width in ((1, 1), (1000, 896), (65536, 2048), (1 << 20, 8), (5000, 65536)):
-        assert f(n, 1000, width) >= 16 * n + n // 1024 * 2 * width * 4
+        assert f(n, 1000, width) >= 16 * n + n // 16384 * 2 * width * 4
         assert f(n, 5, width) <= 256 + 16 * (n + 1024) + 128 * 512 * 4 + (n // 8 + 1) * 2 * (width + 8) * 4
     assert f((1 << 20) + 1, 10, 8) == 0
 
