@@ -20,6 +20,7 @@ import ctypes as C
 import math
 from array import array
 from functools import lru_cache
+from operator import attrgetter
 from typing import Iterable, List, Optional, Tuple, Union
 
 import torch
@@ -31,6 +32,7 @@ from .scores import _DTYPES, _INDEX, _call, _incoming, _no_tangent, _ptr, _scrat
 
 MAX_TOKENS = 1 << 20  # of an embedding's gradient
 
+_dtype_of, _layout_of, _shape_of, _requires_grad_of = map(attrgetter, ("dtype", "layout", "shape", "requires_grad"))
 _embed_scratch = lru_cache(maxsize=256)(lib.dtl_embedding_backward_scratch)
 
 
@@ -155,32 +157,50 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _check_tensors(tensors, name: str) -> None:
+    """Says what is wrong with a list that _tensor_list does not take."""
+    for t in tensors:
+        if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES or t.layout is not torch.strided:
+            raise TypeError(f"{name} must be dense float32, bfloat16 or float16 tensors")
+        if not t.is_cuda or t.device != tensors[0].device:
+            raise ValueError(f"{name} must be on one GPU")
+        if torch.is_grad_enabled() and t.requires_grad:
+            raise ValueError(f"{name} need a gradient, which a norm here does not have: detach them")
+        if not _dense(t):
+            raise ValueError(f"{name} must fill their memory: call .contiguous()")
+
+
+_PLAIN = {torch.Tensor, torch.nn.Parameter}
+
+
 def _tensor_list(tensors, name: str) -> Tuple[List[torch.Tensor], array]:
-    """The tensors and an array of dtl_tensor."""
+    """The tensors and an array of dtl_tensor.  A model has hundreds of them: each
+    attribute is read by one map over the list."""
     if isinstance(tensors, torch.Tensor):
         tensors = [tensors]
     tensors = [t for t in tensors if t is not None]
-    dual = getattr(forward_ad, "_current_level", 0) >= 0
-    grad = torch.is_grad_enabled()
     if _tracing():
         raise RuntimeError("calls of the library cannot be recorded by torch.jit.trace")
-    table = array("Q")
-    device = tensors[0].device if tensors and isinstance(tensors[0], torch.Tensor) else None
-    for t in tensors:
-        dtype = _DTYPES.get(t.dtype) if isinstance(t, torch.Tensor) else None
-        if dtype is None:
-            raise TypeError(f"{name} must be float32, bfloat16 or float16 tensors")
-        if t.layout is not torch.strided:
-            raise TypeError(f"{name} must not be sparse")
-        if dual:
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
             _no_tangent(t, name)
-        if not t.is_cuda or t.device != device:
-            raise ValueError(f"{name} must be on one GPU")
-        if grad and t.requires_grad:
-            raise ValueError(f"{name} need a gradient, which a norm here does not have: detach them")
-        if not (t.is_contiguous() or _dense(t)):
-            raise ValueError(f"{name} must fill their memory: call .contiguous()")
-        table.extend((t.data_ptr(), t.numel(), dtype))
+    table = array("Q", bytes(24 * len(tensors)))
+    if not tensors:
+        return tensors, table
+    plain = set(map(type, tensors)) <= _PLAIN
+    dtypes = set(map(_dtype_of, tensors)) if plain else ()
+    if (not plain or not dtypes <= _DTYPES.keys() or set(map(_layout_of, tensors)) != {torch.strided}
+            or len(places := set(map(torch.Tensor.get_device, tensors))) != 1 or -1 in places
+            or torch.is_grad_enabled() and any(map(_requires_grad_of, tensors))
+            or not all(map(torch.Tensor.is_contiguous, tensors))):
+        _check_tensors(tensors, name)
+        dtypes = set(map(_dtype_of, tensors))
+    table[0::3] = array("Q", map(torch.Tensor.data_ptr, tensors))
+    table[1::3] = array("Q", map(torch.Tensor.numel, tensors))
+    if len(dtypes) == 1:
+        table[2::3] = array("Q", [_DTYPES[tensors[0].dtype]]) * len(tensors)
+    else:
+        table[2::3] = array("Q", [_DTYPES[t.dtype] for t in tensors])
     return tensors, table
 
 
@@ -203,13 +223,16 @@ def _norm(grads, norm_type, scale, max_norm=None, out=None):
         written, to = _tensor_list(out, "out")
         if len(written) != len(grads):
             raise ValueError("out must have a tensor for each gradient")
-        for t, o in zip(grads, written):
-            if o.shape != t.shape or o.device != device:
-                raise ValueError("out must have the gradients' shapes and device")
-            if o.dtype != t.dtype and o.dtype != torch.float32:
-                raise TypeError("out must have the gradients' types, or be float32")
-            if o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()):
-                raise ValueError("out must have the gradients' strides")
+        if written and written[0].device != device:
+            raise ValueError("out must be on the gradients' device")
+        if list(map(_shape_of, written)) != list(map(_shape_of, grads)):
+            raise ValueError("out must have the gradients' shapes")
+        if any(o != t and o != _lib.DTL_F32 for t, o in zip(table[2::3], to[2::3])):
+            raise TypeError("out must have the gradients' types, or be float32")
+        if list(map(torch.Tensor.stride, written)) != list(map(torch.Tensor.stride, grads)):
+            for t, o in zip(grads, written):
+                if o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()):
+                    raise ValueError("out must have the gradients' strides")
     address = table.buffer_info()[0]
     norm = torch.empty((), dtype=torch.float32, device=device)
     need = lib.dtl_grad_norm_scratch(address, len(grads))
