@@ -178,6 +178,8 @@ _SIGS = {
                                  C.c_void_p, sz, C.c_void_p]),
     "dtl_session_token_scores": (C.c_int, [C.c_void_p, sz, sz, u32p, C.c_float, sz, f32p, f32p, C.POINTER(C.c_int32),
                                            f32p]),
+    "dtl_session_adjusted_scores": (C.c_int, [C.c_void_p, sz, sz, C.POINTER(Adjust), u32p, C.c_float, sz, f32p, f32p,
+                                              C.POINTER(C.c_int32), f32p]),
     "dtl_range_encoder_new": (C.c_int, [vpp]),
     "dtl_range_encode": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64]),
     "dtl_range_encoder_finish": (C.c_int, [C.c_void_p, u8p, sz, C.POINTER(sz)]),

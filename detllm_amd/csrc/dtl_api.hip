@@ -1549,6 +1549,126 @@ int decode_step(dtl_session* s, size_t row, size_t tail, dtl_range_decoder* dec,
 
 }  // namespace
 
+namespace {
+
+// A dtl_adjust's host arrays and their places in device memory, one behind the other.
+struct HostParts {
+  struct Part {
+    const void* host;
+    size_t at, bytes;
+  };
+  Part parts[8];
+  int n = 0;
+  size_t bytes = 0;
+  size_t add(const void* host, size_t size) {
+    const size_t at = bytes;
+    if (host && size) parts[n++] = {host, at, size};
+    bytes = (bytes + size + 15) & ~(size_t)15;
+    return at;
+  }
+};
+
+int session_scores(dtl_session* s, size_t first, size_t n, const dtl_adjust* by, const uint32_t* tokens, float temperature,
+                   size_t top, float* log_probs, float* entropy, int32_t* top_ids, float* top_log_probs) {
+  if (!s || (log_probs && !tokens) || (top && (!top_ids || !top_log_probs))) return DTL_ERR_INVALID_ARGUMENT;
+  if (!(temperature >= kScoreMinTemperature && temperature <= kScoreMaxTemperature)) return DTL_ERR_INVALID_ARGUMENT;
+  const size_t V = s->m->vocab;
+  Lane& L = *s->ln;
+  if (n == 0 || n > L.rows_valid || first > L.rows_valid - n) return DTL_ERR_SHAPE;
+  if (V > (size_t)kScoreMaxVocab) return DTL_ERR_CDF_TOO_MANY_SYMBOLS;
+  if (top > (size_t)kScoreMaxTop || top > V) return DTL_ERR_SHAPE;
+  if (log_probs)
+    for (size_t i = 0; i < n; i++)
+      if (tokens[i] >= V) return DTL_ERR_CDF_SYMBOL_OUT_OF_RANGE;
+  if (by)
+    if (const int st = check_adjust(by, n, V)) return st;
+  HIP_TRY(hipSetDevice(s->m->device));
+  // tokens, log probabilities, entropy, alternatives' ids and log
+  // probabilities, then the scratch
+  const size_t scratch = score_scratch_bytes(n, V, top);
+  const size_t o_ids = 12 * n, o_lps = o_ids + 4 * n * top, o_scratch = (o_lps + 4 * n * top + 255) & ~(size_t)255;
+  // then, with `by`, its arrays and the adjusted rows
+  const size_t o_parts = (o_scratch + scratch + 255) & ~(size_t)255;
+  HostParts parts;
+  AdjustArgs adjust{};
+  dtl_adjust& d = adjust.by;
+  size_t o_rows = o_parts, o_history = 0, o_prompt = 0, o_reps = 0, o_pres = 0, o_freq = 0, o_ids_b = 0, o_bias = 0, o_mask = 0;
+  if (by) {
+    d = *by;
+    const size_t hist = by->history_len ? (n - 1) * by->history_stride + by->history_len : 0;
+    const size_t bias = by->bias_len ? (n - 1) * by->bias_stride + by->bias_len : 0;
+    const size_t mask_row = by->allowed_bits == 1 ? (V + 31) / 32 : V;
+    const size_t mask = by->allowed ? ((n - 1) * by->allowed_stride + mask_row) * (by->allowed_bits == 1 ? 4 : 1) : 0;
+    o_history = parts.add(by->history, hist * by->history_bytes);
+    o_prompt = parts.add(by->prompt, n * 4);
+    o_reps = parts.add(by->repetitions, n * 4);
+    o_pres = parts.add(by->presences, n * 4);
+    o_freq = parts.add(by->frequencies, n * 4);
+    o_ids_b = parts.add(by->bias_ids, bias * by->bias_bytes);
+    o_bias = parts.add(by->biases, bias * 4);
+    o_mask = parts.add(by->allowed, mask);
+    o_rows = (o_parts + parts.bytes + 255) & ~(size_t)255;
+  }
+  const size_t need = o_rows + (by ? n * V * 4 : 0);
+  if (s->score_arena.bytes() < need) {
+    s->score_mem = nullptr;
+    s->score_arena.release();
+    const int st = s->score_arena.alloc(&s->score_mem, need);
+    if (st) return st;
+  }
+  uint8_t* mem = s->score_mem;
+  if (log_probs) HIP_TRY(hipMemcpyAsync(mem, tokens, 4 * n, hipMemcpyHostToDevice, L.stream));
+  ScoreArgs a{};
+  a.z = L.logits + first * V;
+  a.stride = V;
+  a.rows = n;
+  a.dtype = DTL_F32;
+  a.vocab = (int)V;
+  a.tokens = log_probs ? mem : nullptr;
+  a.temperature = temperature;
+  a.top = (int)top;
+  a.log_probs = log_probs ? (float*)(mem + 4 * n) : nullptr;
+  a.entropy = (float*)(mem + 8 * n);
+  a.top_ids = (int32_t*)(mem + o_ids);
+  a.top_log_probs = (float*)(mem + o_lps);
+  a.scratch = mem + o_scratch;
+  if (by) {
+    for (int i = 0; i < parts.n; i++)
+      HIP_TRY(hipMemcpyAsync(mem + o_parts + parts.parts[i].at, parts.parts[i].host, parts.parts[i].bytes,
+                             hipMemcpyHostToDevice, L.stream));
+    auto on_device = [&](const void* host, size_t at) -> uint8_t* { return host ? mem + o_parts + at : nullptr; };
+    d.history = on_device(by->history, o_history);
+    d.prompt = (const int32_t*)on_device(by->prompt, o_prompt);
+    d.repetitions = (const float*)on_device(by->repetitions, o_reps);
+    d.presences = (const float*)on_device(by->presences, o_pres);
+    d.frequencies = (const float*)on_device(by->frequencies, o_freq);
+    d.bias_ids = on_device(by->bias_ids, o_ids_b);
+    d.biases = (const float*)on_device(by->biases, o_bias);
+    d.allowed = on_device(by->allowed, o_mask);
+    adjust.z = a.z;
+    adjust.stride = adjust.out_stride = V;
+    adjust.rows = n;
+    adjust.dtype = DTL_F32;
+    adjust.vocab = (int)V;
+    adjust.out = mem + o_rows;
+    a.z = adjust.out;
+    s->prof.timed(L.stream, "adjust_logits", (double)n * V * 8.0, 0.0, [&] { launch_adjust(adjust, L.stream); });
+  }
+  s->prof.timed(L.stream, "token_scores", (double)n * V * 4.0, 0.0, [&] { launch_token_scores(a, L.stream); });
+  HIP_TRY(hipGetLastError());
+  if (log_probs) HIP_TRY(hipMemcpyAsync(log_probs, a.log_probs, 4 * n, hipMemcpyDeviceToHost, L.stream));
+  if (entropy) HIP_TRY(hipMemcpyAsync(entropy, a.entropy, 4 * n, hipMemcpyDeviceToHost, L.stream));
+  if (top) {
+    HIP_TRY(hipMemcpyAsync(top_ids, a.top_ids, 4 * n * top, hipMemcpyDeviceToHost, L.stream));
+    HIP_TRY(hipMemcpyAsync(top_log_probs, a.top_log_probs, 4 * n * top, hipMemcpyDeviceToHost, L.stream));
+  }
+  HIP_TRY(hipStreamSynchronize(L.stream));
+  s->prof.collect();
+  return DTL_OK;
+}
+
+}  // namespace
+
 extern "C" {
 
 const char* dtl_status_string(int status) {
@@ -1980,54 +2100,14 @@ int dtl_forward_ranges(dtl_session* s, const uint32_t* tokens, size_t n, size_t 
 
 int dtl_session_token_scores(dtl_session* s, size_t first, size_t n, const uint32_t* tokens, float temperature,
                              size_t top, float* log_probs, float* entropy, int32_t* top_ids, float* top_log_probs) {
-  if (!s || (log_probs && !tokens) || (top && (!top_ids || !top_log_probs))) return DTL_ERR_INVALID_ARGUMENT;
-  if (!(temperature >= kScoreMinTemperature && temperature <= kScoreMaxTemperature)) return DTL_ERR_INVALID_ARGUMENT;
-  const size_t V = s->m->vocab;
-  Lane& L = *s->ln;
-  if (n == 0 || n > L.rows_valid || first > L.rows_valid - n) return DTL_ERR_SHAPE;
-  if (V > (size_t)kScoreMaxVocab) return DTL_ERR_CDF_TOO_MANY_SYMBOLS;
-  if (top > (size_t)kScoreMaxTop || top > V) return DTL_ERR_SHAPE;
-  if (log_probs)
-    for (size_t i = 0; i < n; i++)
-      if (tokens[i] >= V) return DTL_ERR_CDF_SYMBOL_OUT_OF_RANGE;
-  HIP_TRY(hipSetDevice(s->m->device));
-  // tokens, log probabilities, entropy, alternatives' ids and log
-  // probabilities, then the scratch
-  const size_t scratch = score_scratch_bytes(n, V, top);
-  const size_t o_ids = 12 * n, o_lps = o_ids + 4 * n * top, o_scratch = (o_lps + 4 * n * top + 255) & ~(size_t)255;
-  if (s->score_arena.bytes() < o_scratch + scratch) {
-    s->score_mem = nullptr;
-    s->score_arena.release();
-    const int st = s->score_arena.alloc(&s->score_mem, o_scratch + scratch);
-    if (st) return st;
-  }
-  uint8_t* mem = s->score_mem;
-  if (log_probs) HIP_TRY(hipMemcpyAsync(mem, tokens, 4 * n, hipMemcpyHostToDevice, L.stream));
-  ScoreArgs a{};
-  a.z = L.logits + first * V;
-  a.stride = V;
-  a.rows = n;
-  a.dtype = DTL_F32;
-  a.vocab = (int)V;
-  a.tokens = log_probs ? mem : nullptr;
-  a.temperature = temperature;
-  a.top = (int)top;
-  a.log_probs = log_probs ? (float*)(mem + 4 * n) : nullptr;
-  a.entropy = (float*)(mem + 8 * n);
-  a.top_ids = (int32_t*)(mem + o_ids);
-  a.top_log_probs = (float*)(mem + o_lps);
-  a.scratch = mem + o_scratch;
-  s->prof.timed(L.stream, "token_scores", (double)n * V * 4.0, 0.0, [&] { launch_token_scores(a, L.stream); });
-  HIP_TRY(hipGetLastError());
-  if (log_probs) HIP_TRY(hipMemcpyAsync(log_probs, a.log_probs, 4 * n, hipMemcpyDeviceToHost, L.stream));
-  if (entropy) HIP_TRY(hipMemcpyAsync(entropy, a.entropy, 4 * n, hipMemcpyDeviceToHost, L.stream));
-  if (top) {
-    HIP_TRY(hipMemcpyAsync(top_ids, a.top_ids, 4 * n * top, hipMemcpyDeviceToHost, L.stream));
-    HIP_TRY(hipMemcpyAsync(top_log_probs, a.top_log_probs, 4 * n * top, hipMemcpyDeviceToHost, L.stream));
-  }
-  HIP_TRY(hipStreamSynchronize(L.stream));
-  s->prof.collect();
-  return DTL_OK;
+  return session_scores(s, first, n, nullptr, tokens, temperature, top, log_probs, entropy, top_ids, top_log_probs);
+}
+
+int dtl_session_adjusted_scores(dtl_session* s, size_t first, size_t n, const dtl_adjust* by, const uint32_t* tokens,
+                                float temperature, size_t top, float* log_probs, float* entropy, int32_t* top_ids,
+                                float* top_log_probs) {
+  if (!by) return DTL_ERR_INVALID_ARGUMENT;
+  return session_scores(s, first, n, by, tokens, temperature, top, log_probs, entropy, top_ids, top_log_probs);
 }
 
 int dtl_session_get_info(const dtl_session* s, size_t* n_ctx, size_t* max_chunk, size_t* vocab) {

@@ -187,6 +187,53 @@ class TokenScores(NamedTuple):
     top_log_probs: np.ndarray
 
 
+def _adjust(n, vocab, history, prompt, repetition, presence, frequency, bias_ids, bias, allowed):
+    """A dtl_adjust of host arrays for n rows, and the arrays."""
+    a, keep = _lib.Adjust(), []
+
+    def held(x, dtype, shapes, name):
+        x = np.ascontiguousarray(x, dtype=dtype)
+        if x.shape not in shapes:
+            raise ValueError(f"{name} has shape {x.shape}, expected {' or '.join(map(str, shapes))}")
+        keep.append(x)
+        return x, (x.ctypes.data if x.size else None)
+
+    def rows(x, name):
+        if np.ndim(x) == 0:
+            return float(x), None
+        return 0.0, held(x, np.float32, [(n,)], name)[1]
+
+    def lists(x, name):
+        k = np.shape(x)[-1] if np.ndim(x) else 0
+        return [(n, k), (k,)]
+
+    if history is not None:
+        x, a.history = held(history, np.int64, lists(history, "history"), "history")
+        a.history_bytes, a.history_len, a.history_stride = 8, x.shape[-1], x.shape[-1] if x.ndim > 1 else 0
+        if prompt is not None:
+            a.prompt = held(np.broadcast_to(prompt, (n,)), np.int32, [(n,)], "prompt")[1]
+    elif prompt is not None:
+        raise ValueError("prompt counts places of a history")
+    a.repetition, a.repetitions = rows(repetition, "repetition")
+    a.presence, a.presences = rows(presence, "presence")
+    a.frequency, a.frequencies = rows(frequency, "frequency")
+    if (bias_ids is None) != (bias is None):
+        raise ValueError("bias_ids and bias belong together")
+    if bias is not None:
+        x, a.bias_ids = held(bias_ids, np.int64, lists(bias_ids, "bias_ids"), "bias_ids")
+        a.biases = held(bias, np.float32, [x.shape], "bias")[1]
+        a.bias_bytes, a.bias_len, a.bias_stride = 8, x.shape[-1], x.shape[-1] if x.ndim > 1 else 0
+    if allowed is not None:
+        allowed = np.asarray(allowed)
+        if allowed.dtype not in (np.bool_, np.uint32, np.int32):
+            raise TypeError("allowed must be bool, or words of 32 bits")
+        bits = allowed.dtype != np.bool_
+        k = -(-vocab // 32) if bits else vocab
+        x, a.allowed = held(allowed, np.uint32 if bits else np.uint8, [(n, k), (k,)], "allowed")
+        a.allowed_bits, a.allowed_stride = 1 if bits else 8, k if x.ndim > 1 else 0
+    return a, keep
+
+
 class Session:
     """KvCache + ForwardWorkspace + RopeTables of one decode stream (device)."""
 
@@ -320,22 +367,36 @@ class Session:
         )
         return cum[:n], freq[:n], total[:n]
 
-    def token_scores(self, tokens: Sequence[int], first: int = 0, top: int = 0,
-                     temperature: float = 1.0) -> TokenScores:
+    def token_scores(self, tokens: Sequence[int], first: int = 0, top: int = 0, temperature: float = 1.0, *,
+                     history=None, prompt=None, repetition=1.0, presence=0.0, frequency=0.0, bias_ids=None, bias=None,
+                     allowed=None) -> TokenScores:
         """Log probability of tokens[i] under row first + i of the last forward,
-        the row's entropy and its `top` alternatives, p = softmax(logits / temperature)."""
+        the row's entropy and its `top` alternatives, p = softmax(logits / temperature).
+
+        The rest says what is done to a copy of the rows before (dtl_adjust_logits):
+        penalties for the tokens of history ([n, k], or [k] for every row; -1 is none),
+        whose first prompt[i] places are a prompt; repetition, presence and frequency are
+        numbers or one for each row; bias[..., k] added to bias_ids[..., k]; allowed: bool
+        [n, vocab] or [vocab], or uint32 words of 32 bits [..., ceil(vocab / 32)].  The
+        session's logits stay as they are."""
         toks = _tokens(tokens)
+        by = None
+        if (history is not None or bias_ids is not None or bias is not None or allowed is not None
+                or prompt is not None):
+            by, keep = _adjust(toks.size, self.model.vocab, history, prompt, repetition, presence, frequency, bias_ids, bias,
+                               allowed)
         n = toks.size
         lp = np.empty(n, np.float32)
         entropy = np.empty(n, np.float32)
         ids = np.empty((n, top), np.int32)
         lps = np.empty((n, top), np.float32)
-        check(
-            lib.dtl_session_token_scores(self._h, first, n, ptr(toks, C.c_uint32), temperature, top,
-                                         ptr(lp, C.c_float), ptr(entropy, C.c_float), ptr(ids, C.c_int32),
-                                         ptr(lps, C.c_float)),
-            "dtl_session_token_scores",
-        )
+        out = (ptr(lp, C.c_float), ptr(entropy, C.c_float), ptr(ids, C.c_int32), ptr(lps, C.c_float))
+        if by is None:
+            check(lib.dtl_session_token_scores(self._h, first, n, ptr(toks, C.c_uint32), temperature, top, *out),
+                  "dtl_session_token_scores")
+        else:
+            check(lib.dtl_session_adjusted_scores(self._h, first, n, C.byref(by), ptr(toks, C.c_uint32), temperature, top,
+                                                  *out), "dtl_session_adjusted_scores")
         return TokenScores(lp, entropy, ids, lps)
 
     def cdf(self, row: int = 0, tail_symbols: int = 0):

@@ -238,6 +238,15 @@ int dtl_session_token_scores(dtl_session *session, size_t first, size_t n, const
                              float temperature, size_t top, float *log_probs, float *entropy,
                              int32_t *top_ids, float *top_log_probs);
 
+struct dtl_adjust;
+/* The same of the rows as dtl_adjust_logits (below) would leave them; the session's
+ * logits stay as they are.  The arrays that `by` points to are host memory here, read
+ * before the call returns.  Keeps device memory for the adjusted rows (4 bytes a logit)
+ * and the arrays with the session. */
+int dtl_session_adjusted_scores(dtl_session *session, size_t first, size_t n, const struct dtl_adjust *by,
+                                const uint32_t *tokens, float temperature, size_t top, float *log_probs,
+                                float *entropy, int32_t *top_ids, float *top_log_probs);
+
 /* logits_to_cdf_with_scratch / _with_byte_escapes (cdf.rs:52-106): the
  * full table for one row; freq and cum hold vocab + tail_symbols entries. */
 int dtl_cdf(dtl_session *session, size_t row, size_t tail_symbols, uint32_t *freq, uint64_t *cum,

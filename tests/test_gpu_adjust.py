@@ -10,8 +10,8 @@ import pytest
 HERE = Path(__file__).resolve().parent
 
 
-def run_apart(name):
-    p = subprocess.Popen([sys.executable, "-u", "-m", "pytest", str(HERE / name), "-x", "-v", "-p", "no:cacheprovider",
+def run_apart(name, *which):
+    p = subprocess.Popen([sys.executable, "-u", "-m", "pytest", str(HERE / name), *which, "-x", "-v", "-p", "no:cacheprovider",
                           "--timeout", "60", "--timeout-method", "thread"], cwd=HERE.parent, stdout=subprocess.PIPE,
                          stderr=subprocess.STDOUT, text=True)
     lines = []

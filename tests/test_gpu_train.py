@@ -13,3 +13,17 @@ def test_embeddings():
 @pytest.mark.gpu
 def test_gradient_norms_and_clipping():
     run_apart("torch_clip.py")
+
+
+@pytest.mark.gpu
+def test_the_operators_together():
+    run_apart("torch_together.py")
+
+
+@pytest.mark.gpu
+def test_other_modes():
+    run_apart("torch_more_modes.py")
+
+
+def test_other_modes_without_a_gpu():
+    run_apart("torch_more_modes.py", "-m", "not gpu")
