@@ -231,6 +231,10 @@ using namespace dtl;
 
 namespace {
 
+constexpr size_t kMostCount = (size_t)1 << 36;  // the pieces of one tensor fit a launch
+constexpr uint32_t kMostPieces = 0xffffffffu / kThreads;
+static_assert(kMostCount / kClipPiece <= kMostPieces, "fewer than 2^32 threads");
+
 size_t pieces_of(const dtl_tensor& t, size_t piece = kPiece) { return (t.count + piece - 1) / piece; }
 
 // The tensors' pieces; 0 with *st set for a list that is refused.
@@ -240,7 +244,7 @@ size_t check_tensors(const dtl_tensor* t, size_t n, int* st) {
   for (size_t i = 0; i < n && !*st; i++) {
     if (t[i].dtype != DTL_F32 && t[i].dtype != DTL_BF16 && t[i].dtype != DTL_F16)
       *st = DTL_ERR_INVALID_ARGUMENT;
-    else if (t[i].count > (size_t)1 << 37 || (pieces += pieces_of(t[i])) > (size_t)1 << 31)
+    else if (t[i].count > kMostCount || (pieces += pieces_of(t[i])) > (size_t)1 << 31)
       *st = DTL_ERR_SHAPE;
     else if (t[i].count && (!t[i].data || reinterpret_cast<uintptr_t>(t[i].data) % type_bytes(t[i].dtype)))
       *st = DTL_ERR_INVALID_ARGUMENT;
@@ -289,16 +293,16 @@ void in_launches(K& k, int most, size_t piece, const dtl_tensor* t, size_t n, Pu
   k.n = 0;
   for (size_t i = 0; i < n; i++) {
     if (!t[i].count) continue;
-    k.entry[k.n] = {static_cast<const char*>(t[i].data), (uint64_t)t[i].dtype << kTypeShift | t[i].count};
-    k.first[k.n] = pieces;
-    put(k.n++, i);
-    pieces += (uint32_t)pieces_of(t[i], piece);
-    // a launch has fewer than 2^32 threads
-    if (k.n == most || pieces >= (1u << 23)) {
+    const uint32_t more = (uint32_t)pieces_of(t[i], piece);
+    if (k.n == most || pieces > kMostPieces - more) {
       go(pieces);
       k.n = 0;
       pieces = 0;
     }
+    k.entry[k.n] = {static_cast<const char*>(t[i].data), (uint64_t)t[i].dtype << kTypeShift | t[i].count};
+    k.first[k.n] = pieces;
+    put(k.n++, i);
+    pieces += more;
   }
   if (k.n) go(pieces);
 }

@@ -174,13 +174,14 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
 
 // ---- launches ---------------------------------------------------------------------------
 
-// A launch of `per_row` workgroups a row; of many rows several, of as many as
-// keep the launch's threads below 2^32 (a row has 32 workgroups of 256 at most).
+// A launch of `per_row` workgroups a row; of many rows several, of as many as keep the
+// launch's threads below 2^32.
 constexpr size_t kRowsPerLaunch = 1u << 18;
 template <typename K>
 void launch_rows(void (*kernel)(K), size_t rows, int per_row, int threads, size_t lds, hipStream_t s, K k) {
-  for (k.row0 = 0; k.row0 < rows; k.row0 += kRowsPerLaunch) {
-    const size_t n = rows - k.row0 < kRowsPerLaunch ? rows - k.row0 : kRowsPerLaunch;
+  const size_t fit = 0xffffffffu / ((size_t)per_row * threads), most = fit < kRowsPerLaunch ? fit : kRowsPerLaunch;
+  for (k.row0 = 0; k.row0 < rows; k.row0 += most) {
+    const size_t n = rows - k.row0 < most ? rows - k.row0 : most;
     launch_kernel(kernel, dim3((unsigned)(n * per_row)), dim3(threads), lds, s, k);
   }
 }

@@ -118,6 +118,7 @@ def _beside(t: torch.Tensor, logits: torch.Tensor, shape, dtypes, name: str) -> 
 
 _INDEX = (torch.int64, torch.int32)
 _FLOAT = (torch.float32,)
+_MASK = (torch.int32, torch.bool)
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -320,67 +321,86 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
 # ---- penalties, biases, masks -------------------------------------------------------
 
 
-def _per_row(value, logits, name):
-    """A number, or a tensor with one for each row."""
-    if isinstance(value, torch.Tensor):
-        if value.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{name} is a constant to autograd: detach it")
-        return 0.0, _beside(value, logits, logits.shape[:-1], _FLOAT, name)
-    return float(value), None
-
-
-def _rows_or_shared(t, logits, last, dtypes, name):
-    """A tensor of the logits' leading dimensions, or of one dimension for every row."""
-    shared = isinstance(t, torch.Tensor) and t.dim() == 1
-    return _beside(t, logits, (last,) if shared else (*logits.shape[:-1], last), dtypes, name), 0 if shared else last
-
-
-def _last(t) -> int:
-    return t.shape[-1] if isinstance(t, torch.Tensor) and t.dim() else 0
-
-
 class _By:
     """A dtl_adjust and the tensors that it points to."""
 
     def __init__(self, logits, vocab, history, prompt, repetition, presence, frequency, bias_ids, bias, allowed):
         a = self.struct = _lib.Adjust()
-        lead = logits.shape[:-1]
-        rows = None
+        self.lead, self.device = logits.shape[:-1], logits.device
+        self.dual = getattr(forward_ad, "_current_level", 0) >= 0
+        rows = presences = frequencies = None
         if history is not None:
-            history, a.history_stride = _rows_or_shared(history, logits, _last(history), _INDEX, "history")
-            a.history, a.history_bytes, a.history_len = history.data_ptr(), history.element_size(), history.shape[-1]
+            history, n, a.history_stride = self.rows(history, _INDEX, "history")
+            a.history, a.history_bytes, a.history_len = history.data_ptr(), history.element_size(), n
             if prompt is not None:
-                prompt = _beside(prompt, logits, lead, _INDEX, "prompt").int()
+                prompt = self.tensor(prompt, _INDEX, "prompt", self.lead).int()
                 a.prompt = prompt.data_ptr()
         elif prompt is not None:
             raise ValueError("prompt counts places of a history")
-        a.repetition, rows = _per_row(repetition, logits, "repetition")
-        a.presence, presences = _per_row(presence, logits, "presence")
-        a.frequency, frequencies = _per_row(frequency, logits, "frequency")
-        a.repetitions, a.presences, a.frequencies = _ptr(rows), _ptr(presences), _ptr(frequencies)
+        if isinstance(repetition, torch.Tensor):
+            rows = self.constant(repetition, "repetition", self.lead)
+            a.repetitions = rows.data_ptr()
+        else:
+            a.repetition = repetition
+        if isinstance(presence, torch.Tensor):
+            presences = self.constant(presence, "presence", self.lead)
+            a.presences = presences.data_ptr()
+        else:
+            a.presence = presence
+        if isinstance(frequency, torch.Tensor):
+            frequencies = self.constant(frequency, "frequency", self.lead)
+            a.frequencies = frequencies.data_ptr()
+        else:
+            a.frequency = frequency
         if (bias_ids is None) != (bias is None):
             raise ValueError("bias_ids and bias belong together")
         if bias is not None:
-            if isinstance(bias, torch.Tensor) and bias.requires_grad and torch.is_grad_enabled():
-                raise ValueError("bias is a constant to autograd: detach it")
-            n = _last(bias_ids)
-            bias_ids, a.bias_stride = _rows_or_shared(bias_ids, logits, n, _INDEX, "bias_ids")
-            bias = _beside(bias, logits, bias_ids.shape, _FLOAT, "bias")
-            a.bias_ids, a.bias_bytes, a.bias_len = bias_ids.data_ptr(), bias_ids.element_size(), n
-            a.biases = bias.data_ptr()
+            bias_ids, a.bias_len, a.bias_stride = self.rows(bias_ids, _INDEX, "bias_ids")
+            bias = self.constant(bias, "bias", bias_ids.shape)
+            a.bias_ids, a.bias_bytes, a.biases = bias_ids.data_ptr(), bias_ids.element_size(), bias.data_ptr()
         if allowed is not None:
-            bits = isinstance(allowed, torch.Tensor) and allowed.dtype == torch.int32
-            allowed, a.allowed_stride = _rows_or_shared(allowed, logits, -(-vocab // 32) if bits else vocab,
-                                                        (torch.int32, torch.bool), "allowed")
-            a.allowed, a.allowed_bits = allowed.data_ptr(), 1 if bits else 8
+            allowed, n, a.allowed_stride = self.rows(allowed, _MASK, "allowed")
+            a.allowed_bits = 1 if allowed.dtype == torch.int32 else 8
+            if n != (vocab if a.allowed_bits == 8 else -(-vocab // 32)):
+                raise ValueError(f"allowed has {n} entries in a row, expected one for each logit or 32")
+            a.allowed = allowed.data_ptr()
         self.tensors = (history, prompt, rows, presences, frequencies, bias_ids, bias, allowed)
+
+    def tensor(self, t, dtypes, name, shape=None) -> torch.Tensor:
+        """As _beside; of any shape where none is given."""
+        if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
+            raise TypeError(f"{name} must be a tensor of {' or '.join(str(d) for d in dtypes)}")
+        if self.dual:
+            _no_tangent(t, name)
+        if t.device != self.device:
+            raise ValueError(f"{name} and logits are on different devices")
+        if shape is not None and t.shape != shape:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+        return t.contiguous()
+
+    def rows(self, t, dtypes, name):
+        """A tensor of the logits' leading dimensions and one more, or of one dimension for
+        every row; its row's length, and how far rows are apart."""
+        t = self.tensor(t, dtypes, name)
+        shape = t.shape
+        if len(shape) == 1:
+            return t, shape[0], 0
+        if not shape or shape[:-1] != self.lead:
+            raise ValueError(f"{name} has shape {tuple(shape)}, expected {(*self.lead, 'n')} or ('n',)")
+        return t, shape[-1], shape[-1]
+
+    def constant(self, t, name, shape):
+        t = self.tensor(t, _FLOAT, name, shape)
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} is a constant to autograd: detach it")
+        return t
 
     def for_backward(self):
         """What the gradient needs: whether a token stood in the history, and the mask."""
-        history, prompt, rows, _, _, _, _, allowed = self.tensors
-        if self.struct.repetition == 1.0 and rows is None:
-            history = None
-        return history, rows if history is not None else None, allowed
+        history, _, rows, _, _, _, _, allowed = self.tensors
+        if history is None or self.struct.repetition == 1.0 and rows is None:
+            return None, None, allowed
+        return history, rows, allowed
 
 
 def _adjust(z, by, out, stride, device):
@@ -389,15 +409,13 @@ def _adjust(z, by, out, stride, device):
 
 class _Adjust(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, by):
-        z = _logits_view(logits)
+    def forward(ctx, logits, z, by):
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         _adjust(z, by, out, z.vocab, logits.device)
         history, rows, allowed = by.for_backward()
         # without repetitions a logit's sign does not matter, only where it is
         ctx.save_for_backward(logits if history is not None else None, history, rows, allowed)
-        ctx.like = logits.shape, logits.dtype, logits.device
-        ctx.repetition = by.struct.repetition
+        ctx.by, ctx.like = by.struct, (logits.shape, logits.dtype, logits.device)
         return out
 
     @staticmethod
@@ -407,20 +425,20 @@ class _Adjust(torch.autograd.Function):
         shape, dtype, device = ctx.like
         g = _incoming(g)
         if history is None and allowed is None:
-            return g, None
+            return g, None, None
         grad = torch.empty(shape, dtype=dtype, device=device)
-        a = _lib.Adjust(repetition=ctx.repetition, repetitions=_ptr(rows))
+        a, V = _lib.Adjust(), shape[-1]
+        a.repetition = ctx.by.repetition
         if history is not None:
-            a.history, a.history_bytes, a.history_len = history.data_ptr(), history.element_size(), history.shape[-1]
-            a.history_stride = history.shape[-1] if history.dim() > 1 or len(shape) == 1 else 0
+            a.history, a.history_bytes = history.data_ptr(), ctx.by.history_bytes
+            a.history_len, a.history_stride = ctx.by.history_len, ctx.by.history_stride
+            a.repetitions = _ptr(rows)
         if allowed is not None:
-            a.allowed, a.allowed_bits = allowed.data_ptr(), 1 if allowed.dtype == torch.int32 else 8
-            a.allowed_stride = allowed.shape[-1] if allowed.dim() > 1 or len(shape) == 1 else 0
-        V = shape[-1]
+            a.allowed, a.allowed_bits, a.allowed_stride = allowed.data_ptr(), ctx.by.allowed_bits, ctx.by.allowed_stride
         gv = _lib.Logits(g.data_ptr(), _DTYPES[dtype], g.numel() // V, V, V)
         z = gv if logits is None else _logits_view(logits)
         _call(device, lib.dtl_adjust_logits_backward, C.byref(z), C.byref(a), gv.data, V, grad.data_ptr(), V)
-        return grad, None
+        return grad, None, None
 
 
 def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None, prompt: Optional[torch.Tensor] = None,
@@ -448,7 +466,7 @@ def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = Non
     grad = torch.is_grad_enabled() and logits.requires_grad
     if out is None:
         if grad:
-            return _Adjust.apply(logits, by)
+            return _Adjust.apply(logits, z, by)
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         _adjust(z, by, out, z.vocab, logits.device)
         return out

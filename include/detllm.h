@@ -450,7 +450,7 @@ int dtl_embedding_backward(const void *tokens, int token_bytes, size_t n, const 
                            int grad_dtype, size_t grad_out_stride, float scale, const dtl_table *grad,
                            int add, void *scratch, size_t scratch_bytes, void *stream);
 
-/* `count` elements in device memory, aligned to an element. */
+/* `count` (<= 2^36) elements in device memory, aligned to an element. */
 typedef struct dtl_tensor {
     void *data;
     size_t count;

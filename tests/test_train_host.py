@@ -88,7 +88,7 @@ def clip(t, n=None, out=None, max_norm=1.0, norm=P, scratch=1 << 36, scratch_byt
 def test_tensor_lists():
     good = (G, 100, 0)
     for bad, status in (((G, 100, 3), INVALID), ((0, 100, 0), INVALID), ((G + 2, 100, 0), INVALID), ((G + 1, 100, 1), INVALID),
-                        ((G, (1 << 37) + 1, 0), SHAPE)):
+                        ((G, (1 << 36) + 1, 0), SHAPE)):
         assert clip(tensors((Q, 5, 0), bad)) == status
     assert clip(tensors(good), n=(1 << 16) + 1) == SHAPE
     assert clip(tensors(good), norm=0) == INVALID
@@ -112,7 +112,7 @@ def test_norm_scratch():
 
     t = tensors((G, 1 << 30, 0), (Q, 0, 1), (Q, 1, 2))
     assert lib.dtl_grad_norm_scratch(t.buffer_info()[0], 3) >= ((1 << 30) // 65536) * 8
-    assert lib.dtl_grad_norm_scratch(tensors((G, 1 << 38, 0)).buffer_info()[0], 1) == 0
+    assert lib.dtl_grad_norm_scratch(tensors((G, 1 << 37, 0)).buffer_info()[0], 1) == 0
     assert lib.dtl_grad_norm_scratch(None, 0) >= 4
 
 
