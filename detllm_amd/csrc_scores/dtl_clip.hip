@@ -24,6 +24,11 @@ constexpr int kThreads = 256, kJoinThreads = 1024;
 // elements: norm by 16384 / 32768 332 / 338, but 31 / 17 to join twice the pieces; clipping
 // by 8192 / 16384 / 32768 769 / 795 / 804.
 constexpr size_t kPiece = 32768, kClipPiece = 8192;
+// Workgroups of a clipping in place at most: with a factor of 1 there is nothing to do, and
+// ending the 133000 of 201 bf16 tensors takes 90 us longer; with another one their pieces
+// one after the other take 1180 us instead of 1140.
+constexpr uint32_t kInPlaceGroups = 16384;
+constexpr size_t kCache = (size_t)256 << 20, kKept = (size_t)192 << 20;
 constexpr int kNormEntries = 180, kClipEntries = 128;
 
 struct Entry {
@@ -39,7 +44,8 @@ struct NormK {
   Entry entry[kNormEntries];
   uint32_t first[kNormEntries];  // each tensor's first piece of the launch
   int n;
-  uint32_t slot0;  // of the launch's first piece among all
+  uint32_t slot0;      // of the launch's first piece among all
+  uint32_t keep_from;  // pieces from here on are left in the caches
   double* part;
 };
 struct ClipK {
@@ -47,6 +53,9 @@ struct ClipK {
   char* out[kClipEntries];
   uint32_t first[kClipEntries];
   int n;
+  uint32_t pieces;
+  bool past;  // written past the caches
+  bool in_place;
   const float* factor;
 };
 static_assert(sizeof(NormK) <= 4096 && sizeof(ClipK) <= 4096, "fit a kernel's arguments");
@@ -104,24 +113,28 @@ __device__ __forceinline__ double piece_of(const char* x, uint64_t count, uint64
 // Whichever is larger, NaN above all.
 __device__ __forceinline__ double larger(double a, double b) { return !(a == a) || a > b ? a : b; }
 
-// ONCE: read past the caches.
 template <bool LARGEST, bool ONCE>
+__device__ __forceinline__ double piece_of(const Entry& t, uint64_t at) {
+  switch (type_of(t)) {
+    case DTL_F32: return piece_of<DTL_F32, LARGEST, ONCE>(t.x, count_of(t), at);
+    case DTL_BF16: return piece_of<DTL_BF16, LARGEST, ONCE>(t.x, count_of(t), at);
+    default: return piece_of<DTL_F16, LARGEST, ONCE>(t.x, count_of(t), at);
+  }
+}
+
+template <bool LARGEST>
 __global__ __launch_bounds__(kThreads) void k_norm(NormK a) {
   __shared__ double waves[kThreads / 64];
   const int e = find(a, blockIdx.x);
   const Entry t = a.entry[e];
   const uint64_t at = (uint64_t)(blockIdx.x - a.first[e]) * kPiece;
-  double v = 0.0;
-  switch (type_of(t)) {
-    case DTL_F32: v = piece_of<DTL_F32, LARGEST, ONCE>(t.x, count_of(t), at); break;
-    case DTL_BF16: v = piece_of<DTL_BF16, LARGEST, ONCE>(t.x, count_of(t), at); break;
-    default: v = piece_of<DTL_F16, LARGEST, ONCE>(t.x, count_of(t), at);
-  }
+  const uint32_t slot = a.slot0 + blockIdx.x;
+  double v = slot < a.keep_from ? piece_of<LARGEST, true>(t, at) : piece_of<LARGEST, false>(t, at);
   if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
   __syncthreads();
   if (threadIdx.x) return;
   for (int w = 1; w < kThreads / 64; w++) v = LARGEST ? larger(waves[w], v) : v + waves[w];
-  a.part[a.slot0 + blockIdx.x] = v;
+  a.part[slot] = v;
 }
 
 struct JoinK {
@@ -164,7 +177,8 @@ __global__ __launch_bounds__(kJoinThreads) void k_norm_join(JoinK a) {
 // A lane's stores are 16 bytes and next to its neighbours', so of 16-bit elements that
 // become f32 it reads 8.
 template <int DT, int OUT>
-__device__ __forceinline__ void scale_piece(const char* x, char* y, uint64_t count, uint64_t at, float f) {
+__device__ __forceinline__ void scale_piece(const char* x, char* y, uint64_t count, uint64_t at, float f,
+                                            bool past) {
   constexpr int n = Type<OUT>::kInPacket, ahead = 4;
   typedef uint32_t half __attribute__((ext_vector_type(2)));
   typedef half half2 __attribute__((aligned(2)));
@@ -191,7 +205,7 @@ __device__ __forceinline__ void scale_piece(const char* x, char* y, uint64_t cou
       for (int q = 0; q < 4; q++)
         w[q] = OUT == DTL_F32 ? bits_of<OUT>(value<DT>(p[k], q) * f)
                               : bits_of<OUT>(value<DT>(p[k], 2 * q % n) * f) | bits_of<OUT>(value<DT>(p[k], (2 * q + 1) % n) * f) << 16;
-      *reinterpret_cast<out_mem*>(y + (size_t)(j + k * kThreads * n) * Type<OUT>::kBytes) = w;
+      store_packet(reinterpret_cast<out_mem*>(y + (size_t)(j + k * kThreads * n) * Type<OUT>::kBytes), w, past);
     }
   }
   for (; j < left; j += kThreads * n)
@@ -200,25 +214,27 @@ __device__ __forceinline__ void scale_piece(const char* x, char* y, uint64_t cou
 
 __global__ __launch_bounds__(kThreads) void k_clip(ClipK a) {
   const float f = *a.factor;
-  const uint32_t piece = gridDim.x - 1 - blockIdx.x;  // what the norm read last may still be in the cache
-  const int e = find(a, piece);
-  const Entry t = a.entry[e];
-  const uint64_t at = (uint64_t)(piece - a.first[e]) * kClipPiece;
-  char* y = a.out[e];
-  if (f == 1.0f && y == t.x) return;
-  switch (type_of(t)) {
-    case DTL_F32: scale_piece<DTL_F32, DTL_F32>(t.x, y, count_of(t), at, f); break;
-    case DTL_BF16:
-      if (wide_of(t))
-        scale_piece<DTL_BF16, DTL_F32>(t.x, y, count_of(t), at, f);
-      else
-        scale_piece<DTL_BF16, DTL_BF16>(t.x, y, count_of(t), at, f);
-      break;
-    default:
-      if (wide_of(t))
-        scale_piece<DTL_F16, DTL_F32>(t.x, y, count_of(t), at, f);
-      else
-        scale_piece<DTL_F16, DTL_F16>(t.x, y, count_of(t), at, f);
+  if (f == 1.0f && a.in_place) return;
+  for (uint32_t piece = blockIdx.x; piece < a.pieces; piece += gridDim.x) {
+    const int e = find(a, piece);
+    const Entry t = a.entry[e];
+    // what the norm read last may still be in the cache: backwards
+    const uint64_t last = (count_of(t) - 1) / kClipPiece, at = (last - (piece - a.first[e])) * kClipPiece;
+    char* y = a.out[e];
+    switch (type_of(t)) {
+      case DTL_F32: scale_piece<DTL_F32, DTL_F32>(t.x, y, count_of(t), at, f, a.past); break;
+      case DTL_BF16:
+        if (wide_of(t))
+          scale_piece<DTL_BF16, DTL_F32>(t.x, y, count_of(t), at, f, a.past);
+        else
+          scale_piece<DTL_BF16, DTL_BF16>(t.x, y, count_of(t), at, f, a.past);
+        break;
+      default:
+        if (wide_of(t))
+          scale_piece<DTL_F16, DTL_F32>(t.x, y, count_of(t), at, f, a.past);
+        else
+          scale_piece<DTL_F16, DTL_F16>(t.x, y, count_of(t), at, f, a.past);
+    }
   }
 }
 
@@ -286,12 +302,14 @@ int check_out(const dtl_tensor* t, const dtl_tensor* out, size_t n) {
   return DTL_OK;
 }
 
-// Cuts the list into launches of at most `most` tensors that have elements.
+// Cuts the list, or the list backwards, into launches of at most `most` tensors that
+// have elements.
 template <typename K, typename Put, typename Go>
-void in_launches(K& k, int most, size_t piece, const dtl_tensor* t, size_t n, Put&& put, Go&& go) {
+void in_launches(K& k, int most, size_t piece, bool back, const dtl_tensor* t, size_t n, Put&& put, Go&& go) {
   uint32_t pieces = 0;
   k.n = 0;
-  for (size_t i = 0; i < n; i++) {
+  for (size_t j = 0; j < n; j++) {
+    const size_t i = back ? n - 1 - j : j;
     if (!t[i].count) continue;
     const uint32_t more = (uint32_t)pieces_of(t[i], piece);
     if (k.n == most || pieces > kMostPieces - more) {
@@ -324,15 +342,27 @@ int norm_and_clip(const dtl_tensor* t, size_t n, int largest, float scale, const
   float* factor = static_cast<float*>(scratch);
   NormK k{};
   k.part = reinterpret_cast<double*>(static_cast<char*>(scratch) + 16);
-  // More than the memory-side cache holds is read past it, if not all of it is read again
-  // (201 bf16 tensors, 2.2 GB: 324 us, 395 with it); what it holds stays for the clipping.
+  // More than the memory-side cache holds is read past it, but for what the clipping,
+  // which goes backwards and writes past it, will still find there (kKept; us for norm and
+  // clipping, 0 / 128 / 192 MB kept: 201 bf16 tensors of 2.2 GB 1091 / 1108 / 1076, cached
+  // throughout 1219; 392 MB of f16 to f32 265 / 285 / 249).
   size_t bytes = 0;
   for (size_t i = 0; i < n; i++) bytes += t[i].count * type_bytes(t[i].dtype);
-  const bool once = bytes > (size_t)256 << 20;
-  in_launches(k, kNormEntries, kPiece, t, n, [](int, size_t) {}, [&](uint32_t count) {
-    void (*const kernel)(NormK) = largest ? once ? k_norm<true, true> : k_norm<true, false>
-                                          : once ? k_norm<false, true> : k_norm<false, false>;
-    launch_kernel(kernel, dim3(count), dim3(kThreads), 0, s, k);
+  if (bytes > kCache) {
+    size_t keep = 0, left = clip ? kKept : 0;
+    for (size_t i = n; i-- && left;) {
+      const size_t piece = kPiece * type_bytes(t[i].dtype), fit = left / piece;
+      if (pieces_of(t[i]) >= fit) {
+        keep += fit;
+        break;
+      }
+      keep += pieces_of(t[i]);
+      left -= pieces_of(t[i]) * piece;
+    }
+    k.keep_from = (uint32_t)(pieces - keep);
+  }
+  in_launches(k, kNormEntries, kPiece, false, t, n, [](int, size_t) {}, [&](uint32_t count) {
+    launch_kernel(largest ? k_norm<true> : k_norm<false>, dim3(count), dim3(kThreads), 0, s, k);
     k.slot0 += count;
   });
   JoinK j{k.part, (uint32_t)pieces, clip, scale, max_norm, scale_at, norm, factor};
@@ -340,14 +370,19 @@ int norm_and_clip(const dtl_tensor* t, size_t n, int largest, float scale, const
   if (clip) {
     ClipK c{};
     c.factor = factor;
+    c.past = bytes > kCache;
+    c.in_place = out == nullptr;
     const dtl_tensor* to = out ? out : t;
     in_launches(
-        c, kClipEntries, kClipPiece, t, n,
+        c, kClipEntries, kClipPiece, true, t, n,
         [&](int e, size_t i) {
           c.out[e] = static_cast<char*>(to[i].data);
           if (to[i].dtype == DTL_F32) c.entry[e].bits |= (uint64_t)1 << kWideShift;
         },
-        [&](uint32_t count) { launch_kernel(k_clip, dim3(count), dim3(kThreads), 0, s, c); });
+        [&](uint32_t count) {
+          c.pieces = count;
+          launch_kernel(k_clip, dim3(c.in_place && count > kInPlaceGroups ? kInPlaceGroups : count), dim3(kThreads), 0, s, c);
+        });
   }
   return launch_status();
 }
