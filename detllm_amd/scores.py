@@ -321,6 +321,14 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
 # ---- penalties, biases, masks -------------------------------------------------------
 
 
+def _spaced(t):
+    """A tensor whose rows are used as they lie, and how far they are apart (0: one for all):
+    the first places of a longer buffer are not copied."""
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t, t.stride(0)
+    return t.contiguous(), 0 if t.dim() == 1 else t.shape[-1]
+
+
 class _By:
     """A dtl_adjust and the tensors that it points to."""
 
@@ -333,7 +341,7 @@ class _By:
             history, n, a.history_stride = self.rows(history, _INDEX, "history")
             a.history, a.history_bytes, a.history_len = history.data_ptr(), history.element_size(), n
             if prompt is not None:
-                prompt = self.tensor(prompt, _INDEX, "prompt", self.lead).int()
+                prompt = self.tensor(prompt, _INDEX, "prompt", self.lead).int().contiguous()
                 a.prompt = prompt.data_ptr()
         elif prompt is not None:
             raise ValueError("prompt counts places of a history")
@@ -341,22 +349,24 @@ class _By:
             rows = self.constant(repetition, "repetition", self.lead)
             a.repetitions = rows.data_ptr()
         else:
-            a.repetition = repetition
+            a.repetition = float(repetition)
         if isinstance(presence, torch.Tensor):
             presences = self.constant(presence, "presence", self.lead)
             a.presences = presences.data_ptr()
         else:
-            a.presence = presence
+            a.presence = float(presence)
         if isinstance(frequency, torch.Tensor):
             frequencies = self.constant(frequency, "frequency", self.lead)
             a.frequencies = frequencies.data_ptr()
         else:
-            a.frequency = frequency
+            a.frequency = float(frequency)
         if (bias_ids is None) != (bias is None):
             raise ValueError("bias_ids and bias belong together")
         if bias is not None:
-            bias_ids, a.bias_len, a.bias_stride = self.rows(bias_ids, _INDEX, "bias_ids")
-            bias = self.constant(bias, "bias", bias_ids.shape)
+            bias = self.constant(bias, "bias", bias_ids.shape if isinstance(bias_ids, torch.Tensor) else None)
+            bias_ids, a.bias_len, _ = self.rows(bias_ids, _INDEX, "bias_ids")
+            bias_ids = bias_ids.contiguous()  # one spacing for both
+            a.bias_stride = 0 if bias_ids.dim() == 1 else a.bias_len
             a.bias_ids, a.bias_bytes, a.biases = bias_ids.data_ptr(), bias_ids.element_size(), bias.data_ptr()
         if allowed is not None:
             allowed, n, a.allowed_stride = self.rows(allowed, _MASK, "allowed")
@@ -376,24 +386,22 @@ class _By:
             raise ValueError(f"{name} and logits are on different devices")
         if shape is not None and t.shape != shape:
             raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-        return t.contiguous()
+        return t
 
     def rows(self, t, dtypes, name):
         """A tensor of the logits' leading dimensions and one more, or of one dimension for
         every row; its row's length, and how far rows are apart."""
-        t = self.tensor(t, dtypes, name)
-        shape = t.shape
-        if len(shape) == 1:
-            return t, shape[0], 0
-        if not shape or shape[:-1] != self.lead:
+        shape = self.tensor(t, dtypes, name).shape
+        if len(shape) != 1 and (not shape or shape[:-1] != self.lead):
             raise ValueError(f"{name} has shape {tuple(shape)}, expected {(*self.lead, 'n')} or ('n',)")
-        return t, shape[-1], shape[-1]
+        t, stride = _spaced(t)
+        return t, shape[-1], stride
 
     def constant(self, t, name, shape):
         t = self.tensor(t, _FLOAT, name, shape)
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} is a constant to autograd: detach it")
-        return t
+        return t.contiguous()
 
     def for_backward(self):
         """What the gradient needs: whether a token stood in the history, and the mask."""
@@ -415,7 +423,7 @@ class _Adjust(torch.autograd.Function):
         history, rows, allowed = by.for_backward()
         # without repetitions a logit's sign does not matter, only where it is
         ctx.save_for_backward(logits if history is not None else None, history, rows, allowed)
-        ctx.by, ctx.like = by.struct, (logits.shape, logits.dtype, logits.device)
+        ctx.repetition, ctx.like = by.struct.repetition, (logits.shape, logits.dtype, logits.device)
         return out
 
     @staticmethod
@@ -428,13 +436,14 @@ class _Adjust(torch.autograd.Function):
             return g, None, None
         grad = torch.empty(shape, dtype=dtype, device=device)
         a, V = _lib.Adjust(), shape[-1]
-        a.repetition = ctx.by.repetition
+        a.repetition = ctx.repetition
         if history is not None:
-            a.history, a.history_bytes = history.data_ptr(), ctx.by.history_bytes
-            a.history_len, a.history_stride = ctx.by.history_len, ctx.by.history_stride
+            history, a.history_stride = _spaced(history)
+            a.history, a.history_bytes, a.history_len = history.data_ptr(), history.element_size(), history.shape[-1]
             a.repetitions = _ptr(rows)
         if allowed is not None:
-            a.allowed, a.allowed_bits, a.allowed_stride = allowed.data_ptr(), ctx.by.allowed_bits, ctx.by.allowed_stride
+            allowed, a.allowed_stride = _spaced(allowed)
+            a.allowed, a.allowed_bits = allowed.data_ptr(), 8 if allowed.dtype == torch.bool else 1
         gv = _lib.Logits(g.data_ptr(), _DTYPES[dtype], g.numel() // V, V, V)
         z = gv if logits is None else _logits_view(logits)
         _call(device, lib.dtl_adjust_logits_backward, C.byref(z), C.byref(a), gv.data, V, grad.data_ptr(), V)

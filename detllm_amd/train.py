@@ -28,7 +28,7 @@ from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import DetllmError, lib
-from .scores import _DTYPES, _INDEX, _call, _incoming, _no_tangent, _ptr, _scratch, _tracing
+from .scores import _DTYPES, _INDEX, _call, _no_tangent, _ptr, _scratch, _tracing
 
 MAX_TOKENS = 1 << 20  # of an embedding's gradient
 
@@ -79,10 +79,14 @@ def _lookup(weight, tokens, scale):
 
 def _gradient(tokens, grad, scale, out, add):
     g, n = _table(out, "out"), tokens.numel()
+    if grad.dim() == 2 and grad.stride(1) == 1 and grad.stride(0) >= g.width:  # rows of a wider tensor are not copied
+        spacing = grad.stride(0)
+    else:
+        grad, spacing = grad.contiguous(), g.width
     need = _embed_scratch(n, g.vocab, g.width)
     scratch = _scratch(need, out.device)
     _call(out.device, lib.dtl_embedding_backward, _ptr(tokens), tokens.element_size(), n, _ptr(grad), _DTYPES[grad.dtype],
-          g.width, scale, C.byref(g), int(add), _ptr(scratch), need)
+          spacing, scale, C.byref(g), int(add), _ptr(scratch), need)
     return out
 
 
@@ -98,7 +102,8 @@ class _Embedding(torch.autograd.Function):
     def backward(ctx, g):
         tokens, = ctx.saved_tensors
         shape, dtype, device = ctx.like
-        return _gradient(tokens, _incoming(g), ctx.scale, torch.empty(shape, dtype=dtype, device=device), False), None, None
+        _no_tangent(g, "the gradient")
+        return _gradient(tokens, g, ctx.scale, torch.empty(shape, dtype=dtype, device=device), False), None, None
 
 
 def embedding(weight: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.0) -> torch.Tensor:
@@ -124,7 +129,6 @@ def embedding_grad(tokens: torch.Tensor, grad: torch.Tensor, vocab: Optional[int
     tokens = _token_ids(tokens, grad.device)
     if not grad.dim() or grad.shape[:-1] != tokens.shape:
         raise ValueError(f"grad has shape {tuple(grad.shape)}, expected {(*tokens.shape, 'width')}")
-    grad = grad.contiguous()
     if out is None:
         if vocab is None or add:
             raise ValueError("embedding_grad needs a vocab or an out, and out for add")

@@ -172,6 +172,37 @@ def test_out_between_the_rows_and_into_another_tensor():
         scores.adjust_logits(both.view(12, 3001)[:6], **kw, out=both.view(12, 3001)[3:9])
 
 
+def test_parts_of_longer_buffers():
+    """The first places of a history that grows, masks and biases cut from wider ones,
+    one row for all by expand: as their copies, forward and backward."""
+    z, kw, rows = case(12, 6, 3000, "bf16", 500, 20, "bits", per_row=True)
+
+    def wider(t, n):
+        buf = torch.full((*t.shape[:-1], t.shape[-1] + n), 1, dtype=t.dtype, device=DEV)
+        buf[..., n // 2:n // 2 + t.shape[-1]] = t
+        return buf[..., n // 2:n // 2 + t.shape[-1]]
+
+    cut = {k: wider(v, 14) if v.dim() == 2 else torch.stack([v, v], 1)[:, 1] for k, v in kw.items()}
+    assert not any(v.is_contiguous() for v in cut.values())
+    first = {k: v[:1] for k, v in kw.items()}
+    alike = {k: v.expand(6, *v.shape[1:]) for k, v in first.items()}
+    copied = {k: v.contiguous() for k, v in alike.items()}
+    for a, b in ((cut, kw), (alike, copied)):
+        leaf = z.clone().requires_grad_()
+        got = [scores.adjust_logits(leaf, **x) for x in (a, b)]
+        assert torch.equal(*got)
+        g = torch.randn_like(got[0])
+        assert torch.equal(*(torch.autograd.grad(x, leaf, g)[0] for x in got))
+        with torch.autograd.graph.save_on_cpu():
+            moved = scores.adjust_logits(leaf, **a)
+        assert torch.equal(torch.autograd.grad(moved, leaf, g)[0], torch.autograd.grad(scores.adjust_logits(leaf, **b), leaf, g)[0])
+    three = {k: v[:, None].expand(6, 2, *v.shape[1:]) for k, v in kw.items()}
+    got = scores.adjust_logits(z[:, None].expand(6, 2, 3000).contiguous(), **three)
+    assert torch.equal(got[:, 0], got[:, 1]) and torch.equal(got[:, 0], scores.adjust_logits(z, **kw))
+    assert torch.equal(scores.adjust_logits(z, history=kw["history"], repetition=np.float32(1.5)),
+                       scores.adjust_logits(z, history=kw["history"], repetition=1.5))
+
+
 def test_nothing_to_do_copies():
     z = torch.randn(3, 100, device=DEV)
     for kw in ({}, dict(history=torch.zeros(3, 5, dtype=torch.long, device=DEV)),

@@ -86,6 +86,12 @@ def test_leading_shapes_and_strides():
     out = torch.full((100, 33), 9.0, device=DEV).bfloat16()
     train.embedding_grad(tokens, g, out=out[:, 5:25])
     assert torch.equal(out[:, 5:25], train.embedding_grad(tokens, g, 100)) and (out[:, :5] == 9).all() and (out[:, 25:] == 9).all()
+    wider = torch.randn(24, 31, device=DEV).bfloat16()
+    leaf = w.clone().requires_grad_()
+    for x in (wider[:, 3:23], wider[:, :20], wider[:1, 5:25].expand(24, 20)):
+        want = train.embedding_grad(tokens, x.contiguous(), 100)
+        assert torch.equal(train.embedding_grad(tokens, x, 100), want)
+        assert torch.equal(torch.autograd.grad(train.embedding(leaf, tokens), leaf, x)[0], want)
     every_other = torch.randn(24, 40, device=DEV).bfloat16()[:, ::2]
     assert torch.equal(train.embedding_grad(tokens, every_other, 100), train.embedding_grad(tokens, every_other.contiguous(), 100))
 
