@@ -24,7 +24,7 @@ the same for this library's own sessions, without torch.
 from __future__ import annotations
 
 import ctypes as C
-from functools import lru_cache
+from functools import lru_cache, wraps
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -415,6 +415,17 @@ def _adjust(z, by, out, stride, device):
     _call(device, lib.dtl_adjust_logits, C.byref(z), C.byref(by.struct), out.data_ptr(), stride)
 
 
+def _once(backward):
+    """once_differentiable, without its wrapper where no second derivative can follow."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    @wraps(backward)
+    def run(ctx, g):
+        return guarded(ctx, g) if torch.is_grad_enabled() else backward(ctx, g)
+
+    return run
+
+
 class _Adjust(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, z, by):
@@ -423,18 +434,18 @@ class _Adjust(torch.autograd.Function):
         history, rows, allowed = by.for_backward()
         # without repetitions a logit's sign does not matter, only where it is
         ctx.save_for_backward(logits if history is not None else None, history, rows, allowed)
-        ctx.repetition, ctx.like = by.struct.repetition, (logits.shape, logits.dtype, logits.device)
+        ctx.repetition = by.struct.repetition
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g):
         logits, history, rows, allowed = ctx.saved_tensors
-        shape, dtype, device = ctx.like
         g = _incoming(g)
         if history is None and allowed is None:
             return g, None, None
-        grad = torch.empty(shape, dtype=dtype, device=device)
+        shape = g.shape
+        grad = g.new_empty(shape)
         a, V = _lib.Adjust(), shape[-1]
         a.repetition = ctx.repetition
         if history is not None:
@@ -444,9 +455,9 @@ class _Adjust(torch.autograd.Function):
         if allowed is not None:
             allowed, a.allowed_stride = _spaced(allowed)
             a.allowed, a.allowed_bits = allowed.data_ptr(), 8 if allowed.dtype == torch.bool else 1
-        gv = _lib.Logits(g.data_ptr(), _DTYPES[dtype], g.numel() // V, V, V)
+        gv = _lib.Logits(g.data_ptr(), _DTYPES[g.dtype], g.numel() // V, V, V)
         z = gv if logits is None else _logits_view(logits)
-        _call(device, lib.dtl_adjust_logits_backward, C.byref(z), C.byref(a), gv.data, V, grad.data_ptr(), V)
+        _call(g.device, lib.dtl_adjust_logits_backward, C.byref(z), C.byref(a), gv.data, V, grad.data_ptr(), V)
         return grad, None, None
 
 

@@ -28,7 +28,7 @@ from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import DetllmError, lib
-from .scores import _DTYPES, _INDEX, _call, _no_tangent, _ptr, _scratch, _tracing
+from .scores import _DTYPES, _INDEX, _call, _no_tangent, _once, _ptr, _tracing
 
 MAX_TOKENS = 1 << 20  # of an embedding's gradient
 
@@ -84,7 +84,7 @@ def _gradient(tokens, grad, scale, out, add):
     else:
         grad, spacing = grad.contiguous(), g.width
     need = _embed_scratch(n, g.vocab, g.width)
-    scratch = _scratch(need, out.device)
+    scratch = out.new_empty(need, dtype=torch.uint8)
     _call(out.device, lib.dtl_embedding_backward, _ptr(tokens), tokens.element_size(), n, _ptr(grad), _DTYPES[grad.dtype],
           spacing, scale, C.byref(g), int(add), _ptr(scratch), need)
     return out
@@ -94,16 +94,15 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, tokens, scale):
         ctx.save_for_backward(tokens)
-        ctx.like, ctx.scale = (weight.shape, weight.dtype, weight.device), scale
+        ctx.shape, ctx.scale = weight.shape, scale
         return _lookup(weight, tokens, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g):
         tokens, = ctx.saved_tensors
-        shape, dtype, device = ctx.like
         _no_tangent(g, "the gradient")
-        return _gradient(tokens, g, ctx.scale, torch.empty(shape, dtype=dtype, device=device), False), None, None
+        return _gradient(tokens, g, ctx.scale, g.new_empty(ctx.shape), False), None, None
 
 
 def embedding(weight: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.0) -> torch.Tensor:
@@ -238,9 +237,9 @@ def _norm(grads, norm_type, scale, max_norm=None, out=None):
                 if o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()):
                     raise ValueError("out must have the gradients' strides")
     address = table.buffer_info()[0]
-    norm = torch.empty((), dtype=torch.float32, device=device)
+    norm = grads[0].new_empty((), dtype=torch.float32)
     need = lib.dtl_grad_norm_scratch(address, len(grads))
-    scratch = _scratch(need, device)
+    scratch = grads[0].new_empty(need, dtype=torch.uint8)
     kind = int(norm_type == math.inf)
     if max_norm is None:
         _call(device, lib.dtl_grad_norm, address, len(grads), kind, scale, at, _ptr(norm), _ptr(scratch), need)
