@@ -104,7 +104,6 @@ __device__ __forceinline__ uint32_t by_die(uint32_t block, uint32_t blocks) {
 
 template <int DT, int MODE, bool TABLE, int SEG, int kThreads>
 __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
-  typedef typename Type<DT>::mem mem;
   constexpr int n = Type<DT>::kInPacket, np = SEG / (kThreads * n), kHistory = 4;
   constexpr uint32_t no = MODE == GRAD ? 0u : Type<DT>::kMasked;
   static_assert(np * kThreads * n == SEG, "whole packets");
@@ -136,7 +135,7 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
     bits[i] = ~0u;
     if (j < end) {
       if (masked) bits[i] = allowed_bits<DT>(a, row, j, min(n, end - j));
-      if (MODE != IN_PLACE) p[i] = load_packet<DT>(from, j, end);
+      if (MODE != IN_PLACE) p[i] = load_packet_at_once<DT>(from, j, end);
     }
   }
 
@@ -203,7 +202,7 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
       for (int k = 0; k < 4; k++) hits[i] |= w[k] ? 1u << (q + k) : 0u;
     }
     hits[i] &= bits[i];
-    if (MODE == GRAD && hits[i]) sign[i] = load_packet<DT>(a.z + row * a.z_bytes, base + at, end);
+    if (MODE == GRAD && hits[i]) sign[i] = load_packet_at_once<DT>(a.z + row * a.z_bytes, base + at, end);
   }
 
 #pragma unroll
@@ -220,7 +219,7 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
         for (uint32_t off = all & ~on; off; off &= off - 1) store_one<DT>(out, j + __builtin_ctz(off), -__builtin_inff());
         continue;
       }
-      p[i] = on ? load_packet<DT>(from, j, end) : packet{no, no, no, no};
+      p[i] = on ? load_packet_at_once<DT>(from, j, end) : packet{no, no, no, no};
     }
     packet w = blend<DT>(p[i], bits[i], no);
     for (uint32_t h = hits[i]; h; h &= h - 1) {
@@ -238,7 +237,7 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
       put<DT>(w, q, v);
     }
     if (here == n) {
-      store_packet(reinterpret_cast<mem*>(out + (size_t)j * Type<DT>::kBytes), w, a.past);
+      store_packet<DT>(out + (size_t)j * Type<DT>::kBytes, w, a.past);
     } else {
 #pragma unroll
       for (int q = 0; q < n; q++)

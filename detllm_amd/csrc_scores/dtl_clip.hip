@@ -183,7 +183,6 @@ __device__ __forceinline__ void scale_piece(const char* x, char* y, uint64_t cou
   typedef uint32_t half __attribute__((ext_vector_type(2)));
   typedef half half2 __attribute__((aligned(2)));
   typedef std::conditional_t<DT == OUT, typename Type<DT>::mem, half2> mem;
-  typedef typename Type<OUT>::mem out_mem;
   const int tid = threadIdx.x, left = (int)(count - at < kClipPiece ? count - at : kClipPiece);
   x += at * Type<DT>::kBytes;
   y += at * Type<OUT>::kBytes;
@@ -205,7 +204,7 @@ __device__ __forceinline__ void scale_piece(const char* x, char* y, uint64_t cou
       for (int q = 0; q < 4; q++)
         w[q] = OUT == DTL_F32 ? bits_of<OUT>(value<DT>(p[k], q) * f)
                               : bits_of<OUT>(value<DT>(p[k], 2 * q % n) * f) | bits_of<OUT>(value<DT>(p[k], (2 * q + 1) % n) * f) << 16;
-      store_packet(reinterpret_cast<out_mem*>(y + (size_t)(j + k * kThreads * n) * Type<OUT>::kBytes), w, past);
+      store_packet<OUT>(y + (size_t)(j + k * kThreads * n) * Type<OUT>::kBytes, w, past);
     }
   }
   for (; j < left; j += kThreads * n)

@@ -78,10 +78,35 @@ __device__ __forceinline__ packet load_packet(const char* row, int j, int V) {
   return p;
 }
 
+// The same by loads that do not wait for each other: every element's, the last one's in
+// place of those past V.  V > j.
+template <int DT>
+__device__ __forceinline__ packet load_packet_at_once(const char* row, int j, int V) {
+  constexpr int n = Type<DT>::kInPacket;
+  if (j + n <= V) return *reinterpret_cast<const typename Type<DT>::mem*>(row + (size_t)j * Type<DT>::kBytes);
+  packet p;
+  uint32_t e[n];
+#pragma unroll
+  for (int q = 0; q < n; q++) {
+    const int at = min(j + q, V - 1);
+    if constexpr (DT == DTL_F32)
+      e[q] = reinterpret_cast<const uint32_t*>(row)[at];
+    else
+      e[q] = reinterpret_cast<const uint16_t*>(row)[at];
+  }
+#pragma unroll
+  for (int q = 0; q < n; q++)
+    if (j + q >= V) e[q] = Type<DT>::kMasked & (DT == DTL_F32 ? ~0u : 0xffffu);
+#pragma unroll
+  for (int q = 0; q < 4; q++) p[q] = DT == DTL_F32 ? e[q % n] : e[2 * q % n] | e[(2 * q + 1) % n] << 16;
+  return p;
+}
+
 // Past the caches or not.  The two stores are kept apart: the compiler would make one
 // of them, without the hint.
-template <typename M>
-__device__ __forceinline__ void store_packet(M* to, const packet& p, bool past) {
+template <int DT>
+__device__ __forceinline__ void store_packet(char* at, const packet& p, bool past) {
+  typename Type<DT>::mem* to = reinterpret_cast<typename Type<DT>::mem*>(at);
   if (past) {
     asm volatile("");
     __builtin_nontemporal_store(p, to);
