@@ -429,7 +429,7 @@ def _once(backward):
 class _Adjust(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, z, by):
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = logits.new_empty(logits.shape)
         _adjust(z, by, out, z.vocab, logits.device)
         history, rows, allowed = by.for_backward()
         # without repetitions a logit's sign does not matter, only where it is
@@ -487,7 +487,7 @@ def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = Non
     if out is None:
         if grad:
             return _Adjust.apply(logits, z, by)
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = logits.new_empty(logits.shape)
         _adjust(z, by, out, z.vocab, logits.device)
         return out
     if grad or out.requires_grad and torch.is_grad_enabled():

@@ -71,7 +71,7 @@ def _token_ids(tokens, device) -> torch.Tensor:
 
 def _lookup(weight, tokens, scale):
     t = _table(weight, "weight")
-    out = torch.empty((*tokens.shape, t.width), dtype=weight.dtype, device=weight.device)
+    out = weight.new_empty((*tokens.shape, t.width))
     _call(weight.device, lib.dtl_embedding, C.byref(t), _ptr(tokens), tokens.element_size(), tokens.numel(), scale,
           _ptr(out), t.width)
     return out
@@ -131,7 +131,7 @@ def embedding_grad(tokens: torch.Tensor, grad: torch.Tensor, vocab: Optional[int
     if out is None:
         if vocab is None or add:
             raise ValueError("embedding_grad needs a vocab or an out, and out for add")
-        out = torch.empty((vocab, grad.shape[-1]), dtype=grad.dtype, device=grad.device)
+        out = grad.new_empty((vocab, grad.shape[-1]))
         return _gradient(tokens, grad, float(scale), out, False)
     _need_floats(out, "out")
     if out.requires_grad and torch.is_grad_enabled():
