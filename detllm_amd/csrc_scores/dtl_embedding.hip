@@ -614,7 +614,7 @@ struct Layout {  // of the scratch
 };
 Layout layout_of(size_t n, size_t width) {
   Layout l{};
-  // us for both digits of 74894 tokens by tiles of 1024 / 2048 / 3072 28 / 26 / 29; of
+  // us for both digits of 74894 tokens by tiles of 1024 / 2048 28 / 26; of
   // 500000 by 4096 / 8192 46 / 57
   const size_t per = n <= 65536 ? 1024 : n <= 131072 ? 2048 : (n + kTiles - 1) / kTiles;
   l.tile = (uint32_t)((per + kSortThreads - 1) / kSortThreads * kSortThreads);

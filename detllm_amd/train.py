@@ -5,7 +5,8 @@ For programs that distil into a model of their own with scores.distill_loss: wha
 comes before its first layer and after its last gradient.  The calls enqueue the
 library's kernels (dtl_embedding*, dtl_grad_norm, dtl_clip_grads of
 include/detllm.h, which define every result) on the current stream of the tensors'
-device, do not wait, and can be captured into a graph, as those of scores.py.
+device, do not wait, and can be captured into a graph, as those of scores.py (a
+captured backward needs a leaf of its own, `weight.detach().requires_grad_()`).
 Reverse mode only.
 
     hidden = train.embedding(weight, tokens, scale=weight.shape[1] ** 0.5)

@@ -411,14 +411,15 @@ typedef struct dtl_adjust {
 /* Writes the adjusted logits (their type, row i at out + i * out_stride elements;
  * may be the logits themselves at the same stride, or lie between their rows, but
  * not over a part of them).  Formed in 32 bits and rounded once; what passes a
- * range there is infinite (the lowest float times a repetition, say). */
+ * range there is infinite (the lowest float times a repetition, say).  The arrays of
+ * `by` lie apart from out. */
 int dtl_adjust_logits(const dtl_logits *logits, const dtl_adjust *by, void *out, size_t out_stride,
                       void *stream);
 /* From the gradient of the adjusted logits (their type and shape, row i at
  * grad_out + i * grad_out_stride) that of the logits: times 1 / repetition or
  * repetition where a token stood in the history, 0 where a logit is not allowed,
  * whatever grad_out holds there.  grad may be grad_out itself at the same stride,
- * but lie over no part of the logits. */
+ * but lies over no part of the logits or of the arrays of `by`. */
 int dtl_adjust_logits_backward(const dtl_logits *logits, const dtl_adjust *by, const void *grad_out,
                                size_t grad_out_stride, void *grad, size_t grad_stride, void *stream);
 
