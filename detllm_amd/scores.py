@@ -341,7 +341,10 @@ class _By:
             history, n, a.history_stride = self.rows(history, _INDEX, "history")
             a.history, a.history_bytes, a.history_len = history.data_ptr(), history.element_size(), n
             if prompt is not None:
-                prompt = self.tensor(prompt, _INDEX, "prompt", self.lead).int().contiguous()
+                prompt = self.tensor(prompt, _INDEX, "prompt", self.lead)
+                if prompt.dtype == torch.int64:  # a place past 32 bits stays behind the history's last
+                    prompt = prompt.clamp(0, n).int()
+                prompt = prompt.contiguous()
                 a.prompt = prompt.data_ptr()
         elif prompt is not None:
             raise ValueError("prompt counts places of a history")
