@@ -211,6 +211,7 @@ def _adjust(n, vocab, history, prompt, repetition, presence, frequency, bias_ids
         x, a.history = held(history, np.int64, lists(history, "history"), "history")
         a.history_bytes, a.history_len, a.history_stride = 8, x.shape[-1], x.shape[-1] if x.ndim > 1 else 0
         if prompt is not None:
+            prompt = np.clip(prompt, 0, a.history_len)  # before it is narrowed
             a.prompt = held(np.broadcast_to(prompt, (n,)), np.int32, [(n,)], "prompt")[1]
     elif prompt is not None:
         raise ValueError("prompt counts places of a history")
