@@ -198,6 +198,12 @@ def _adjust(n, vocab, history, prompt, repetition, presence, frequency, bias_ids
         keep.append(x)
         return x, (x.ctypes.data if x.size else None)
 
+    def whole(x, name):
+        x = np.asarray(x)
+        if x.size and x.dtype.kind not in "iu":
+            raise TypeError(f"{name} must be whole numbers of at most 64 bits")
+        return x
+
     def rows(x, name):
         if np.ndim(x) == 0:
             return float(x), None
@@ -208,10 +214,10 @@ def _adjust(n, vocab, history, prompt, repetition, presence, frequency, bias_ids
         return [(n, k), (k,)]
 
     if history is not None:
-        x, a.history = held(history, np.int64, lists(history, "history"), "history")
+        x, a.history = held(whole(history, "history"), np.int64, lists(history, "history"), "history")
         a.history_bytes, a.history_len, a.history_stride = 8, x.shape[-1], x.shape[-1] if x.ndim > 1 else 0
         if prompt is not None:
-            prompt = np.clip(prompt, 0, a.history_len)  # before it is narrowed
+            prompt = np.clip(whole(prompt, "prompt"), 0, a.history_len)  # before it is narrowed
             a.prompt = held(np.broadcast_to(prompt, (n,)), np.int32, [(n,)], "prompt")[1]
     elif prompt is not None:
         raise ValueError("prompt counts places of a history")
@@ -221,7 +227,7 @@ def _adjust(n, vocab, history, prompt, repetition, presence, frequency, bias_ids
     if (bias_ids is None) != (bias is None):
         raise ValueError("bias_ids and bias belong together")
     if bias is not None:
-        x, a.bias_ids = held(bias_ids, np.int64, lists(bias_ids, "bias_ids"), "bias_ids")
+        x, a.bias_ids = held(whole(bias_ids, "bias_ids"), np.int64, lists(bias_ids, "bias_ids"), "bias_ids")
         a.biases = held(bias, np.float32, [x.shape], "bias")[1]
         a.bias_bytes, a.bias_len, a.bias_stride = 8, x.shape[-1], x.shape[-1] if x.ndim > 1 else 0
     if allowed is not None:
