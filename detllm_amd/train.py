@@ -126,6 +126,8 @@ def embedding_grad(tokens: torch.Tensor, grad: torch.Tensor, vocab: Optional[int
     ([vocab, width], of grad's type or float32); with add, on top of what it holds (an
     output matrix that shares its weight, say), its other rows left alone."""
     _need_floats(grad, "grad")
+    if grad.requires_grad and torch.is_grad_enabled():
+        raise ValueError("grad is a constant to autograd: detach it")
     tokens = _token_ids(tokens, grad.device)
     if not grad.dim() or grad.shape[:-1] != tokens.shape:
         raise ValueError(f"grad has shape {tuple(grad.shape)}, expected {(*tokens.shape, 'width')}")

@@ -1,0 +1,11 @@
+"""detllm_amd.train over the ranges of its arguments, on torch tensors, in processes of
+their own: torch has a HIP runtime of its own, which the library shares only where
+torch is loaded first."""
+import pytest
+
+from test_gpu_adjust import run_apart
+
+
+@pytest.mark.gpu
+def test_constants():
+    run_apart("torch_constants.py")

@@ -1,0 +1,24 @@
+"""Calls of detllm_amd.train that autograd does not see refuse what needs a gradient,
+whose result would be cut off without a word.  Run by test_gpu_train_forms.py in a
+process of its own."""
+import pytest
+import torch  # first: the library shares its HIP runtime
+
+from detllm_amd import train
+
+pytestmark = pytest.mark.gpu
+
+
+def test_rows_of_an_embedding_gradient():
+    g = torch.randn(5, 6, device="cuda")
+    tokens = torch.tensor([1, 0, 3, 1, -1], device="cuda")
+    want = train.embedding_grad(tokens, g, 4)
+    leaf = g.clone().requires_grad_()
+    for x in (leaf, leaf * 1):
+        for kw in ({}, dict(out=torch.zeros(4, 6, device="cuda")), dict(out=torch.zeros(4, 6, device="cuda"), add=True)):
+            with pytest.raises(ValueError, match="grad is a constant"):
+                train.embedding_grad(tokens, x, 4, **kw)
+        assert torch.equal(train.embedding_grad(tokens, x.detach(), 4), want)
+        for mode in (torch.no_grad, torch.inference_mode):  # where nothing is recorded
+            with mode():
+                assert torch.equal(train.embedding_grad(tokens, x, 4), want)
