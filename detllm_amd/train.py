@@ -222,6 +222,8 @@ def _norm(grads, norm_type, scale, max_norm=None, out=None):
         if scale.dtype != torch.float32 or scale.numel() != 1 or scale.device != device:
             raise ValueError("scale must be a number or one float32 on the gradients' device")
         _no_tangent(scale, "scale")
+        if scale.requires_grad and torch.is_grad_enabled():
+            raise ValueError("scale is a constant to autograd: detach it")
         at, scale = scale.data_ptr(), 0.0
     written = grads
     to = None

@@ -22,3 +22,23 @@ def test_rows_of_an_embedding_gradient():
         for mode in (torch.no_grad, torch.inference_mode):  # where nothing is recorded
             with mode():
                 assert torch.equal(train.embedding_grad(tokens, x, 4), want)
+
+
+def test_a_scale():
+    grads = [torch.randn(50, device="cuda"), torch.randn(7, device="cuda").bfloat16()]
+    scale = torch.tensor(0.25, device="cuda")
+    leaf = scale.clone().requires_grad_()
+    calls = (lambda s: train.grad_norm(grads, scale=s),
+             lambda s: train.clip_grad_norm(grads, 0.5, scale=s, out=[torch.empty_like(t) for t in grads]))
+    for call in calls:
+        want = call(scale)
+        for s in (leaf, leaf * 1):
+            with pytest.raises(ValueError, match="scale is a constant"):
+                call(s)
+            assert torch.equal(call(s.detach()), want)
+            with torch.no_grad():
+                assert torch.equal(call(s), want)
+    before = [t.clone() for t in grads]
+    with pytest.raises(ValueError):
+        train.clip_grad_norm(grads, 0.5, scale=leaf)
+    assert all(torch.equal(a, b) for a, b in zip(grads, before))
