@@ -214,9 +214,11 @@ def _norm(grads, norm_type, scale, max_norm=None, out=None):
     grads, table = _tensor_list(grads, "grads")
     if norm_type not in (2, math.inf):
         raise ValueError("norm_type must be 2 or inf")
-    if not grads:
-        return torch.zeros(())
-    device = grads[0].device
+    if grads:
+        beside = grads[0]
+    else:  # the scale's device, or the current one
+        beside = torch.empty(0, device=scale.device if isinstance(scale, torch.Tensor) and scale.is_cuda else "cuda")
+    device = beside.device
     at = None
     if isinstance(scale, torch.Tensor):
         if scale.dtype != torch.float32 or scale.numel() != 1 or scale.device != device:
@@ -242,9 +244,9 @@ def _norm(grads, norm_type, scale, max_norm=None, out=None):
                 if o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()):
                     raise ValueError("out must have the gradients' strides")
     address = table.buffer_info()[0]
-    norm = grads[0].new_empty((), dtype=torch.float32)
+    norm = beside.new_empty((), dtype=torch.float32)
     need = lib.dtl_grad_norm_scratch(address, len(grads))
-    scratch = grads[0].new_empty(need, dtype=torch.uint8)
+    scratch = beside.new_empty(need, dtype=torch.uint8)
     kind = int(norm_type == math.inf)
     if max_norm is None:
         _call(device, lib.dtl_grad_norm, address, len(grads), kind, scale, at, _ptr(norm), _ptr(scratch), need)

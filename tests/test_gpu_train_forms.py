@@ -9,3 +9,8 @@ from test_gpu_adjust import run_apart
 @pytest.mark.gpu
 def test_constants():
     run_apart("torch_constants.py")
+
+
+@pytest.mark.gpu
+def test_lists_without_elements():
+    run_apart("torch_no_gradients.py")
