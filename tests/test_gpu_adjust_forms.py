@@ -13,3 +13,8 @@ def test_prompts():
 
 def test_prompts_without_a_gpu():
     run_apart("torch_adjust_prompts.py", "-m", "not gpu")
+
+
+@pytest.mark.gpu
+def test_every_kernel():
+    run_apart("torch_adjust_kernels.py")
