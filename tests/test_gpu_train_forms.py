@@ -14,3 +14,8 @@ def test_constants():
 @pytest.mark.gpu
 def test_lists_without_elements():
     run_apart("torch_no_gradients.py")
+
+
+@pytest.mark.gpu
+def test_long_runs_of_a_token():
+    run_apart("torch_embedding_runs.py")
