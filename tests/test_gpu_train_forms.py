@@ -19,3 +19,8 @@ def test_lists_without_elements():
 @pytest.mark.gpu
 def test_long_runs_of_a_token():
     run_apart("torch_embedding_runs.py")
+
+
+@pytest.mark.gpu
+def test_large_lists_and_norms():
+    run_apart("torch_clip_large.py")
