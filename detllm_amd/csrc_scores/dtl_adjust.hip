@@ -251,11 +251,10 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
   }
 }
 
-template <int DT, int MODE, int SEG, int THREADS>
-void launch_as(AdjustK& k, size_t rows, bool table, hipStream_t s) {
+template <int DT, int MODE, bool TABLE, int SEG, int THREADS>
+void launch_as(AdjustK& k, size_t rows, hipStream_t s) {
   k.nseg = (k.V + SEG - 1) / SEG;
-  launch_rows(table ? k_adjust<DT, MODE, true, SEG, THREADS> : k_adjust<DT, MODE, false, SEG, THREADS>, rows, k.nseg, THREADS,
-              0, s, k);
+  launch_rows(k_adjust<DT, MODE, TABLE, SEG, THREADS>, rows, k.nseg, THREADS, 0, s, k);
 }
 
 // A row's segments by its length and the history's.  us of 2048 logits by four waves /
@@ -267,11 +266,11 @@ void launch_as(AdjustK& k, size_t rows, bool table, hipStream_t s) {
 template <int DT, int MODE>
 void launch_mode(AdjustK& k, size_t rows, bool table, hipStream_t s) {
   if (k.V <= 4096 || (rows * k.V < (1u << 21) && k.history_len <= 1024))
-    launch_as<DT, MODE, 2048, 256>(k, rows, table, s);
-  else if (k.history_len > 4096)
-    launch_as<DT, MODE, 16384, 1024>(k, rows, table, s);
+    by_bool(table, [&](auto t) { launch_as<DT, MODE, decltype(t)::value, 2048, 256>(k, rows, s); });
+  else if (k.history_len > 4096)  // of which there is a table
+    launch_as<DT, MODE, true, 16384, 1024>(k, rows, s);
   else
-    launch_as<DT, MODE, 8192, 512>(k, rows, table, s);
+    by_bool(table, [&](auto t) { launch_as<DT, MODE, decltype(t)::value, 8192, 512>(k, rows, s); });
 }
 
 }  // namespace
