@@ -149,7 +149,7 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
     __syncthreads();
     if (a.bias_len) {
       auto place = [&](long id, int k) {
-        const uint64_t j = (uint64_t)(id - base);
+        const uint64_t j = (uint64_t)id - (uint64_t)base;
         if (j < (uint64_t)(end - base)) atomicMax(table + j, (uint32_t)k + 1);
       };
       place(bias_id, tid);
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(kThreads) void k_adjust(AdjustK a) {
     }
     if (a.history_len) {
       auto count = [&](long id, int at) {
-        const uint64_t j = (uint64_t)(id - base);
+        const uint64_t j = (uint64_t)id - (uint64_t)base;
         if (j >= (uint64_t)(end - base)) return;
         if (at < prompt)
           atomicOr(table + j, kInPrompt);

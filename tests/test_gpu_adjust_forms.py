@@ -18,3 +18,8 @@ def test_prompts_without_a_gpu():
 @pytest.mark.gpu
 def test_every_kernel():
     run_apart("torch_adjust_kernels.py")
+
+
+@pytest.mark.gpu
+def test_ids():
+    run_apart("torch_ids.py")
