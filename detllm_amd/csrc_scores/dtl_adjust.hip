@@ -258,11 +258,12 @@ void launch_as(AdjustK& k, size_t rows, hipStream_t s) {
 }
 
 // A row's segments by its length and the history's.  us of 2048 logits by four waves /
-// 8192 by eight / 16384 by sixteen: 16384 rows of 1000 bf16 24 / 46 / 93, 8192 of 2500
-// 36 / 43 / 65; histories of 200, 16 rows of 32000 3.9 / 4.7 / 5.4; of 2048, 64 rows of
-// 151936 - / 11.7 / 12.7; of 8192, 512 such rows 345 / 139 / 110; of 32768, 8 of them 42 /
-// 25 / 17.  Segments of 8192 by four or sixteen waves: 2048 rows of 151936 f32 524 / 452,
-// eight 456; 4096 of bf16 514 / 545, eight 429.
+// 8192 by eight / 16384 by sixteen: 16384 rows of 1000 bf16 25 / 52 / 101, 8192 of 2500
+// 37 / 42 / 65; histories of 200, 16 rows of 32000 3.9 / 4.6 / 5.4; of 2048, 64 rows of
+// 151936 15.2 / 11.6 / 12.7; of 8192, 512 such rows 207 / 108 / 103; of 32768, 64 of them
+// 80 / 33 / 27, 8 of them 17.3 / 11.5 / 12.1.  Segments of 8192 by four / eight / sixteen
+// waves: 2048 rows of 151936 f32 478 / 436 / 470; 4096 of bf16 418 / 417 / 573, their
+// gradients 527 / 464 / 633.
 template <int DT, int MODE>
 void launch_mode(AdjustK& k, size_t rows, bool table, hipStream_t s) {
   if (k.V <= 4096 || (rows * k.V < (1u << 21) && k.history_len <= 1024))

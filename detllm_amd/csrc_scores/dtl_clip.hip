@@ -6,8 +6,9 @@
 // factor is known only when every element has been read.  A launch takes a table of
 // tensors as its argument (nothing to upload, nothing that a captured graph could lose),
 // each workgroup a piece of one of them.  Squares and sums are in 64 bits: a gradient of
-// 1e20 has a norm, one of 1e-30 too, and the sum does not depend on how it is cut.  The
-// pieces' sums are joined by one workgroup in a fixed order.
+// 1e20 has a norm, one of 1e-30 too.  The pieces' sums are joined by one workgroup in a
+// fixed order: the same list gives the same bits; the same elements cut otherwise differ by
+// some 2^-53 of the sum, far below the norm's rounding to 32 bits.
 #include "dtl_scores.h"
 
 #include <algorithm>
@@ -21,12 +22,12 @@ namespace {
 
 constexpr int kThreads = 256, kJoinThreads = 1024;
 // Elements a workgroup reads for the norm, and scales.  us for 201 bf16 tensors of 1.1e9
-// elements: norm by 16384 / 32768 332 / 338, but 31 / 17 to join twice the pieces; clipping
-// by 8192 / 16384 / 32768 769 / 795 / 804.
+// elements: norm by 16384 / 32768 328 / 325, and 10 / 6.5 to join the pieces; clipping by
+// 8192 / 16384 / 32768 757 / 792 / 808.
 constexpr size_t kPiece = 32768, kClipPiece = 8192;
 // Workgroups of a clipping in place at most: with a factor of 1 there is nothing to do, and
-// ending the 133000 of 201 bf16 tensors takes 90 us longer; with another one their pieces
-// one after the other take 1180 us instead of 1140.
+// 201 bf16 tensors of 133000 pieces take 347 us in all instead of the 368 of a workgroup a
+// piece; with another one their pieces one after the other take 1175 instead of 1144.
 constexpr uint32_t kInPlaceGroups = 16384;
 constexpr size_t kCache = (size_t)256 << 20, kKept = (size_t)192 << 20;
 constexpr int kNormEntries = 180, kClipEntries = 128;
@@ -343,8 +344,8 @@ int norm_and_clip(const dtl_tensor* t, size_t n, int largest, float scale, const
   k.part = reinterpret_cast<double*>(static_cast<char*>(scratch) + 16);
   // More than the memory-side cache holds is read past it, but for what the clipping,
   // which goes backwards and writes past it, will still find there (kKept; us for norm and
-  // clipping, 0 / 128 / 192 MB kept: 201 bf16 tensors of 2.2 GB 1091 / 1108 / 1076, cached
-  // throughout 1219; 392 MB of f16 to f32 265 / 285 / 249).
+  // clipping, 0 / 128 / 192 MB kept: 201 bf16 tensors of 2.2 GB 1098 / 1087 / 1086, cached
+  // throughout 1125; 392 MB of f16 to f32 264 / 260 / 253, cached throughout 259).
   size_t bytes = 0;
   for (size_t i = 0; i < n; i++) bytes += t[i].count * type_bytes(t[i].dtype);
   if (bytes > kCache) {

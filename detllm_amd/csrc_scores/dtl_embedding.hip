@@ -584,8 +584,8 @@ __global__ __launch_bounds__(kThreads) void k_embedding_join(SumK a) {
 
 // What does not fit the memory-side cache together with what it is made of is written
 // past it, so that what is read beside it stays.  One pass of lookup and gradient, us,
-// past / not: 65536 bf16 rows of 2048 into 32000 161 / 223, 16384 of 896 into 151936
-// 80 / 88, 8192 f32 rows of 2048 into 32000 95 / 108; where it fits (2048 f32 rows of 576
+// past / not: 65536 bf16 rows of 2048 into 32000 167 / 208, 16384 of 896 into 151936
+// 80 / 86, 8192 f32 rows of 2048 into 32000 94 / 102; where it fits (2048 f32 rows of 576
 // into 49152) 37 / 30.
 bool past_caches(size_t bytes) { return bytes > (size_t)256 << 20; }
 
@@ -614,8 +614,8 @@ struct Layout {  // of the scratch
 };
 Layout layout_of(size_t n, size_t width) {
   Layout l{};
-  // us for both digits of 74894 tokens by tiles of 1024 / 2048 28 / 26; of
-  // 500000 by 4096 / 8192 46 / 57
+  // us for both digits of 74894 tokens by tiles of 1024 / 2048 24 / 24; of
+  // 500000 by 4096 / 8192 41 / 54
   const size_t per = n <= 65536 ? 1024 : n <= 131072 ? 2048 : (n + kTiles - 1) / kTiles;
   l.tile = (uint32_t)((per + kSortThreads - 1) / kSortThreads * kSortThreads);
   l.tiles = (int)((n + l.tile - 1) / (l.tile ? l.tile : 1));
@@ -761,7 +761,7 @@ int dtl_embedding_backward(const void* tokens, int token_bytes, size_t n, const 
   }
   if (n <= (size_t)kAlone) {
     // us, zeros aside: 7 to 200 tokens 4 by counting, 9 by digits; 1000 5, 2118 8, 4096 11
-    // by digits, 8000 19 (16 and three more launches otherwise)
+    // by digits, 8000 19 (18 in four launches)
     launch_kernel(n <= kFew ? k_sort_few : k_sort_alone, dim3((unsigned)(1 + k.pieces)), dim3(kSortThreads), 0, s, k);
   } else {
     k.tiles = l.tiles;

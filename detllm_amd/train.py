@@ -122,9 +122,10 @@ def embedding(weight: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.0)
 def embedding_grad(tokens: torch.Tensor, grad: torch.Tensor, vocab: Optional[int] = None, *, scale: float = 1.0,
                    out: Optional[torch.Tensor] = None, add: bool = False) -> torch.Tensor:
     """dtl_embedding_backward: the gradient of embedding's weight for that of its rows,
-    grad[..., width], for loops that run their own backward pass.  out: where it goes
-    ([vocab, width], of grad's type or float32); with add, on top of what it holds (an
-    output matrix that shares its weight, say), its other rows left alone."""
+    grad[..., width] (a constant to autograd), for loops that run their own backward
+    pass.  out: where it goes ([vocab, width], of grad's type or float32); with add, on
+    top of what it holds (an output matrix that shares its weight, say), its other rows
+    left alone."""
     _need_floats(grad, "grad")
     if grad.requires_grad and torch.is_grad_enabled():
         raise ValueError("grad is a constant to autograd: detach it")
@@ -261,9 +262,10 @@ def grad_norm(grads: Union[torch.Tensor, Iterable[Optional[torch.Tensor]]], *, n
               scale: Union[float, torch.Tensor] = 1.0) -> torch.Tensor:
     """dtl_grad_norm: scale times the norm over all elements of the tensors (float32,
     bfloat16 or float16, mixed as they come; None is left out), on the device: the 2-norm,
-    summed in 64 bits, or with norm_type=inf the largest magnitude.  scale: what the
-    gradients are to be multiplied by (1 / the loss scale), a number or one float32 on
-    the device."""
+    summed in 64 bits, or with norm_type=inf the largest magnitude; 0 (on the scale's
+    device, or the current one) where there are no tensors.  scale: what the gradients
+    are to be multiplied by (1 / the loss scale), a number or one float32 on the device,
+    a constant to autograd as the gradients are."""
     return _norm(grads, norm_type, scale if isinstance(scale, torch.Tensor) else float(scale))
 
 

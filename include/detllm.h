@@ -472,8 +472,9 @@ int dtl_grad_norm(const dtl_tensor *tensors, size_t n, int largest, float scale,
  * 32-bit factor, the product rounded once: into `out` (n tensors of the same counts, of
  * the gradients' types or f32), or in place where out is NULL, where a factor of 1
  * writes nothing.  As the formula has it an infinite norm leaves zeros (NaN for
- * infinities), a NaN norm NaN.  out[i] may be tensors[i] itself; other overlaps are
- * refused. */
+ * infinities), a NaN norm NaN; finite elements whose norm passes the range of *norm are
+ * multiplied by the c of the norm in 64 bits.  out[i] may be tensors[i] itself; other
+ * overlaps are refused. */
 int dtl_clip_grads(const dtl_tensor *tensors, size_t n, int largest, float scale, const float *scale_at,
                    float max_norm, const dtl_tensor *out, float *norm, void *scratch,
                    size_t scratch_bytes, void *stream);
