@@ -1580,8 +1580,15 @@ int session_scores(dtl_session* s, size_t first, size_t n, const dtl_adjust* by,
   if (log_probs)
     for (size_t i = 0; i < n; i++)
       if (tokens[i] >= V) return DTL_ERR_CDF_SYMBOL_OUT_OF_RANGE;
-  if (by)
+  if (by) {
     if (const int st = check_adjust(by, n, V)) return st;
+    for (size_t i = 0; by->history_len && i < n; i++) {  // each row's as the single values
+      const float r = by->repetitions ? by->repetitions[i] : 1.0f;
+      if (!(r > 0.0f && r < __builtin_inff())) return DTL_ERR_INVALID_ARGUMENT;
+      for (const float* rows : {by->presences, by->frequencies})
+        if (rows && !(rows[i] - rows[i] == 0.0f)) return DTL_ERR_INVALID_ARGUMENT;
+    }
+  }
   HIP_TRY(hipSetDevice(s->m->device));
   // tokens, log probabilities, entropy, alternatives' ids and log
   // probabilities, then the scratch

@@ -383,7 +383,8 @@ int dtl_distill_step(const dtl_logits *logits, const dtl_teacher *teacher, float
  *            prompt's.  A token anywhere in it: z > 0 ? z / repetition :
  *            z * repetition.  One that stands n > 0 times behind the prompt: less
  *            presence + frequency * n.  repetitions, presences, frequencies
- *            ([rows] each, or NULL) are taken in place of the single values.
+ *            ([rows] each, or NULL) are taken in place of the single values; in device
+ *            memory their ranges are the caller's to keep.
  *   biases   bias_len (at most 4096) ids and what is added to their logits, row i
  *            at bias_ids + i * bias_stride and biases + i * bias_stride (0: every
  *            row's).  Of an id that occurs twice the later place counts; an id
