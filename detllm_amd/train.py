@@ -140,7 +140,7 @@ def embedding_grad(tokens: torch.Tensor, grad: torch.Tensor, vocab: Optional[int
     _need_floats(out, "out")
     if out.requires_grad and torch.is_grad_enabled():
         raise ValueError("out has no gradient")
-    if out.device != grad.device or out.dim() != 2 or out.shape != (vocab or out.shape[0], grad.shape[-1]):
+    if out.device != grad.device or out.dim() != 2 or out.shape != (out.shape[0] if vocab is None else vocab, grad.shape[-1]):
         raise ValueError("out must have grad's device and width, and the vocab")
     if out.dtype not in (grad.dtype, torch.float32):
         raise TypeError("out must have the type of grad, or be float32")

@@ -42,3 +42,12 @@ def test_a_scale():
     with pytest.raises(ValueError):
         train.clip_grad_norm(grads, 0.5, scale=leaf)
     assert all(torch.equal(a, b) for a, b in zip(grads, before))
+
+
+def test_a_vocabulary_beside_out():
+    g, tokens, out = torch.randn(3, 6, device="cuda"), torch.tensor([1, 0, 3], device="cuda"), torch.ones(4, 6, device="cuda")
+    for vocab in (0, 3, 5, -4):
+        with pytest.raises(ValueError):
+            train.embedding_grad(tokens, g, vocab, out=out)
+    assert (out == 1).all()
+    assert torch.equal(train.embedding_grad(tokens, g, 4, out=out.clone()), train.embedding_grad(tokens, g, out=out.clone()))
